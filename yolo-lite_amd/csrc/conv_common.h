@@ -19,19 +19,14 @@ __device__ __forceinline__ float silu_f(float v) {
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * v));
 #endif
 }
-// Four SiLUs with the three full-rate steps as PACKED fp32 instructions (v_pk_mul_f32 / v_pk_add_f32: two values per lane and
-// instruction; hipcc leaves adjacent scalar silu_f calls unpacked): 6 + 8 instructions per four values instead of 12 + 8, the
-// same IEEE operations on the same operands -- bit-identical to silu_f.  The fused small-channel kernels are bound by
-// instruction issue (NOTEBOOK section 13).
+// Four SiLUs as vector steps: the same IEEE operations on the same operands as silu_f, bit-identical to it.  (Written for packed
+// fp32 instructions, two values per lane; the build leaves those out -- Makefile, NOPK -- and each step is four scalar ones.)
 typedef __attribute__((ext_vector_type(4))) float silu_f32x4;
 __device__ __forceinline__ silu_f32x4 silu4(silu_f32x4 v) {
 #ifdef YL_ABL_NO_SILU
   return v;
 #else
-  // (the constants live in registers the compiler cannot see through: a packed instruction takes no 32-bit literal, and with a
-  // visible constant hipcc falls back to four scalar multiplies / adds)
-  float kc = -1.44269504088896340736f, one = 1.0f;
-  asm volatile("" : "+v"(kc), "+v"(one));
+  const float kc = -1.44269504088896340736f, one = 1.0f;
   const silu_f32x4 kv = {kc, kc, kc, kc}, ov = {one, one, one, one};
   const silu_f32x4 t = v * kv;
   silu_f32x4 e;

@@ -270,8 +270,8 @@ __global__ __launch_bounds__(256) void dwconv3_kernel(DwArgs a) {
       const int dx = min(t - 1, a.W - x0);
       v[kh][t] = *reinterpret_cast<const bf16x8*>(inb + ((kh - 1) * a.in.W1 + dx) * 8);
     }
-  // (round 5) channel PAIRS as two-element vectors: __builtin_elementwise_fma on them is ONE v_pk_fma_f32 per pair -- the same IEEE
-  // fused multiply-add on the same operands in the same order as 72 scalar v_fma_f32 per pixel, in half the instructions
+  // channel PAIRS as two-element vectors: the same IEEE fused multiply-adds on the same operands in the same order as 72 scalar
+  // v_fma_f32 per pixel (which is what the build makes of them: no packed fp32 instructions, Makefile, NOPK)
   typedef __attribute__((ext_vector_type(2))) float dw_f2;
   dw_f2 acc[DW_PX][4];
   {
