@@ -23,7 +23,7 @@ extern "C" {
 #define YL_ABI_VERSION 21
 
 /* element types */
-enum { YL_BF16 = 0, YL_F32 = 1, YL_F16 = 2, YL_U8 = 3, YL_FP8 = 4 /* OCP e4m3 */ };
+enum { YL_BF16 = 0, YL_F32 = 1, YL_F16 = 2, YL_U8 = 3, YL_FP8 = 4 /* OCP e4m3 */, YL_MX4 = 5 /* e2m1 in blocks of 32, one e8m0 scale each */ };
 
 /* op kinds of an engine program */
 enum {
@@ -342,6 +342,31 @@ int yl_preprocess_u8(const uint8_t* bgr_hwc, int batch, int h, int w, float* out
 int yl_letterbox_u8(const uint8_t* src_bgr_hwc, int src_h, int src_w, int src_pitch, uint8_t* dst_chw, int H,
                     int W, int top, int left, int new_h, int new_w, const int32_t* xtab, const int32_t* ytab,
                     void* stream);
+
+/* ---- 4-bit microscaled products (csrc/mx4.hip) -----------------------------------------------------------------------------
+ * MX4 = OCP microscaling with e2m1 elements: blocks of 32 consecutive columns share one scale byte s, which stands for 2^(s - 127).
+ * A matrix [rows][cols] is two arrays: codes[rows][ceil(cols / 32) * 16] (two 4-bit codes to a byte, the first in the low half;
+ * magnitudes 0, 1/2, 1, 3/2, 2, 3, 4, 6 for codes 0..7, sign in bit 3; 16-byte aligned) and scales[rows][ceil(cols / 32)]; the
+ * codes behind the last column are zeros.  The step below the e4m3 convs: a pointwise conv (nn/modules/conv.py:35-53 with k = 1,
+ * the projections of block.py:863-1038) is yl_mx4_linear over pixels as rows.  No counterpart in the reference.
+ *
+ * yl_mx4_quantize: x[rows][cols] (YL_BF16, YL_F16 or YL_F32; row stride in elements) -> codes, scales.  Per block the scale byte is
+ * max(E - 2, 0), E the biased fp32 exponent of the largest magnitude; elements round to nearest even and saturate at 6.  A block
+ * that holds an infinity or a NaN gets scale 255 and reads as NaN.
+ * yl_mx4_dequantize: the values the codes stand for (exact in bf16 and fp32; fp16 rounds and overflows as a conversion does). */
+int yl_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, uint8_t* codes, uint8_t* scales,
+                    void* stream);
+int yl_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* y, int y_dtype,
+                      int64_t y_stride, void* stream);
+/* y[rows][n] = act(x[rows][k] w[n][k]^T + bias[n]) (+ res[rows][n] after the activation, as in YL_OP_CONV): both operands in MX4,
+ * fp32 accumulation, act = 1: SiLU.  x: values (x_dtype YL_BF16 / YL_F16 / YL_F32, x_scales ignored), quantised by the call into
+ * `work`, or x_dtype = YL_MX4: codes with x_scales (x_stride ignored: codes and scales are dense).  bias fp32 or NULL; res has
+ * y's type, NULL: none; res may be y itself.  Strides in elements; y_dtype YL_BF16 / YL_F16 / YL_F32.  `work`: 16-byte aligned
+ * device scratch of yl_mx4_linear_workspace_bytes bytes (-1: the sizes are refused), not shared by calls that may overlap. */
+int64_t yl_mx4_linear_workspace_bytes(int x_dtype, int64_t rows, int64_t n, int64_t k);
+int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype, int64_t rows, int64_t x_stride, const uint8_t* w_codes,
+                  const uint8_t* w_scales, int64_t n, int64_t k, const float* bias, int act, const void* res, int64_t res_stride,
+                  void* y, int y_dtype, int64_t y_stride, void* work, int64_t work_bytes, void* stream);
 
 /* ---- multi-GPU exchange of the sharded path ---------------------------------
  * One process per GPU, weights replicated, images sharded; the ONLY exchanges are root -> ranks input slices and ranks ->

@@ -17,6 +17,10 @@ _LAZY = {
     "DetectionPredictor": ("engine.predictor", "DetectionPredictor"),
     "Results": ("engine.results", "Results"),
     "Boxes": ("engine.results", "Boxes"),
+    "Mx4Tensor": ("nn.mx4", "Mx4Tensor"),
+    "mx4_quantize": ("nn.mx4", "mx4_quantize"),
+    "mx4_dequantize": ("nn.mx4", "mx4_dequantize"),
+    "mx4_linear": ("nn.mx4", "mx4_linear"),
 }
 
 

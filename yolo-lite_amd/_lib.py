@@ -103,7 +103,7 @@ def xcc_census(stream, n_workgroups: int = 4096):
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ["YL_AMD_LIB"]) if os.environ.get("YL_AMD_LIB") else _PKG / "libyl_amd.so"  # dev override
 
-YL_BF16, YL_F32, YL_F16, YL_U8, YL_FP8 = 0, 1, 2, 3, 4
+YL_BF16, YL_F32, YL_F16, YL_U8, YL_FP8, YL_MX4 = 0, 1, 2, 3, 4, 5
 OP_CONV, OP_DWCONV3, OP_SPPF_POOL, OP_UPSAMPLE, OP_ATTENTION, OP_STEM = 1, 2, 3, 4, 5, 6
 
 EXPORTS = (  # include/yl_amd.h: the product ABI
@@ -113,7 +113,7 @@ EXPORTS = (  # include/yl_amd.h: the product ABI
     "yl_preprocess_u8", "yl_letterbox_u8", "yl_nms_ml_workspace_bytes", "yl_nms_ml", "yl_engine_profile_detect",
     "yl_engine_prefilter_fused", "yl_engine_detect_graph_prepare", "yl_graph_launch_many", "yl_engine_detect_graph_rebind",
     "yl_comm_get_unique_id", "yl_comm_create", "yl_comm_destroy", "yl_comm_rank", "yl_comm_world", "yl_comm_scatter",
-    "yl_comm_gather", "yl_comm_barrier",
+    "yl_comm_gather", "yl_comm_barrier", "yl_mx4_quantize", "yl_mx4_dequantize", "yl_mx4_linear_workspace_bytes", "yl_mx4_linear",
 )
 COMM_ID_BYTES = 128  # YL_COMM_ID_BYTES
 DIAG_EXPORTS = (  # include/yl_amd_diag.h: probes for tools/ and the runtime self-checks, not part of the product ABI
@@ -260,6 +260,14 @@ def lib() -> C.CDLL:
         f.argtypes = [vp, vp, vp, i64, i32, vp]
     L.yl_comm_barrier.restype = i32
     L.yl_comm_barrier.argtypes = [vp, vp]
+    L.yl_mx4_quantize.restype = i32
+    L.yl_mx4_quantize.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
+    L.yl_mx4_dequantize.restype = i32
+    L.yl_mx4_dequantize.argtypes = [vp, vp, i64, i64, vp, i32, i64, vp]
+    L.yl_mx4_linear_workspace_bytes.restype = i64
+    L.yl_mx4_linear_workspace_bytes.argtypes = [i32, i64, i64, i64]
+    L.yl_mx4_linear.restype = i32
+    L.yl_mx4_linear.argtypes = [vp, vp, i32, i64, i64, vp, vp, i64, i64, vp, i32, vp, i64, vp, i32, i64, vp, i64, vp]
     if L.yl_abi_version() != 21:
         raise RuntimeError("libyl_amd.so ABI version mismatch; rebuild it")
     _lib = L

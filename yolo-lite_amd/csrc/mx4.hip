@@ -1,0 +1,341 @@
+// MX4: 4-bit microscaled floating point (OCP microscaling: e2m1 elements, one e8m0 scale per 32 columns) -- quantisation, its
+// inverse, and the product y = act(x w^T + bias) [+ res] on v_mfma_scale_f32_16x16x128_f8f6f4, which multiplies the block scales
+// in.  The step below the e4m3 convs (conv_f8.hip): a pointwise conv IS such a product over pixels.
+//
+// One block of 32 values v:  E = biased exponent of the largest |v|,  scale byte s = max(E - 2, 0),  X = 2^(s - 127),
+// code = e2m1(v / X): magnitudes 0, 1/2, 1, 3/2, 2, 3, 4, 6 (codes 0..7), sign in bit 3, round to nearest even, saturating at 6
+// (|v| / X < 8: a value in (7, 8) loses up to a quarter -- the definition's choice of the scale).  v / X is exact (a power of
+// two), so the rounding to the code is the only one.  A block with a value that is not finite gets s = 255 and reads as NaN.
+//
+// Storage: codes[rows][ceil(cols / 32) * 16] bytes, two codes to a byte, the first in the low half; scales[rows][ceil(cols / 32)].
+// Columns behind the last are zeros.  An MFMA operand of 16 rows x 128 columns is then, per lane (row = lane & 15, block
+// g = lane >> 4), one aligned 16-byte load of codes and one scale byte: nothing is rearranged between memory and the pipe.
+#include <type_traits>
+
+#include "conv_common.h"
+
+namespace yl {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+
+// ------------------------------------------------------------------------------------------------ element access
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  return (float)v;
+}
+// eight values from p, the ones from `n` on as zeros; VEC: p is 16-byte aligned and all eight are there
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = a[j];
+        v[4 + j] = b[j];
+      }
+    } else {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      const t8 a = *reinterpret_cast<const t8*>(p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = (float)a[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<f32x4*>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
+      reinterpret_cast<f32x4*>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+      typedef T t8 __attribute__((ext_vector_type(8)));
+      *reinterpret_cast<t8*>(p) = t8{(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)v[4], (T)v[5], (T)v[6], (T)v[7]};
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = (T)v[j];
+  }
+}
+
+// the other lanes of a group of four: max over the 32 values of a block
+__device__ __forceinline__ unsigned quad_max(unsigned m) {
+  unsigned o = (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xF, 0xF, true);  // lanes 1 0 3 2
+  m = m > o ? m : o;
+  o = (unsigned)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xF, 0xF, true);  // lanes 2 3 0 1
+  return m > o ? m : o;
+}
+
+// Four lanes hold a block, eight values each: -> this lane's eight codes (4 bytes), the block's scale byte.
+__device__ __forceinline__ unsigned quantize8(const float (&v)[8], unsigned* scale_byte) {
+  unsigned m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned b = __float_as_uint(v[j]) & 0x7FFFFFFFu;  // |v|, ordered as an integer; inf and NaN are the largest
+    m = m > b ? m : b;
+  }
+  m = quad_max(m);
+  const unsigned e = m >> 23;
+  const unsigned s = e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+  const float x = __uint_as_float(s ? s << 23 : 0x00400000u);
+  unsigned c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], x, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], x, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], x, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], x, 3);
+  *scale_byte = s;
+  return c;
+}
+
+// the float 2^(s - 127); NaN for 255.  (2^-127 is not a normal number: its own bit pattern.)
+__device__ __forceinline__ float scale_value(unsigned s) {
+  return __uint_as_float(s == 0 ? 0x00400000u : (s == 255u ? 0x7FC00000u : s << 23));
+}
+
+// item = (row, group of eight columns) of a [rows][per_row] list; one division per thread, in 64 bits only where the list needs it
+struct Item {
+  long long row;
+  int c8;
+};
+__device__ __forceinline__ Item item_of(unsigned long long i, unsigned per_row) {
+  Item t;
+  if (i <= 0xFFFFFFFFull) {
+    const unsigned q = (unsigned)i / per_row;
+    t.row = q;
+    t.c8 = (int)((unsigned)i - q * per_row);
+  } else {
+    t.row = (long long)(i / per_row);
+    t.c8 = (int)(i - (unsigned long long)t.row * per_row);
+  }
+  return t;
+}
+
+struct QuantArgs {
+  const void* x;
+  long long rows, stride;  // stride in elements
+  int cols, kb;            // blocks per row
+  int vec;                 // every group of eight starts on 16 bytes
+  uint8_t* codes;
+  uint8_t* scales;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(QuantArgs a) {
+  const unsigned per_row = 4u * (unsigned)a.kb;
+  const unsigned long long i = (unsigned long long)blockIdx.x * 256u + threadIdx.x;
+  if (i >= (unsigned long long)a.rows * per_row) return;  // (whole groups of four lanes: the list's length is a multiple of 4)
+  const Item t = item_of(i, per_row);
+  float v[8];
+  load8(static_cast<const T*>(a.x) + t.row * a.stride + t.c8 * 8, a.cols - t.c8 * 8, a.vec, v);
+  unsigned s;
+  const unsigned c = quantize8(v, &s);
+  reinterpret_cast<unsigned*>(a.codes)[i] = c;
+  if ((t.c8 & 3) == 0) a.scales[t.row * a.kb + (t.c8 >> 2)] = (uint8_t)s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(QuantArgs a, T* y) {
+  const unsigned per_row = 4u * (unsigned)a.kb;
+  const unsigned long long i = (unsigned long long)blockIdx.x * 256u + threadIdx.x;
+  if (i >= (unsigned long long)a.rows * per_row) return;
+  const Item t = item_of(i, per_row);
+  const unsigned c = reinterpret_cast<const unsigned*>(a.codes)[i];
+  const float x = scale_value(a.scales[t.row * a.kb + (t.c8 >> 2)]);
+  float v[8];
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+  const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+  v[0] = p0[0] * x, v[1] = p0[1] * x, v[2] = p1[0] * x, v[3] = p1[1] * x;
+  v[4] = p2[0] * x, v[5] = p2[1] * x, v[6] = p3[0] * x, v[7] = p3[1] * x;
+  store8(y + t.row * a.stride + t.c8 * 8, a.cols - t.c8 * 8, a.vec, v);
+}
+
+// ------------------------------------------------------------------------------------------------ product
+struct LinearArgs {
+  const uint8_t *xc, *xs;  // activations: codes, scales
+  const uint8_t *wc, *ws;  // weight
+  long long rows;
+  int n, k, kb;
+  const float* bias;
+  const void* res;
+  long long res_stride;
+  void* y;
+  long long y_stride;
+  int act;
+};
+
+__device__ __forceinline__ v8i widen(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
+
+// y[m][n .. n + 4) = epilogue of four accumulators
+template <typename T>
+__device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 acc, long long m, int n) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (n + r >= a.n) break;
+    float v = acc[r];
+    if (a.bias) v += a.bias[n + r];
+    if (a.act) v = silu_f(v);
+    if (a.res) v += (float)static_cast<const T*>(a.res)[m * a.res_stride + n + r];
+    static_cast<T*>(a.y)[m * a.y_stride + n + r] = (T)v;
+  }
+}
+
+// One wave: 16 weight rows (operand A) x 16 activation rows (operand B), operands straight from memory.
+template <typename T>
+__global__ __launch_bounds__(64) void mx4_product_kernel(LinearArgs a, int ntiles) {
+  const int lane = threadIdx.x, g = lane >> 4, r = lane & 15;
+  const int n0 = (int)(blockIdx.x % (unsigned)ntiles) * 16;
+  const long long m0 = (long long)(blockIdx.x / (unsigned)ntiles) * 16;
+  const bool okn = n0 + r < a.n, okm = m0 + r < a.rows;
+  const long long wr = okn ? n0 + r : 0, xr = okm ? m0 + r : 0;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int b0 = 0; b0 < a.kb; b0 += 4) {
+    const int b = b0 + g;
+    v4i wv = {0, 0, 0, 0}, xv = {0, 0, 0, 0};
+    int sw = 127, sx = 127;
+    if (b < a.kb) {
+      if (okn) {
+        wv = *reinterpret_cast<const v4i*>(a.wc + (wr * a.kb + b) * 16);
+        sw = a.ws[wr * a.kb + b];
+      }
+      if (okm) {
+        xv = *reinterpret_cast<const v4i*>(a.xc + (xr * a.kb + b) * 16);
+        sx = a.xs[xr * a.kb + b];
+      }
+    }
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(wv), widen(xv), acc, 4, 4, 0, sw, 0, sx);
+  }
+  if (okm) finish4<T>(a, acc, m0 + r, n0 + 4 * g);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static int elem_bytes(int dtype) { return dtype == YL_F32 ? 4 : 2; }
+static bool value_type(int dtype) { return dtype == YL_BF16 || dtype == YL_F16 || dtype == YL_F32; }
+
+// the shape checks the entry points share; `who` names the call in the message
+static int check_matrix(const char* who, long long rows, long long cols, long long stride) {
+  if (rows < 0 || cols < 1) return fail(-1, std::string(who) + ": rows >= 0 and columns >= 1 are needed");
+  if (cols > (1LL << 22)) return fail(-3, std::string(who) + ": more than 4194304 columns");
+  if (rows > (1LL << 40) / ((cols + 31) / 32)) return fail(-3, std::string(who) + ": more than 2^40 blocks");
+  if (rows > 1 && stride < cols) return fail(-1, std::string(who) + ": the row stride is smaller than a row");
+  return 0;
+}
+
+template <typename F>
+static int by_type(int dtype, F f) {
+  if (dtype == YL_BF16) return f((__bf16*)nullptr);
+  if (dtype == YL_F16) return f((_Float16*)nullptr);
+  return f((float*)nullptr);
+}
+
+static int grid_of(const char* who, long long rows, int kb, unsigned* grid) {
+  const long long wg = (rows * 4 * kb + 255) / 256;
+  if (wg > 0x7FFFFFFFLL) return fail(-3, std::string(who) + ": more rows than one launch covers");
+  *grid = (unsigned)wg;
+  return 0;
+}
+
+static int quantize_launch(const void* x, int dtype, long long rows, long long cols, long long stride, uint8_t* codes,
+                           uint8_t* scales, hipStream_t s) {
+  QuantArgs a{};
+  a.x = x, a.rows = rows, a.stride = stride, a.cols = (int)cols, a.kb = (int)((cols + 31) / 32);
+  a.vec = aligned16(x) && (rows == 1 || stride * elem_bytes(dtype) % 16 == 0);
+  a.codes = codes, a.scales = scales;
+  unsigned grid;
+  if (int rc = grid_of("mx4_quantize", rows, a.kb, &grid)) return rc;
+  return by_type(dtype, [&](auto* t) {
+    hipLaunchKernelGGL(mx4_quantize_kernel<std::remove_pointer_t<decltype(t)>>, dim3(grid), dim3(256), 0, s, a);
+    YL_HIP(hipGetLastError());
+    return 0;
+  });
+}
+
+}  // namespace yl
+
+using namespace yl;
+
+extern "C" int yl_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, uint8_t* codes,
+                               uint8_t* scales, void* stream) {
+  if (!value_type(x_dtype)) return fail(-1, "mx4_quantize: bf16, fp16 or fp32 values");
+  if (int rc = check_matrix("mx4_quantize", rows, cols, x_stride)) return rc;
+  if (rows == 0) return 0;
+  if (!x || !codes || !scales) return fail(-1, "mx4_quantize: null pointer");
+  if (!aligned16(codes)) return fail(-1, "mx4_quantize: codes must be 16-byte aligned");
+  return quantize_launch(x, x_dtype, rows, cols, x_stride, codes, scales, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int yl_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* y, int y_dtype,
+                                 int64_t y_stride, void* stream) {
+  if (!value_type(y_dtype)) return fail(-1, "mx4_dequantize: bf16, fp16 or fp32 values");
+  if (int rc = check_matrix("mx4_dequantize", rows, cols, y_stride)) return rc;
+  if (rows == 0) return 0;
+  if (!y || !codes || !scales) return fail(-1, "mx4_dequantize: null pointer");
+  if (!aligned16(codes)) return fail(-1, "mx4_dequantize: codes must be 16-byte aligned");
+  QuantArgs a{};
+  a.rows = rows, a.stride = y_stride, a.cols = (int)cols, a.kb = (int)((cols + 31) / 32);
+  a.vec = aligned16(y) && (rows == 1 || y_stride * elem_bytes(y_dtype) % 16 == 0);
+  a.codes = const_cast<uint8_t*>(codes), a.scales = const_cast<uint8_t*>(scales);
+  unsigned grid;
+  if (int rc = grid_of("mx4_dequantize", rows, a.kb, &grid)) return rc;
+  return by_type(y_dtype, [&](auto* t) {
+    typedef std::remove_pointer_t<decltype(t)> T;
+    hipLaunchKernelGGL(mx4_dequantize_kernel<T>, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), a, static_cast<T*>(y));
+    YL_HIP(hipGetLastError());
+    return 0;
+  });
+}
+
+// workspace of a product: the activations' codes and scales, when they arrive as values
+static long long linear_codes_bytes(long long rows, long long k) { return rows * ((k + 31) / 32) * 16; }
+
+extern "C" int64_t yl_mx4_linear_workspace_bytes(int x_dtype, int64_t rows, int64_t n, int64_t k) {
+  if (check_matrix("mx4_linear", rows, k, k) || check_matrix("mx4_linear", n, k, k)) return -1;
+  if (x_dtype == YL_MX4 || rows == 0) return 0;
+  return (linear_codes_bytes(rows, k) + rows * ((k + 31) / 32) + 255) / 256 * 256;
+}
+
+extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype, int64_t rows, int64_t x_stride,
+                             const uint8_t* w_codes, const uint8_t* w_scales, int64_t n, int64_t k, const float* bias, int act,
+                             const void* res, int64_t res_stride, void* y, int y_dtype, int64_t y_stride, void* work,
+                             int64_t work_bytes, void* stream) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!value_type(x_dtype) && x_dtype != YL_MX4) return fail(-1, "mx4_linear: activations are bf16, fp16, fp32 or MX4");
+  if (!value_type(y_dtype)) return fail(-1, "mx4_linear: bf16, fp16 or fp32 results");
+  if (int rc = check_matrix("mx4_linear", rows, k, x_dtype == YL_MX4 ? k : x_stride)) return rc;
+  if (int rc = check_matrix("mx4_linear", n, k, k)) return rc;
+  if (n < 1 || n > (1 << 22)) return fail(n < 1 ? -1 : -3, "mx4_linear: 1 to 4194304 output columns");
+  if (rows == 0) return 0;
+  if (rows > 1 && (y_stride < n || (res && res_stride < n))) return fail(-1, "mx4_linear: a row stride is smaller than a row");
+  if (!x || !w_codes || !w_scales || !y) return fail(-1, "mx4_linear: null pointer");
+  if (x_dtype == YL_MX4 && !x_scales) return fail(-1, "mx4_linear: MX4 activations come with their scales");
+  if (!aligned16(w_codes) || (x_dtype == YL_MX4 && !aligned16(x))) return fail(-1, "mx4_linear: codes must be 16-byte aligned");
+  const long long need = yl_mx4_linear_workspace_bytes(x_dtype, rows, n, k);
+  if (need > 0 && (!work || work_bytes < need || !aligned16(work))) return fail(-1, "mx4_linear: workspace missing, too small or not 16-byte aligned");
+  LinearArgs a{};
+  a.rows = rows, a.n = (int)n, a.k = (int)k, a.kb = (int)((k + 31) / 32);
+  a.wc = w_codes, a.ws = w_scales, a.bias = bias, a.act = act;
+  a.res = res, a.res_stride = res_stride, a.y = y, a.y_stride = y_stride;
+  if (x_dtype == YL_MX4) {
+    a.xc = static_cast<const uint8_t*>(x), a.xs = x_scales;
+  } else {
+    uint8_t* codes = static_cast<uint8_t*>(work);
+    uint8_t* scales = codes + linear_codes_bytes(rows, k);
+    if (int rc = quantize_launch(x, x_dtype, rows, k, x_stride, codes, scales, s)) return rc;
+    a.xc = codes, a.xs = scales;
+  }
+  const long long ntiles = (n + 15) / 16, mtiles = (rows + 15) / 16;
+  if (ntiles * mtiles > 0x7FFFFFFFLL) return fail(-3, "mx4_linear: more tiles than one launch covers");
+  return by_type(y_dtype, [&](auto* t) {
+    hipLaunchKernelGGL(mx4_product_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)(ntiles * mtiles)), dim3(64), 0, s, a, (int)ntiles);
+    YL_HIP(hipGetLastError());
+    return 0;
+  });
+}
