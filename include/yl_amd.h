@@ -368,6 +368,35 @@ int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype, int64_t r
                   const uint8_t* w_scales, int64_t n, int64_t k, const float* bias, int act, const void* res, int64_t res_stride,
                   void* y, int y_dtype, int64_t y_stride, void* work, int64_t work_bytes, void* stream);
 
+/* ---- block-sparse attention (csrc/block_attn.hip) --------------------------------------------------------------------------
+ * Attention in which every query reads `topk` blocks of `block` (32, 64 or 128) consecutive keys, the ones a cheap score selects
+ * for it: YL_OP_ATTENTION (nn/modules/block.py:905-913) for token maps on which all pairs are too many.  No counterpart in the
+ * reference.  Tensors bf16 or fp16; heads a multiple of kv_heads (query head h reads kv head h / (heads / kv_heads)); dk, dv
+ * multiples of 8 up to 128; at most 4096 key blocks.
+ *   mask: [batch][nk] bytes (row stride mask_stride), non-zero = the key may be read; NULL: all.  What a masked key or value holds
+ *   does not matter.  A query without a readable key gets zeros (and -1 for every block).
+ * An element (b, t, h, c) of a tensor lies at data[b * batch + t * token + h * head + c]: strides in elements, multiples of 8, not
+ * negative (0 broadcasts); data 16-byte aligned. */
+typedef struct yl_heads {
+  void* data;
+  int64_t batch, token, head;
+} yl_heads;
+/* picked[batch][kv_heads][nq][topk]: for each query and kv head the blocks of largest score (sum of q over the kv head's query
+ * heads) . (mean of the block's readable keys), in 64 bits, ties to the lower index (a NaN score ranks as -inf), blocks without a
+ * readable key never; in ascending order, the rest of the row -1.  `work`: 16-byte aligned device scratch of
+ * yl_block_select_workspace_bytes bytes (-1: the sizes are refused), not shared by calls that may overlap. */
+int64_t yl_block_select_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dk, int block);
+int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dk,
+                    int block, int topk, const uint8_t* mask, int64_t mask_stride, int32_t* picked, void* work, int64_t work_bytes,
+                    void* stream);
+/* out[b][i][h] = softmax over the readable keys of the blocks picked[b][h's kv head][i] of (scale * q . k), times v.  Entries of
+ * `picked` outside [0, blocks) are no block; a block named twice counts once; the order does not matter.  fp32 accumulation.
+ * `work` as above, yl_block_attention_workspace_bytes bytes. */
+int64_t yl_block_attention_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block, int topk);
+int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl_heads* v, int dtype, int batch, int nq, int nk, int heads,
+                       int kv_heads, int dk, int dv, int block, int topk, const int32_t* picked, const uint8_t* mask,
+                       int64_t mask_stride, float scale, const yl_heads* out, void* work, int64_t work_bytes, void* stream);
+
 /* ---- multi-GPU exchange of the sharded path ---------------------------------
  * One process per GPU, weights replicated, images sharded; the ONLY exchanges are root -> ranks input slices and ranks ->
  * root packed result records (`b * max_det * 6` fp32 box words + `b` int32 counts per rank and step).  RCCL over xGMI, grouped

@@ -21,6 +21,8 @@ _LAZY = {
     "mx4_quantize": ("nn.mx4", "mx4_quantize"),
     "mx4_dequantize": ("nn.mx4", "mx4_dequantize"),
     "mx4_linear": ("nn.mx4", "mx4_linear"),
+    "block_select": ("nn.block_attention", "block_select"),
+    "block_attention": ("nn.block_attention", "block_attention"),
 }
 
 

@@ -114,6 +114,7 @@ EXPORTS = (  # include/yl_amd.h: the product ABI
     "yl_engine_prefilter_fused", "yl_engine_detect_graph_prepare", "yl_graph_launch_many", "yl_engine_detect_graph_rebind",
     "yl_comm_get_unique_id", "yl_comm_create", "yl_comm_destroy", "yl_comm_rank", "yl_comm_world", "yl_comm_scatter",
     "yl_comm_gather", "yl_comm_barrier", "yl_mx4_quantize", "yl_mx4_dequantize", "yl_mx4_linear_workspace_bytes", "yl_mx4_linear",
+    "yl_block_select_workspace_bytes", "yl_block_select", "yl_block_attention_workspace_bytes", "yl_block_attention",
 )
 COMM_ID_BYTES = 128  # YL_COMM_ID_BYTES
 DIAG_EXPORTS = (  # include/yl_amd_diag.h: probes for tools/ and the runtime self-checks, not part of the product ABI
@@ -148,6 +149,10 @@ class Op(C.Structure):
 class Level(C.Structure):
     _fields_ = [("offset", C.c_int64), ("offset_cls", C.c_int64), ("H", C.c_int32), ("W", C.c_int32),
                 ("stride", C.c_float), ("nc8", C.c_int32), ("offset_xywh", C.c_int64)]
+
+
+class Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_int64), ("token", C.c_int64), ("head", C.c_int64)]
 
 
 _lib = None
@@ -268,6 +273,15 @@ def lib() -> C.CDLL:
     L.yl_mx4_linear_workspace_bytes.argtypes = [i32, i64, i64, i64]
     L.yl_mx4_linear.restype = i32
     L.yl_mx4_linear.argtypes = [vp, vp, i32, i64, i64, vp, vp, i64, i64, vp, i32, vp, i64, vp, i32, i64, vp, i64, vp]
+    hp = C.POINTER(Heads)
+    L.yl_block_select_workspace_bytes.restype = i64
+    L.yl_block_select_workspace_bytes.argtypes = [i32] * 7
+    L.yl_block_select.restype = i32
+    L.yl_block_select.argtypes = [hp, hp] + [i32] * 9 + [vp, i64, vp, vp, i64, vp]
+    L.yl_block_attention_workspace_bytes.restype = i64
+    L.yl_block_attention_workspace_bytes.argtypes = [i32] * 9
+    L.yl_block_attention.restype = i32
+    L.yl_block_attention.argtypes = [hp, hp, hp] + [i32] * 10 + [vp, vp, i64, f32, hp, vp, i64, vp]
     if L.yl_abi_version() != 21:
         raise RuntimeError("libyl_amd.so ABI version mismatch; rebuild it")
     _lib = L

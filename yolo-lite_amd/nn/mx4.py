@@ -13,6 +13,7 @@ from typing import NamedTuple, Optional, Union
 import torch
 
 from .. import _lib
+from ._face import call as _call, on_gpu as _on_gpu
 
 BLOCK = 32  # columns that share one scale
 _TYPES = {torch.bfloat16: _lib.YL_BF16, torch.float32: _lib.YL_F32, torch.float16: _lib.YL_F16}
@@ -25,32 +26,6 @@ class Mx4Tensor(NamedTuple):
     codes: torch.Tensor
     scales: torch.Tensor
     cols: int
-
-
-def _on_gpu(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if t.device.type != "cuda":
-            raise RuntimeError(f"{what} runs on the GPU only (HIP kernel, no CPU fallback)")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on different devices ({dev} and {t.device})")
-        dev = t.device
-    return dev
-
-
-def _call(dev: torch.device, fn, what: str, *args) -> None:
-    """fn(*args, stream) with ``dev`` as the current device, on its current stream."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    if rc:
-        _lib.check(rc, what)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
