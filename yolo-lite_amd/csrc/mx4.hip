@@ -169,6 +169,9 @@ struct LinearArgs {
   void* y;
   long long y_stride;
   int act;
+  int vec;                         // every group of eight results (and residuals) starts on 16 bytes
+  int ntiles, mtiles;              // tiled product: tiles along n and the rows, groups of 64 rows of the tiled scales
+  int wgroups, xgroups;
 };
 
 __device__ __forceinline__ v8i widen(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
@@ -213,6 +216,221 @@ __global__ __launch_bounds__(64) void mx4_product_kernel(LinearArgs a, int ntile
     acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(wv), widen(xv), acc, 4, 4, 0, sw, 0, sx);
   }
   if (okm) finish4<T>(a, acc, m0 + r, n0 + 4 * g);
+}
+
+// ------------------------------------------------------------------------------------------------ tiled product
+// D = W X^T on 16 x 16 tiles: operand A = weight rows, so a lane's four results are consecutive columns of y.  Rows of two adjacent
+// weight tiles interleave (row r of tile t is column (t / 2) 32 + (r / 4) 8 + (t & 1) 4 + r % 4): the two tiles of a lane are then 8
+// consecutive columns, 16 bytes of a bf16 row.
+__device__ __forceinline__ int weight_row(int t, int r) { return (t >> 1) * 32 + (r >> 2) * 8 + (t & 1) * 4 + (r & 3); }
+
+// Scales in the order the pipe takes them: S[k4][group of 64 rows][lane][tile 0..3], a dword = the bytes of four successive k-steps
+// (128 columns each) for the lane's row and block -- v_mfma_scale picks the byte by an immediate, so 16 bytes per lane feed four
+// tiles through 512 columns and no instruction unpacks anything.
+__device__ __forceinline__ unsigned scale_slot(int row64, int block16, bool weight) {
+  // row64: row inside its group of 64; block16: block inside its group of 16 columns-blocks -> byte offset in the 1 KiB
+  int t, r;
+  if (weight) {  // inverse of weight_row
+    const int q = row64 & 31;
+    t = (row64 >> 5) * 2 + ((q >> 2) & 1);
+    r = (q >> 3) * 4 + (q & 3);
+  } else {
+    t = row64 >> 4;
+    r = row64 & 15;
+  }
+  return (unsigned)((((block16 & 3) * 16 + r) * 4 + t) * 4 + (block16 >> 2));
+}
+
+struct TileArgs {
+  QuantArgs q;         // x; q.codes nullptr: x comes quantised, q.scales are its scales
+  uint8_t* xs;         // tiled scales of x
+  const uint8_t* ws;   // the weight's scales [n][kb]
+  uint8_t* wst;        // ... tiled
+  int n, xgroups, wgroups;  // groups of 64 rows
+};
+
+// One workgroup: 64 rows x 512 columns of x -- codes and the 1 KiB of tiled scales -- or the scales of 64 weight rows.
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_tile_kernel(TileArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t sm[1024];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int kb = a.q.kb;
+  const bool weight = (int)blockIdx.y >= a.xgroups;
+  const int rg = weight ? (int)blockIdx.y - a.xgroups : (int)blockIdx.y, k4 = blockIdx.x;
+  reinterpret_cast<unsigned*>(sm)[tid] = 0x7F7F7F7Fu;
+  __syncthreads();
+  if (weight || !a.q.codes) {
+    const uint8_t* src = weight ? a.ws : a.q.scales;
+    const long long rows = weight ? a.n : a.q.rows;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int row = u * 16 + (tid >> 4), blk = tid & 15;
+      const long long gr = (long long)rg * 64 + row;
+      const int gb = k4 * 16 + blk;
+      if (gr < rows && gb < kb) sm[scale_slot(row, blk, weight)] = src[gr * kb + gb];
+    }
+  } else {
+    const int c8 = k4 * 64 + lane;  // this lane's group of eight columns
+    const bool live = c8 < 4 * kb;
+    const T* x = static_cast<const T*>(a.q.x);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[8][8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {  // eight rows in flight
+        const long long row = (long long)rg * 64 + wave * 16 + h * 8 + u;
+        const int left = live && row < a.q.rows ? a.q.cols - c8 * 8 : 0;
+        load8(x + row * a.q.stride + c8 * 8, left, a.q.vec, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int r64 = wave * 16 + h * 8 + u;
+        const long long row = (long long)rg * 64 + r64;
+        unsigned s;
+        const unsigned c = quantize8(v[u], &s);
+        if (live && row < a.q.rows) {
+          reinterpret_cast<unsigned*>(a.q.codes)[row * (4 * kb) + c8] = c;
+          if ((lane & 3) == 0) sm[scale_slot(r64, lane >> 2, false)] = (uint8_t)s;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  unsigned* dst = reinterpret_cast<unsigned*>(weight ? a.wst : a.xs) + ((size_t)k4 * (weight ? a.wgroups : a.xgroups) + rg) * 256;
+  dst[tid] = reinterpret_cast<const unsigned*>(sm)[tid];
+}
+
+// y[m][n .. n + 8)
+template <typename T>
+__device__ __forceinline__ void finish8(const LinearArgs& a, const float (&acc)[8], const float (&bias)[8], long long m, int n) {
+  float v[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) v[r] = acc[r] + bias[r];
+  if (a.act) silu8(v);
+  if (a.res) {
+    float q[8];
+    load8(static_cast<const T*>(a.res) + m * a.res_stride + n, a.n - n, a.vec, q);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] += q[r];
+  }
+  store8(static_cast<T*>(a.y) + m * a.y_stride + n, a.n - n, a.vec, v);
+}
+
+typedef __attribute__((address_space(3))) void lds_void_m;
+
+// A workgroup of 2 x 2 waves owns 32 WT weight rows x 32 XT activation rows; a wave WT x XT tiles.  Both operands pass through LDS by
+// LDS-DMA in slices of one k-step (128 columns, 64 bytes of a row) through a ring of four: a 1 KiB piece is 16 rows, four lanes per
+// row, so memory sees 64-byte runs; the four 16-byte blocks of a row are rotated by xor with row / 4, which makes the fragment read
+// (16 rows, one block) conflict-free although rows lie 64 bytes apart.
+template <typename T, int WT, int XT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void mx4_gemm_kernel(LinearArgs a) {
+  constexpr int NS = 4;
+  constexpr int TN = 32 * WT, TM = 32 * XT;
+  constexpr int NPA = TN / 16, NP = NPA + TM / 16, PW = NP / 4;  // 1 KiB pieces of a slice; per wave
+  constexpr int STAGE = NP * 1024;
+  extern __shared__ __attribute__((aligned(16))) unsigned char gsm[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  const int wn = wave >> 1, wm = wave & 1;
+  // tiles: groups of eight activation tiles walk the weight tiles together, consecutive workgroups of an XCD share both
+  const int tile = xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  const int per = 8 * a.ntiles, grp = tile / per, first = grp * 8;
+  const int gm = min(8, a.mtiles - first), rest = tile - grp * per;
+  const int tm = first + rest % gm, tn = rest / gm;
+  const long long m0 = (long long)tm * TM;
+  const int n0 = tn * TN;
+  const int pitch = a.kb * 16;
+  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.wc + (long long)n0 * pitch), (short)0, (unsigned)min(TN, a.n - n0) * (unsigned)pitch, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(a.xc + m0 * pitch), (short)0, (unsigned)min((long long)TM, a.rows - m0) * (unsigned)pitch, 0x00020000);
+  const int nk = (a.kb + 3) >> 2;  // slices
+  // this lane's part of a piece: row lane / 4, block (lane & 3) ^ (row / 4)
+  const int pr = lane >> 2, pb = (lane & 3) ^ (pr >> 2);
+  unsigned src[PW];  // byte offset in the operand, without the slice
+#pragma unroll
+  for (int i = 0; i < PW; ++i) {
+    const int p = wave + 4 * i;
+    src[i] = (unsigned)(p < NPA ? weight_row(p, pr) : (p - NPA) * 16 + pr) * (unsigned)pitch + (unsigned)pb * 16u;
+  }
+  auto issue = [&](int it, int slot) __attribute__((always_inline)) {
+    const unsigned past = it * 4 + pb < a.kb ? (unsigned)it * 64u : OOB_LANE;  // columns behind the last: zeros
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int p = wave + 4 * i;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < NPA / 4 ? rw : rx, (lds_void_m*)(gsm + slot * STAGE + p * 1024), 16,
+                                               (int)(past == OOB_LANE ? OOB_LANE : src[i] + past), 0, 0, 0);
+    }
+  };
+  // tiled scales of this wave's tiles
+  const v4i* wsp = reinterpret_cast<const v4i*>(a.ws) + ((size_t)(n0 >> 6) + wn * (WT / 4)) * 64 + lane;
+  const v4i* xsp = reinterpret_cast<const v4i*>(a.xs) + ((size_t)(m0 >> 6) + wm * (XT / 4)) * 64 + lane;
+  const size_t wstep = (size_t)a.wgroups * 64, xstep = (size_t)a.xgroups * 64;
+  const int wleft = a.wgroups - ((n0 >> 6) + wn * (WT / 4)), xleft = a.xgroups - (int)((m0 >> 6) + wm * (XT / 4));
+
+  f32x4 acc[WT][XT];
+#pragma unroll
+  for (int i = 0; i < WT; ++i)
+#pragma unroll
+    for (int j = 0; j < XT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const unsigned fo = (unsigned)r * 64u + (unsigned)((g ^ (r >> 2)) * 16);  // a fragment inside its piece
+  const unsigned char* ap = gsm + wn * WT * 1024 + fo;
+  const unsigned char* bp = gsm + (NPA + wm * XT) * 1024 + fo;
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s) issue(s, s);
+  v4i sw[WT / 4], sx[XT / 4];
+  for (int k4 = 0; k4 * 4 < nk; ++k4) {
+#pragma unroll
+    for (int i = 0; i < WT / 4; ++i) sw[i] = i < wleft ? wsp[k4 * wstep + i * 64] : v4i{0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F};
+#pragma unroll
+    for (int i = 0; i < XT / 4; ++i) sx[i] = i < xleft ? xsp[k4 * xstep + i * 64] : v4i{0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F};
+    auto slice = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int S = decltype(tag)::value;
+      const int it = k4 * 4 + S;
+      if (it >= nk) return;
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * PW) : "memory");
+      __builtin_amdgcn_s_barrier();
+      issue(it + NS - 1, (S + NS - 1) % NS);
+      v4i fa[WT], fb[XT];
+#pragma unroll
+      for (int j = 0; j < XT; ++j) fb[j] = *reinterpret_cast<const v4i*>(bp + S * STAGE + j * 1024);
+#pragma unroll
+      for (int i = 0; i < WT; ++i) fa[i] = *reinterpret_cast<const v4i*>(ap + S * STAGE + i * 1024);
+#pragma unroll
+      for (int i = 0; i < WT; ++i)
+#pragma unroll
+        for (int j = 0; j < XT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(fa[i]), widen(fb[j]), acc[i][j], 4, 4, S, sw[i >> 2][i & 3], S,
+                                                                       sx[j >> 2][j & 3]);
+    };
+    slice(std::integral_constant<int, 0>{});
+    slice(std::integral_constant<int, 1>{});
+    slice(std::integral_constant<int, 2>{});
+    slice(std::integral_constant<int, 3>{});
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last refills, all out of range)
+#pragma unroll
+  for (int i = 0; i < WT / 2; ++i) {
+    const int n = n0 + (wn * (WT / 2) + i) * 32 + g * 8;
+    if (n >= a.n) break;
+    float bias[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) bias[q] = a.bias && n + q < a.n ? a.bias[n + q] : 0.f;
+#pragma unroll
+    for (int j = 0; j < XT; ++j) {
+      const long long m = m0 + (wm * XT + j) * 16 + r;
+      if (m >= a.rows) break;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v[q] = acc[2 * i][j][q];
+        v[4 + q] = acc[2 * i + 1][j][q];
+      }
+      finish8<T>(a, v, bias, m, n);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -293,13 +511,48 @@ extern "C" int yl_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, in
   });
 }
 
-// workspace of a product: the activations' codes and scales, when they arrive as values
-static long long linear_codes_bytes(long long rows, long long k) { return rows * ((k + 31) / 32) * 16; }
+// ---- how a product runs: a wave per 16 x 16 tile for few rows, else tiles through LDS on the pipe's own order of the scales
+struct Plan {
+  bool tiled;
+  int wt, xt;                    // tiles per wave
+  long long ntiles, mtiles;
+  long long codes, xs, ws, all;  // bytes: codes of x, scales of x, tiled scales of the weight, the workspace
+  long long xgroups, wgroups, k4;
+};
+
+static Plan plan_linear(int x_dtype, long long rows, long long n, long long k) {
+  Plan p{};
+  const long long kb = (k + 31) / 32;
+  p.tiled = rows > 32;
+  p.codes = x_dtype == YL_MX4 ? 0 : (rows * kb * 16 + 255) / 256 * 256;
+  if (p.tiled) {
+    p.wt = p.xt = 8;
+    if (((n + 255) / 256) * ((rows + 255) / 256) < 192) p.wt = p.xt = 4;
+    p.ntiles = (n + 32 * p.wt - 1) / (32 * p.wt), p.mtiles = (rows + 32 * p.xt - 1) / (32 * p.xt);
+    p.k4 = (kb + 15) / 16, p.xgroups = (rows + 63) / 64, p.wgroups = (n + 63) / 64;
+    p.xs = p.k4 * p.xgroups * 1024, p.ws = p.k4 * p.wgroups * 1024;
+  } else {
+    p.wt = p.xt = 1;
+    p.ntiles = (n + 15) / 16, p.mtiles = (rows + 15) / 16;
+    p.xs = x_dtype == YL_MX4 ? 0 : (rows * kb + 255) / 256 * 256;
+  }
+  p.all = p.codes + p.xs + p.ws;
+  return p;
+}
+
+template <typename T, int WT, int XT>
+static int gemm_launch(const LinearArgs& a, hipStream_t s) {
+  auto kern = mx4_gemm_kernel<T, WT, XT>;
+  const int lds = 4 * (2 * WT + 2 * XT) * 1024;
+  if (int rc = allow_big_lds(reinterpret_cast<const void*>(kern), lds)) return rc;
+  hipLaunchKernelGGL(kern, dim3((unsigned)a.ntiles * (unsigned)a.mtiles), dim3(256), lds, s, a);
+  YL_HIP(hipGetLastError());
+  return 0;
+}
 
 extern "C" int64_t yl_mx4_linear_workspace_bytes(int x_dtype, int64_t rows, int64_t n, int64_t k) {
   if (check_matrix("mx4_linear", rows, k, k) || check_matrix("mx4_linear", n, k, k)) return -1;
-  if (x_dtype == YL_MX4 || rows == 0) return 0;
-  return (linear_codes_bytes(rows, k) + rows * ((k + 31) / 32) + 255) / 256 * 256;
+  return rows == 0 ? 0 : plan_linear(x_dtype, rows, n, k).all;
 }
 
 extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype, int64_t rows, int64_t x_stride,
@@ -317,25 +570,48 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
   if (!x || !w_codes || !w_scales || !y) return fail(-1, "mx4_linear: null pointer");
   if (x_dtype == YL_MX4 && !x_scales) return fail(-1, "mx4_linear: MX4 activations come with their scales");
   if (!aligned16(w_codes) || (x_dtype == YL_MX4 && !aligned16(x))) return fail(-1, "mx4_linear: codes must be 16-byte aligned");
-  const long long need = yl_mx4_linear_workspace_bytes(x_dtype, rows, n, k);
-  if (need > 0 && (!work || work_bytes < need || !aligned16(work))) return fail(-1, "mx4_linear: workspace missing, too small or not 16-byte aligned");
+  const Plan p = plan_linear(x_dtype, rows, n, k);
+  if (p.all > 0 && (!work || work_bytes < p.all || !aligned16(work)))
+    return fail(-1, "mx4_linear: workspace missing, too small or not 16-byte aligned");
+  if (p.ntiles * p.mtiles > 0x7FFFFFFFLL || p.xgroups + p.wgroups > 65535)
+    return fail(-3, "mx4_linear: more rows than one launch covers");
   LinearArgs a{};
   a.rows = rows, a.n = (int)n, a.k = (int)k, a.kb = (int)((k + 31) / 32);
   a.wc = w_codes, a.ws = w_scales, a.bias = bias, a.act = act;
   a.res = res, a.res_stride = res_stride, a.y = y, a.y_stride = y_stride;
-  if (x_dtype == YL_MX4) {
-    a.xc = static_cast<const uint8_t*>(x), a.xs = x_scales;
-  } else {
-    uint8_t* codes = static_cast<uint8_t*>(work);
-    uint8_t* scales = codes + linear_codes_bytes(rows, k);
-    if (int rc = quantize_launch(x, x_dtype, rows, k, x_stride, codes, scales, s)) return rc;
-    a.xc = codes, a.xs = scales;
+  const int ye = elem_bytes(y_dtype);
+  a.vec = aligned16(y) && (rows == 1 || y_stride * ye % 16 == 0) && (!res || (aligned16(res) && (rows == 1 || res_stride * ye % 16 == 0)));
+  a.ntiles = (int)p.ntiles, a.mtiles = (int)p.mtiles, a.xgroups = (int)p.xgroups, a.wgroups = (int)p.wgroups;
+  uint8_t* const codes = static_cast<uint8_t*>(work);
+  uint8_t* const xs = codes + p.codes;
+  const bool packed = x_dtype == YL_MX4;
+  a.xc = packed ? static_cast<const uint8_t*>(x) : codes;
+  if (!p.tiled) {
+    a.xs = packed ? x_scales : xs;
+    if (!packed)
+      if (int rc = quantize_launch(x, x_dtype, rows, k, x_stride, codes, xs, s)) return rc;
+    return by_type(y_dtype, [&](auto* t) {
+      hipLaunchKernelGGL(mx4_product_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)(p.ntiles * p.mtiles)), dim3(64), 0, s, a,
+                         (int)p.ntiles);
+      YL_HIP(hipGetLastError());
+      return 0;
+    });
   }
-  const long long ntiles = (n + 15) / 16, mtiles = (rows + 15) / 16;
-  if (ntiles * mtiles > 0x7FFFFFFFLL) return fail(-3, "mx4_linear: more tiles than one launch covers");
+  TileArgs ta{};
+  ta.q.x = x, ta.q.rows = rows, ta.q.stride = x_stride, ta.q.cols = (int)k, ta.q.kb = a.kb;
+  ta.q.vec = aligned16(x) && x_stride * elem_bytes(x_dtype) % 16 == 0;
+  ta.q.codes = packed ? nullptr : codes, ta.q.scales = const_cast<uint8_t*>(x_scales);
+  ta.xs = xs, ta.ws = w_scales, ta.wst = xs + p.xs, ta.n = (int)n, ta.xgroups = a.xgroups, ta.wgroups = a.wgroups;
+  if (int rc = by_type(packed ? YL_BF16 : x_dtype, [&](auto* t) {
+        hipLaunchKernelGGL(mx4_tile_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)p.k4, (unsigned)(p.xgroups + p.wgroups)), dim3(256), 0,
+                           s, ta);
+        YL_HIP(hipGetLastError());
+        return 0;
+      }))
+    return rc;
+  a.xs = ta.xs, a.ws = ta.wst;
   return by_type(y_dtype, [&](auto* t) {
-    hipLaunchKernelGGL(mx4_product_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)(ntiles * mtiles)), dim3(64), 0, s, a, (int)ntiles);
-    YL_HIP(hipGetLastError());
-    return 0;
+    typedef std::remove_pointer_t<decltype(t)> T;
+    return p.wt == 8 ? gemm_launch<T, 8, 8>(a, s) : gemm_launch<T, 4, 4>(a, s);
   });
 }
