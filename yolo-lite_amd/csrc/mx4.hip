@@ -176,7 +176,7 @@ struct LinearArgs {
 
 __device__ __forceinline__ v8i widen(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
-// y[m][n .. n + 4) = epilogue of four accumulators
+// y[m][n .. n + 4): bias, SiLU, residual, one rounding
 template <typename T>
 __device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 acc, long long m, int n) {
 #pragma unroll
@@ -190,32 +190,81 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 acc, long lon
   }
 }
 
-// One wave: 16 weight rows (operand A) x 16 activation rows (operand B), operands straight from memory.
-template <typename T>
-__global__ __launch_bounds__(64) void mx4_product_kernel(LinearArgs a, int ntiles) {
-  const int lane = threadIdx.x, g = lane >> 4, r = lane & 15;
-  const int n0 = (int)(blockIdx.x % (unsigned)ntiles) * 16;
-  const long long m0 = (long long)(blockIdx.x / (unsigned)ntiles) * 16;
-  const bool okn = n0 + r < a.n, okm = m0 + r < a.rows;
-  const long long wr = okn ? n0 + r : 0, xr = okm ? m0 + r : 0;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int b0 = 0; b0 < a.kb; b0 += 4) {
-    const int b = b0 + g;
-    v4i wv = {0, 0, 0, 0}, xv = {0, 0, 0, 0};
-    int sw = 127, sx = 127;
-    if (b < a.kb) {
-      if (okn) {
-        wv = *reinterpret_cast<const v4i*>(a.wc + (wr * a.kb + b) * 16);
-        sw = a.ws[wr * a.kb + b];
+// ------------------------------------------------------------------------------------------------ product, split over k
+// Few rows: the product is the time it takes to read the weight (one row of x: 0.53 bytes per multiply-add), and a grid of large
+// tiles would leave most of the chip idle.  A workgroup owns 16 WT weight rows x 16 XT rows of x; its NW waves take the k-steps in
+// turn, operands straight from memory into registers, and the partial sums meet in LDS in a fixed order.
+template <typename T, int WT, int XT, int NW>
+__global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
+  __shared__ __attribute__((aligned(16))) f32x4 part[NW][WT * XT][64];
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int n0 = (int)(blockIdx.x % (unsigned)a.ntiles) * (16 * WT);
+  const long long m0 = (long long)(blockIdx.x / (unsigned)a.ntiles) * (16 * XT);
+  const uint8_t *wp[WT], *wsp[WT], *xp[XT], *xsp[XT];
+#pragma unroll
+  for (int i = 0; i < WT; ++i) {  // rows behind the last: the last one's values, not stored
+    const long long row = min(n0 + i * 16 + r, a.n - 1);
+    wp[i] = a.wc + row * a.kb * 16;
+    wsp[i] = a.ws + row * a.kb;
+  }
+#pragma unroll
+  for (int j = 0; j < XT; ++j) {
+    const long long row = min(m0 + j * 16 + r, a.rows - 1);
+    xp[j] = a.xc + row * a.kb * 16;
+    xsp[j] = a.xs + row * a.kb;
+  }
+  f32x4 acc[WT][XT];
+#pragma unroll
+  for (int i = 0; i < WT; ++i)
+#pragma unroll
+    for (int j = 0; j < XT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int nk = (a.kb + 3) >> 2;
+  constexpr int U = WT * XT <= 2 ? 4 : 2;  // k-steps whose loads are in flight together
+  for (int it0 = wave; it0 < nk; it0 += U * NW) {
+    v4i w[U][WT], x[U][XT];
+    int sw[U][WT], sx[U][XT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = (it0 + u * NW) * 4 + g;
+      const bool in = b < a.kb;  // columns behind the last: zeros
+      const int bb = in ? b : 0;
+#pragma unroll
+      for (int i = 0; i < WT; ++i) {
+        w[u][i] = *reinterpret_cast<const v4i*>(wp[i] + (long long)bb * 16);
+        sw[u][i] = wsp[i][bb];
+        if (!in) w[u][i] = v4i{0, 0, 0, 0}, sw[u][i] = 127;
       }
-      if (okm) {
-        xv = *reinterpret_cast<const v4i*>(a.xc + (xr * a.kb + b) * 16);
-        sx = a.xs[xr * a.kb + b];
+#pragma unroll
+      for (int j = 0; j < XT; ++j) {
+        x[u][j] = *reinterpret_cast<const v4i*>(xp[j] + (long long)bb * 16);
+        sx[u][j] = in ? xsp[j][bb] : 127;
       }
     }
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(wv), widen(xv), acc, 4, 4, 0, sw, 0, sx);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < WT; ++i)
+#pragma unroll
+        for (int j = 0; j < XT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(w[u][i]), widen(x[u][j]), acc[i][j], 4, 4, 0, sw[u][i], 0, sx[u][j]);
   }
-  if (okm) finish4<T>(a, acc, m0 + r, n0 + 4 * g);
+#pragma unroll
+  for (int i = 0; i < WT; ++i)
+#pragma unroll
+    for (int j = 0; j < XT; ++j) part[wave][i * XT + j][lane] = acc[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int t0 = 0; t0 < WT * XT; t0 += NW) {
+    const int t = t0 + wave;
+    if (t >= WT * XT) break;
+    const int i = t / XT, j = t % XT;
+    const long long m = m0 + j * 16 + r;
+    f32x4 s = part[0][t][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) s += part[w][t][lane];
+    if (m < a.rows) finish4<T>(a, s, m, n0 + i * 16 + 4 * g);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ tiled product
@@ -251,88 +300,71 @@ struct TileArgs {
 
 // One workgroup: 64 rows x 512 columns of x -- codes and the 1 KiB of tiled scales -- or the scales of 64 weight rows.
 template <typename T>
-__global__ __launch_bounds__(256) void mx4_tile_kernel(TileArgs a) {
+__global__ __launch_bounds__(1024) void mx4_tile_kernel(TileArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[1024];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kb = a.q.kb;
   const bool weight = (int)blockIdx.y >= a.xgroups;
   const int rg = weight ? (int)blockIdx.y - a.xgroups : (int)blockIdx.y, k4 = blockIdx.x;
-  reinterpret_cast<unsigned*>(sm)[tid] = 0x7F7F7F7Fu;
+  sm[tid] = 0x7F;
   __syncthreads();
   if (weight || !a.q.codes) {
     const uint8_t* src = weight ? a.ws : a.q.scales;
     const long long rows = weight ? a.n : a.q.rows;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int row = u * 16 + (tid >> 4), blk = tid & 15;
-      const long long gr = (long long)rg * 64 + row;
-      const int gb = k4 * 16 + blk;
-      if (gr < rows && gb < kb) sm[scale_slot(row, blk, weight)] = src[gr * kb + gb];
-    }
+    const int row = tid >> 4, blk = tid & 15;
+    const long long gr = (long long)rg * 64 + row;
+    const int gb = k4 * 16 + blk;
+    if (gr < rows && gb < kb) sm[scale_slot(row, blk, weight)] = src[gr * kb + gb];
   } else {
     const int c8 = k4 * 64 + lane;  // this lane's group of eight columns
     const bool live = c8 < 4 * kb;
     const T* x = static_cast<const T*>(a.q.x);
+    float v[4][8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[8][8];
+    for (int u = 0; u < 4; ++u) {  // a wave's four rows are in flight together
+      const long long row = (long long)rg * 64 + wave * 4 + u;
+      const int left = live && row < a.q.rows ? a.q.cols - c8 * 8 : 0;
+      load8(x + row * a.q.stride + c8 * 8, left, a.q.vec, v[u]);
+    }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {  // eight rows in flight
-        const long long row = (long long)rg * 64 + wave * 16 + h * 8 + u;
-        const int left = live && row < a.q.rows ? a.q.cols - c8 * 8 : 0;
-        load8(x + row * a.q.stride + c8 * 8, left, a.q.vec, v[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int r64 = wave * 16 + h * 8 + u;
-        const long long row = (long long)rg * 64 + r64;
-        unsigned s;
-        const unsigned c = quantize8(v[u], &s);
-        if (live && row < a.q.rows) {
-          reinterpret_cast<unsigned*>(a.q.codes)[row * (4 * kb) + c8] = c;
-          if ((lane & 3) == 0) sm[scale_slot(r64, lane >> 2, false)] = (uint8_t)s;
-        }
+    for (int u = 0; u < 4; ++u) {
+      const int r64 = wave * 4 + u;
+      const long long row = (long long)rg * 64 + r64;
+      unsigned s;
+      const unsigned c = quantize8(v[u], &s);
+      if (live && row < a.q.rows) {
+        reinterpret_cast<unsigned*>(a.q.codes)[row * (4 * kb) + c8] = c;
+        if ((lane & 3) == 0) sm[scale_slot(r64, lane >> 2, false)] = (uint8_t)s;
       }
     }
   }
   __syncthreads();
-  unsigned* dst = reinterpret_cast<unsigned*>(weight ? a.wst : a.xs) + ((size_t)k4 * (weight ? a.wgroups : a.xgroups) + rg) * 256;
-  dst[tid] = reinterpret_cast<const unsigned*>(sm)[tid];
-}
-
-// y[m][n .. n + 8)
-template <typename T>
-__device__ __forceinline__ void finish8(const LinearArgs& a, const float (&acc)[8], const float (&bias)[8], long long m, int n) {
-  float v[8];
-#pragma unroll
-  for (int r = 0; r < 8; ++r) v[r] = acc[r] + bias[r];
-  if (a.act) silu8(v);
-  if (a.res) {
-    float q[8];
-    load8(static_cast<const T*>(a.res) + m * a.res_stride + n, a.n - n, a.vec, q);
-#pragma unroll
-    for (int r = 0; r < 8; ++r) v[r] += q[r];
+  if (tid < 256) {
+    unsigned* dst = reinterpret_cast<unsigned*>(weight ? a.wst : a.xs) + ((size_t)k4 * (weight ? a.wgroups : a.xgroups) + rg) * 256;
+    dst[tid] = reinterpret_cast<const unsigned*>(sm)[tid];
   }
-  store8(static_cast<T*>(a.y) + m * a.y_stride + n, a.n - n, a.vec, v);
 }
 
 typedef __attribute__((address_space(3))) void lds_void_m;
 
-// A workgroup of 2 x 2 waves owns 32 WT weight rows x 32 XT activation rows; a wave WT x XT tiles.  Both operands pass through LDS by
-// LDS-DMA in slices of one k-step (128 columns, 64 bytes of a row) through a ring of four: a 1 KiB piece is 16 rows, four lanes per
-// row, so memory sees 64-byte runs; the four 16-byte blocks of a row are rotated by xor with row / 4, which makes the fragment read
-// (16 rows, one block) conflict-free although rows lie 64 bytes apart.
-template <typename T, int WT, int XT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void mx4_gemm_kernel(LinearArgs a) {
-  constexpr int NS = 4;
-  constexpr int TN = 32 * WT, TM = 32 * XT;
-  constexpr int NPA = TN / 16, NP = NPA + TM / 16, PW = NP / 4;  // 1 KiB pieces of a slice; per wave
+// A workgroup of 2 x NWM waves owns 32 WT weight rows x 16 NWM XT activation rows; a wave WT x XT tiles.  Both operands pass through
+// LDS by LDS-DMA in slices of KS k-steps (128 columns, 64 bytes of a row each) through a ring of NS; a 1 KiB piece is 16 / KS rows,
+// neighbouring lanes on one row.  The 16-byte blocks of a row are permuted by xor with a function of the row, which makes the
+// fragment reads (16 rows, one block) conflict-free although rows lie 64 or 128 bytes apart.
+template <typename T, int WT, int XT, int NWM, int KS, int NS>
+__global__ __launch_bounds__(128 * NWM, 2) void mx4_gemm_kernel(LinearArgs a) {
+  constexpr int NW = 2 * NWM;
+  constexpr int TN = 32 * WT, TM = 16 * NWM * XT;
+  constexpr int TILE = KS * 1024;                                // bytes of a 16-row tile in a slice
+  constexpr int NPA = TN / 16 * KS, NP = NPA + TM / 16 * KS, PW = NP / NW;  // 1 KiB pieces of a slice; per wave
   constexpr int STAGE = NP * 1024;
+  constexpr int LB = 2 + (KS == 2), LM = (1 << LB) - 1;          // lanes per row of a piece: 4 KS
+  static_assert(NP % NW == 0 && NPA % NW == 0 && NW % KS == 0, "pieces divide over the waves");
   extern __shared__ __attribute__((aligned(16))) unsigned char gsm[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int wn = wave >> 1, wm = wave & 1;
+  const int wn = wave / NWM, wm = wave % NWM;
   // tiles: groups of eight activation tiles walk the weight tiles together, consecutive workgroups of an XCD share both
   const int tile = xcd_remap((int)blockIdx.x, (int)gridDim.x);
   const int per = 8 * a.ntiles, grp = tile / per, first = grp * 8;
@@ -345,29 +377,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void m
       (void*)(a.wc + (long long)n0 * pitch), (short)0, (unsigned)min(TN, a.n - n0) * (unsigned)pitch, 0x00020000);
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(a.xc + m0 * pitch), (short)0, (unsigned)min((long long)TM, a.rows - m0) * (unsigned)pitch, 0x00020000);
-  const int nk = (a.kb + 3) >> 2;  // slices
-  // this lane's part of a piece: row lane / 4, block (lane & 3) ^ (row / 4)
-  const int pr = lane >> 2, pb = (lane & 3) ^ (pr >> 2);
+  const int nk = (a.kb + 3) >> 2;            // k-steps
+  // the permutation of a row's blocks, and this lane's part of a piece: row lane / (4 KS), block (lane mod 4 KS) permuted
+  auto swz = [](int row) { return KS == 1 ? -(row >> 2) & 3 : (row >> 1) & 7; };
+  const int pr = lane >> LB;
   unsigned src[PW];  // byte offset in the operand, without the slice
+  int blk = 0;       // (the same for every piece of a wave: its pieces cover the same half of a tile)
 #pragma unroll
   for (int i = 0; i < PW; ++i) {
-    const int p = wave + 4 * i;
-    src[i] = (unsigned)(p < NPA ? weight_row(p, pr) : (p - NPA) * 16 + pr) * (unsigned)pitch + (unsigned)pb * 16u;
+    const int p = wave + NW * i, t = p / KS, row = (p % KS) * (16 / KS) + pr;
+    const int b = (lane & LM) ^ swz(row);
+    src[i] = (unsigned)(p < NPA ? weight_row(t, row) : (t - NPA / KS) * 16 + row) * (unsigned)pitch + (unsigned)b * 16u;
+    blk = b;
   }
-  auto issue = [&](int it, int slot) __attribute__((always_inline)) {
-    const unsigned past = it * 4 + pb < a.kb ? (unsigned)it * 64u : OOB_LANE;  // columns behind the last: zeros
+  auto issue = [&](int sl, int slot) __attribute__((always_inline)) {
+    const unsigned past = sl * (4 * KS) + blk < a.kb ? (unsigned)sl * (64u * KS) : OOB_LANE;  // columns behind the last: zeros
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
-      const int p = wave + 4 * i;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < NPA / 4 ? rw : rx, (lds_void_m*)(gsm + slot * STAGE + p * 1024), 16,
+      const int p = wave + NW * i;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < NPA / NW ? rw : rx, (lds_void_m*)(gsm + slot * STAGE + p * 1024), 16,
                                                (int)(past == OOB_LANE ? OOB_LANE : src[i] + past), 0, 0, 0);
     }
   };
-  // tiled scales of this wave's tiles
+  // tiled scales of this wave's tiles: four tiles' bytes for four slices are 16 bytes of a lane
+  struct Scales {
+    v4i w[WT / 4], x[XT / 4];
+  };
   const v4i* wsp = reinterpret_cast<const v4i*>(a.ws) + ((size_t)(n0 >> 6) + wn * (WT / 4)) * 64 + lane;
   const v4i* xsp = reinterpret_cast<const v4i*>(a.xs) + ((size_t)(m0 >> 6) + wm * (XT / 4)) * 64 + lane;
   const size_t wstep = (size_t)a.wgroups * 64, xstep = (size_t)a.xgroups * 64;
   const int wleft = a.wgroups - ((n0 >> 6) + wn * (WT / 4)), xleft = a.xgroups - (int)((m0 >> 6) + wm * (XT / 4));
+  const int k4n = (nk + 3) >> 2;
+  auto scales = [&](int k4, Scales& s) __attribute__((always_inline)) {
+    const v4i one = {0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F};
+    const int k = min(k4, k4n - 1);
+#pragma unroll
+    for (int i = 0; i < WT / 4; ++i) s.w[i] = i < wleft ? wsp[k * wstep + i * 64] : one;
+#pragma unroll
+    for (int i = 0; i < XT / 4; ++i) s.x[i] = i < xleft ? xsp[k * xstep + i * 64] : one;
+  };
 
   f32x4 acc[WT][XT];
 #pragma unroll
@@ -375,60 +423,99 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void m
 #pragma unroll
     for (int j = 0; j < XT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const unsigned fo = (unsigned)r * 64u + (unsigned)((g ^ (r >> 2)) * 16);  // a fragment inside its piece
-  const unsigned char* ap = gsm + wn * WT * 1024 + fo;
-  const unsigned char* bp = gsm + (NPA + wm * XT) * 1024 + fo;
+  const unsigned char* ap = gsm + wn * WT * TILE + r * (64 * KS);
+  const unsigned char* bp = gsm + (NPA * 1024) + wm * XT * TILE + r * (64 * KS);
+  struct Frags {
+    v4i w[WT], x[XT];
+  };
+  auto load = [&](int slot, int ks, Frags& f) __attribute__((always_inline)) {
+    const unsigned o = (unsigned)slot * STAGE + (unsigned)(((ks * 4 + g) ^ swz(r)) * 16);
+#pragma unroll
+    for (int j = 0; j < XT; ++j) f.x[j] = *reinterpret_cast<const v4i*>(bp + o + j * TILE);
+#pragma unroll
+    for (int i = 0; i < WT; ++i) f.w[i] = *reinterpret_cast<const v4i*>(ap + o + i * TILE);
+  };
+  auto mma = [&](const Frags& f, const Scales& s, auto tag) __attribute__((always_inline)) {
+    constexpr int S = decltype(tag)::value;
+#pragma unroll
+    for (int i = 0; i < WT; ++i)
+#pragma unroll
+      for (int j = 0; j < XT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(f.w[i]), widen(f.x[j]), acc[i][j], 4, 4, S, s.w[i >> 2][i & 3], S,
+                                                                     s.x[j >> 2][j & 3]);
+  };
+  // my pieces of the oldest slice in flight have landed, my reads are done; behind the barrier so have everybody's
+  auto enter = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * PW) : "memory");
+    __builtin_amdgcn_s_barrier();
+  };
+  Scales sc, sn;
+  scales(0, sn);
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s) issue(s, s);
-  v4i sw[WT / 4], sx[XT / 4];
-  for (int k4 = 0; k4 * 4 < nk; ++k4) {
-#pragma unroll
-    for (int i = 0; i < WT / 4; ++i) sw[i] = i < wleft ? wsp[k4 * wstep + i * 64] : v4i{0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F};
-#pragma unroll
-    for (int i = 0; i < XT / 4; ++i) sx[i] = i < xleft ? xsp[k4 * xstep + i * 64] : v4i{0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F, 0x7F7F7F7F};
-    auto slice = [&](auto tag) __attribute__((always_inline)) {
+  int slot = 0, sl = 0;
+  for (int k4 = 0; k4 < k4n; ++k4) {
+    sc = sn;
+    scales(k4 + 1, sn);
+    auto step = [&](auto tag) __attribute__((always_inline)) {
       constexpr int S = decltype(tag)::value;
-      const int it = k4 * 4 + S;
-      if (it >= nk) return;
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * PW) : "memory");
-      __builtin_amdgcn_s_barrier();
-      issue(it + NS - 1, (S + NS - 1) % NS);
-      v4i fa[WT], fb[XT];
-#pragma unroll
-      for (int j = 0; j < XT; ++j) fb[j] = *reinterpret_cast<const v4i*>(bp + S * STAGE + j * 1024);
-#pragma unroll
-      for (int i = 0; i < WT; ++i) fa[i] = *reinterpret_cast<const v4i*>(ap + S * STAGE + i * 1024);
-#pragma unroll
-      for (int i = 0; i < WT; ++i)
-#pragma unroll
-        for (int j = 0; j < XT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(fa[i]), widen(fb[j]), acc[i][j], 4, 4, S, sw[i >> 2][i & 3], S,
-                                                                       sx[j >> 2][j & 3]);
+      if (k4 * 4 + S >= nk) return;
+      if constexpr (S % KS == 0) {
+        enter();
+        issue(sl + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+      }
+      Frags f;
+      load(slot, S % KS, f);
+      mma(f, sc, tag);
+      if constexpr ((S + 1) % KS == 0) {
+        ++sl;
+        slot = slot + 1 == NS ? 0 : slot + 1;
+      }
     };
-    slice(std::integral_constant<int, 0>{});
-    slice(std::integral_constant<int, 1>{});
-    slice(std::integral_constant<int, 2>{});
-    slice(std::integral_constant<int, 3>{});
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 3>{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last refills, all out of range)
+
+  // epilogue, a row of y at a time: a lane's pieces of it are 64 bytes apart, so a row's stores (and residual loads) complete lines
+  float bias[WT / 2][8];
 #pragma unroll
-  for (int i = 0; i < WT / 2; ++i) {
-    const int n = n0 + (wn * (WT / 2) + i) * 32 + g * 8;
-    if (n >= a.n) break;
-    float bias[8];
+  for (int i = 0; i < WT / 2; ++i)
 #pragma unroll
-    for (int q = 0; q < 8; ++q) bias[q] = a.bias && n + q < a.n ? a.bias[n + q] : 0.f;
+    for (int q = 0; q < 8; ++q) {
+      const int n = n0 + (wn * (WT / 2) + i) * 32 + g * 8 + q;
+      bias[i][q] = a.bias && n < a.n ? a.bias[n] : 0.f;
+    }
 #pragma unroll
-    for (int j = 0; j < XT; ++j) {
-      const long long m = m0 + (wm * XT + j) * 16 + r;
-      if (m >= a.rows) break;
-      float v[8];
+  for (int j = 0; j < XT; ++j) {
+    const long long m = m0 + (wm * XT + j) * 16 + r;
+    if (m < a.rows) {
+      float rv[WT / 2][8];
+      if (a.res) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        v[q] = acc[2 * i][j][q];
-        v[4 + q] = acc[2 * i + 1][j][q];
+        for (int i = 0; i < WT / 2; ++i) {
+          const int n = n0 + (wn * (WT / 2) + i) * 32 + g * 8;
+          load8(static_cast<const T*>(a.res) + m * a.res_stride + n, a.n - n, a.vec, rv[i]);
+        }
       }
-      finish8<T>(a, v, bias, m, n);
+#pragma unroll
+      for (int i = 0; i < WT / 2; ++i) {
+        const int n = n0 + (wn * (WT / 2) + i) * 32 + g * 8;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          v[q] = acc[2 * i][j][q] + bias[i][q];
+          v[4 + q] = acc[2 * i + 1][j][q] + bias[i][4 + q];
+        }
+        if (a.act) silu8(v);
+        if (a.res) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] += rv[i][q];
+        }
+        store8(static_cast<T*>(a.y) + m * a.y_stride + n, a.n - n, a.vec, v);
+      }
     }
   }
 }
@@ -513,8 +600,8 @@ extern "C" int yl_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, in
 
 // ---- how a product runs: a wave per 16 x 16 tile for few rows, else tiles through LDS on the pipe's own order of the scales
 struct Plan {
-  bool tiled;
-  int wt, xt;                    // tiles per wave
+  bool tiled, big;
+  int wt, xt;                    // split over k: 16-row tiles of a workgroup
   long long ntiles, mtiles;
   long long codes, xs, ws, all;  // bytes: codes of x, scales of x, tiled scales of the weight, the workspace
   long long xgroups, wgroups, k4;
@@ -523,29 +610,43 @@ struct Plan {
 static Plan plan_linear(int x_dtype, long long rows, long long n, long long k) {
   Plan p{};
   const long long kb = (k + 31) / 32;
-  p.tiled = rows > 32;
   p.codes = x_dtype == YL_MX4 ? 0 : (rows * kb * 16 + 255) / 256 * 256;
+  const long long tiles128 = ((n + 127) / 128) * ((rows + 127) / 128), tiles256 = ((n + 255) / 256) * ((rows + 255) / 256);
+  // Measured, kernel alone, tiles of 128 against the split form: 64 x 768 x 768 6.8 / 5.4 us, 400 x 768 x 768 (24 tiles) 7.0 / 5.8,
+  // 256 x 1024 x 4096 (16 tiles) 15.2 / 14.8, 33 x 8192 x 8192 25 / 20; 128 x 4096 x 4096 (32 tiles) 15.6 / 15.1,
+  // 1600 x 768 x 768 (78) 7.5 / 11, 512 x 4096 x 4096 (128) 16.5 / 48.
+  p.tiled = rows > 64 && tiles128 >= 32;
   if (p.tiled) {
-    p.wt = p.xt = 8;
-    if (((n + 255) / 256) * ((rows + 255) / 256) < 192) p.wt = p.xt = 4;
-    p.ntiles = (n + 32 * p.wt - 1) / (32 * p.wt), p.mtiles = (rows + 32 * p.xt - 1) / (32 * p.xt);
+    // tiles of 128: three workgroups on a CU hide each other's prologue and epilogue, tiles of 256 move half the bytes.  Measured,
+    // tiles of 128 / 256: 204800 x 384 x 384 53 / 81 us, 51200 x 384 x 768 24 / 32; 4096^3 50 / 41, 16384 x 4096 x 4096 232 / 191.
+    p.big = tiles256 >= 192 && kb >= 32;
+    const int tile = p.big ? 256 : 128;
+    p.ntiles = (n + tile - 1) / tile, p.mtiles = (rows + tile - 1) / tile;
     p.k4 = (kb + 15) / 16, p.xgroups = (rows + 63) / 64, p.wgroups = (n + 63) / 64;
     p.xs = p.k4 * p.xgroups * 1024, p.ws = p.k4 * p.wgroups * 1024;
   } else {
-    p.wt = p.xt = 1;
-    p.ntiles = (n + 15) / 16, p.mtiles = (rows + 15) / 16;
+    p.wt = rows <= 32 ? 1 : 2;
+    p.xt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    p.ntiles = (n + 16 * p.wt - 1) / (16 * p.wt), p.mtiles = (rows + 16 * p.xt - 1) / (16 * p.xt);
     p.xs = x_dtype == YL_MX4 ? 0 : (rows * kb + 255) / 256 * 256;
   }
   p.all = p.codes + p.xs + p.ws;
   return p;
 }
 
-template <typename T, int WT, int XT>
+template <typename T, int WT, int XT, int NWM, int KS, int NS>
 static int gemm_launch(const LinearArgs& a, hipStream_t s) {
-  auto kern = mx4_gemm_kernel<T, WT, XT>;
-  const int lds = 4 * (2 * WT + 2 * XT) * 1024;
+  auto kern = mx4_gemm_kernel<T, WT, XT, NWM, KS, NS>;
+  const int lds = NS * KS * (2 * WT + NWM * XT) * 1024;
   if (int rc = allow_big_lds(reinterpret_cast<const void*>(kern), lds)) return rc;
-  hipLaunchKernelGGL(kern, dim3((unsigned)a.ntiles * (unsigned)a.mtiles), dim3(256), lds, s, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)a.ntiles * (unsigned)a.mtiles), dim3(128 * NWM), lds, s, a);
+  YL_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T, int WT, int XT, int NW>
+static int split_launch(const LinearArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((mx4_split_kernel<T, WT, XT, NW>), dim3((unsigned)a.ntiles * (unsigned)a.mtiles), dim3(64 * NW), 0, s, a);
   YL_HIP(hipGetLastError());
   return 0;
 }
@@ -591,10 +692,9 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
     if (!packed)
       if (int rc = quantize_launch(x, x_dtype, rows, k, x_stride, codes, xs, s)) return rc;
     return by_type(y_dtype, [&](auto* t) {
-      hipLaunchKernelGGL(mx4_product_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)(p.ntiles * p.mtiles)), dim3(64), 0, s, a,
-                         (int)p.ntiles);
-      YL_HIP(hipGetLastError());
-      return 0;
+      typedef std::remove_pointer_t<decltype(t)> T;
+      if (p.xt == 1) return split_launch<T, 1, 1, 8>(a, s);
+      return p.xt == 2 ? split_launch<T, 1, 2, 8>(a, s) : split_launch<T, 2, 4, 8>(a, s);
     });
   }
   TileArgs ta{};
@@ -603,7 +703,7 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
   ta.q.codes = packed ? nullptr : codes, ta.q.scales = const_cast<uint8_t*>(x_scales);
   ta.xs = xs, ta.ws = w_scales, ta.wst = xs + p.xs, ta.n = (int)n, ta.xgroups = a.xgroups, ta.wgroups = a.wgroups;
   if (int rc = by_type(packed ? YL_BF16 : x_dtype, [&](auto* t) {
-        hipLaunchKernelGGL(mx4_tile_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)p.k4, (unsigned)(p.xgroups + p.wgroups)), dim3(256), 0,
+        hipLaunchKernelGGL(mx4_tile_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)p.k4, (unsigned)(p.xgroups + p.wgroups)), dim3(1024), 0,
                            s, ta);
         YL_HIP(hipGetLastError());
         return 0;
@@ -612,6 +712,6 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
   a.xs = ta.xs, a.ws = ta.wst;
   return by_type(y_dtype, [&](auto* t) {
     typedef std::remove_pointer_t<decltype(t)> T;
-    return p.wt == 8 ? gemm_launch<T, 8, 8>(a, s) : gemm_launch<T, 4, 4>(a, s);
+    return p.big ? gemm_launch<T, 8, 4, 4, 2, 2>(a, s) : gemm_launch<T, 4, 4, 2, 1, 3>(a, s);
   });
 }
