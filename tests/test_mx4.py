@@ -49,7 +49,7 @@ def test_quantize_refusals(change, code):
     assert L.yl_mx4_dequantize(*a.values()) == code and b"mx4_dequantize" in L.yl_last_error()
 
 
-LINEAR = dict(x=_ptr(1), x_scales=None, x_dtype=0, rows=4, x_stride=64, w_codes=_ptr(2), w_scales=_ptr(3), n=16, k=64, bias=None, act=0,
+LINEAR = dict(x=_ptr(1), x_scales=None, x_dtype=0, rows=40, x_stride=64, w_codes=_ptr(2), w_scales=_ptr(3), n=16, k=64, bias=None, act=0,
               res=None, res_stride=0, y=_ptr(5), y_dtype=0, y_stride=16, work=_ptr(6), work_bytes=1 << 20, stream=None)
 
 

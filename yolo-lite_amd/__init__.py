@@ -31,7 +31,8 @@ def __getattr__(name):
         import importlib
 
         mod, attr = _LAZY[name]
-        return getattr(importlib.import_module(f"{__name__}.{mod}"), attr)
+        got = globals()[name] = getattr(importlib.import_module(f"{__name__}.{mod}"), attr)  # (the next access is a plain one)
+        return got
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 

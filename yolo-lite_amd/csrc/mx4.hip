@@ -73,25 +73,29 @@ __device__ __forceinline__ unsigned quad_max(unsigned m) {
   return m > o ? m : o;
 }
 
+// the scale byte of a block from its largest magnitude, the bits of |v| (inf and NaN are the largest)
+__device__ __forceinline__ unsigned scale_of(unsigned m) {
+  const unsigned e = m >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+__device__ __forceinline__ unsigned codes8(const float (&v)[8], unsigned s) {
+  const float x = __uint_as_float(s ? s << 23 : 0x00400000u);  // 2^(s - 127)
+  unsigned c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], x, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], x, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], x, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], x, 3);
+}
 // Four lanes hold a block, eight values each: -> this lane's eight codes (4 bytes), the block's scale byte.
 __device__ __forceinline__ unsigned quantize8(const float (&v)[8], unsigned* scale_byte) {
   unsigned m = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const unsigned b = __float_as_uint(v[j]) & 0x7FFFFFFFu;  // |v|, ordered as an integer; inf and NaN are the largest
+    const unsigned b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
     m = m > b ? m : b;
   }
-  m = quad_max(m);
-  const unsigned e = m >> 23;
-  const unsigned s = e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
-  const float x = __uint_as_float(s ? s << 23 : 0x00400000u);
-  unsigned c = 0;
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], x, 0);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], x, 1);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], x, 2);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], x, 3);
-  *scale_byte = s;
-  return c;
+  *scale_byte = scale_of(quad_max(m));
+  return codes8(v, *scale_byte);
 }
 
 // the float 2^(s - 127); NaN for 255.  (2^-127 is not a normal number: its own bit pattern.)
@@ -115,6 +119,28 @@ __device__ __forceinline__ Item item_of(unsigned long long i, unsigned per_row) 
     t.c8 = (int)(i - (unsigned long long)t.row * per_row);
   }
   return t;
+}
+
+// One lane holds a whole block: 32 values from p (zeros from the n-th on) -> the 16 bytes of codes, the scale byte.
+template <typename T>
+__device__ __forceinline__ v4i quantize32(const T* p, int n, bool vec, int* scale_byte) {
+  float v[4][8];
+  unsigned m = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    load8(p + q * 8, n - q * 8, vec, v[q]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const unsigned b = __float_as_uint(v[q][j]) & 0x7FFFFFFFu;
+      m = m > b ? m : b;
+    }
+  }
+  const unsigned s = scale_of(m);
+  v4i c;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) c[q] = (int)codes8(v[q], s);
+  *scale_byte = (int)s;
+  return c;
 }
 
 struct QuantArgs {
@@ -159,7 +185,10 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(QuantArgs a, T* y) 
 
 // ------------------------------------------------------------------------------------------------ product
 struct LinearArgs {
-  const uint8_t *xc, *xs;  // activations: codes, scales
+  const void* x;           // activations: codes (or, for few rows, values), row stride in elements of what it is
+  long long x_stride;
+  int xvec;                // values: every group of eight starts on 16 bytes
+  const uint8_t* xs;       // scales
   const uint8_t *wc, *ws;  // weight
   long long rows;
   int n, k, kb;
@@ -176,17 +205,39 @@ struct LinearArgs {
 
 __device__ __forceinline__ v8i widen(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
-// y[m][n .. n + 4): bias, SiLU, residual, one rounding
+// y[m][n .. n + 4): bias, SiLU, residual, one rounding (everything is loaded before anything is used)
 template <typename T>
-__device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 acc, long long m, int n) {
+__device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 v, long long m, int n) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  const int left = a.n - n;
+  const T* rp = static_cast<const T*>(a.res) + m * a.res_stride + n;
+  T* yp = static_cast<T*>(a.y) + m * a.y_stride + n;
+  const bool vec = a.vec && left >= 4;
+  float bias[4], res[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) bias[r] = a.bias && r < left ? a.bias[n + r] : 0.f;
+  if (a.res) {
+    if (vec) {
+      const t4 q = *reinterpret_cast<const t4*>(rp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) res[r] = (float)q[r];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) res[r] = r < left ? (float)rp[r] : 0.f;
+    }
+  }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    if (n + r >= a.n) break;
-    float v = acc[r];
-    if (a.bias) v += a.bias[n + r];
-    if (a.act) v = silu_f(v);
-    if (a.res) v += (float)static_cast<const T*>(a.res)[m * a.res_stride + n + r];
-    static_cast<T*>(a.y)[m * a.y_stride + n + r] = (T)v;
+    v[r] += bias[r];
+    if (a.act) v[r] = silu_f(v[r]);
+    if (a.res) v[r] += res[r];
+  }
+  if (vec) {
+    *reinterpret_cast<t4*>(yp) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < left) yp[r] = (T)v[r];
   }
 }
 
@@ -194,14 +245,18 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 acc, long lon
 // Few rows: the product is the time it takes to read the weight (one row of x: 0.53 bytes per multiply-add), and a grid of large
 // tiles would leave most of the chip idle.  A workgroup owns 16 WT weight rows x 16 XT rows of x; its NW waves take the k-steps in
 // turn, operands straight from memory into registers, and the partial sums meet in LDS in a fixed order.
-template <typename T, int WT, int XT, int NW>
+// X: what x is: codes (uint8_t), or the values themselves -- a lane's part of the operand is one row's block of 32, so each lane
+// quantises its own, without a launch, a workspace or an exchange (16 rows; every workgroup does it again, under the weight's loads).
+template <typename T, typename X, int WT, int XT, int NW>
 __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
   __shared__ __attribute__((aligned(16))) f32x4 part[NW][WT * XT][64];
   const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int n0 = (int)(blockIdx.x % (unsigned)a.ntiles) * (16 * WT);
   const long long m0 = (long long)(blockIdx.x / (unsigned)a.ntiles) * (16 * XT);
-  const uint8_t *wp[WT], *wsp[WT], *xp[XT], *xsp[XT];
+  constexpr bool CODES = std::is_same_v<X, uint8_t>;
+  const uint8_t *wp[WT], *wsp[WT], *xsp[XT];
+  const X* xp[XT];
 #pragma unroll
   for (int i = 0; i < WT; ++i) {  // rows behind the last: the last one's values, not stored
     const long long row = min(n0 + i * 16 + r, a.n - 1);
@@ -211,7 +266,7 @@ __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
 #pragma unroll
   for (int j = 0; j < XT; ++j) {
     const long long row = min(m0 + j * 16 + r, a.rows - 1);
-    xp[j] = a.xc + row * a.kb * 16;
+    xp[j] = static_cast<const X*>(a.x) + row * a.x_stride;
     xsp[j] = a.xs + row * a.kb;
   }
   f32x4 acc[WT][XT];
@@ -237,8 +292,12 @@ __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < XT; ++j) {
-        x[u][j] = *reinterpret_cast<const v4i*>(xp[j] + (long long)bb * 16);
-        sx[u][j] = in ? xsp[j][bb] : 127;
+        if constexpr (CODES) {
+          x[u][j] = *reinterpret_cast<const v4i*>(xp[j] + (long long)bb * 16);
+          sx[u][j] = in ? xsp[j][bb] : 127;
+        } else {
+          x[u][j] = quantize32(xp[j] + (long long)bb * 32, in ? a.k - bb * 32 : 0, a.xvec, &sx[u][j]);
+        }
       }
     }
 #pragma unroll
@@ -376,7 +435,7 @@ __global__ __launch_bounds__(128 * NWM, 2) void mx4_gemm_kernel(LinearArgs a) {
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
       (void*)(a.wc + (long long)n0 * pitch), (short)0, (unsigned)min(TN, a.n - n0) * (unsigned)pitch, 0x00020000);
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(a.xc + m0 * pitch), (short)0, (unsigned)min((long long)TM, a.rows - m0) * (unsigned)pitch, 0x00020000);
+      (void*)(static_cast<const uint8_t*>(a.x) + m0 * pitch), (short)0, (unsigned)min((long long)TM, a.rows - m0) * (unsigned)pitch, 0x00020000);
   const int nk = (a.kb + 3) >> 2;            // k-steps
   // the permutation of a row's blocks, and this lane's part of a piece: row lane / (4 KS), block (lane mod 4 KS) permuted
   auto swz = [](int row) { return KS == 1 ? -(row >> 2) & 3 : (row >> 1) & 7; };
@@ -628,7 +687,8 @@ static Plan plan_linear(int x_dtype, long long rows, long long n, long long k) {
     p.wt = rows <= 32 ? 1 : 2;
     p.xt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
     p.ntiles = (n + 16 * p.wt - 1) / (16 * p.wt), p.mtiles = (rows + 16 * p.xt - 1) / (16 * p.xt);
-    p.xs = x_dtype == YL_MX4 ? 0 : (rows * kb + 255) / 256 * 256;
+    if (p.xt == 1) p.codes = 0;  // (x is quantised where it is read)
+    p.xs = x_dtype == YL_MX4 || p.xt == 1 ? 0 : (rows * kb + 255) / 256 * 256;
   }
   p.all = p.codes + p.xs + p.ws;
   return p;
@@ -644,9 +704,9 @@ static int gemm_launch(const LinearArgs& a, hipStream_t s) {
   return 0;
 }
 
-template <typename T, int WT, int XT, int NW>
+template <typename T, typename X, int WT, int XT, int NW>
 static int split_launch(const LinearArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_split_kernel<T, WT, XT, NW>), dim3((unsigned)a.ntiles * (unsigned)a.mtiles), dim3(64 * NW), 0, s, a);
+  hipLaunchKernelGGL((mx4_split_kernel<T, X, WT, XT, NW>), dim3((unsigned)a.ntiles * (unsigned)a.mtiles), dim3(64 * NW), 0, s, a);
   YL_HIP(hipGetLastError());
   return 0;
 }
@@ -686,20 +746,29 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
   uint8_t* const codes = static_cast<uint8_t*>(work);
   uint8_t* const xs = codes + p.codes;
   const bool packed = x_dtype == YL_MX4;
-  a.xc = packed ? static_cast<const uint8_t*>(x) : codes;
+  const int xvec = !packed && aligned16(x) && (rows == 1 || x_stride * elem_bytes(x_dtype) % 16 == 0);
+  a.x = packed ? x : codes, a.x_stride = 16LL * a.kb;
   if (!p.tiled) {
     a.xs = packed ? x_scales : xs;
+    if (!packed && p.xt == 1) {
+      a.x = x, a.x_stride = x_stride, a.xvec = xvec;
+      return by_type(y_dtype, [&](auto* t) {
+        return by_type(x_dtype, [&](auto* u) {
+          return split_launch<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(u)>, 1, 1, 8>(a, s);
+        });
+      });
+    }
     if (!packed)
       if (int rc = quantize_launch(x, x_dtype, rows, k, x_stride, codes, xs, s)) return rc;
     return by_type(y_dtype, [&](auto* t) {
       typedef std::remove_pointer_t<decltype(t)> T;
-      if (p.xt == 1) return split_launch<T, 1, 1, 8>(a, s);
-      return p.xt == 2 ? split_launch<T, 1, 2, 8>(a, s) : split_launch<T, 2, 4, 8>(a, s);
+      if (p.xt == 1) return split_launch<T, uint8_t, 1, 1, 8>(a, s);
+      return p.xt == 2 ? split_launch<T, uint8_t, 1, 2, 8>(a, s) : split_launch<T, uint8_t, 2, 4, 8>(a, s);
     });
   }
   TileArgs ta{};
   ta.q.x = x, ta.q.rows = rows, ta.q.stride = x_stride, ta.q.cols = (int)k, ta.q.kb = a.kb;
-  ta.q.vec = aligned16(x) && x_stride * elem_bytes(x_dtype) % 16 == 0;
+  ta.q.vec = xvec;
   ta.q.codes = packed ? nullptr : codes, ta.q.scales = const_cast<uint8_t*>(x_scales);
   ta.xs = xs, ta.ws = w_scales, ta.wst = xs + p.xs, ta.n = (int)n, ta.xgroups = a.xgroups, ta.wgroups = a.wgroups;
   if (int rc = by_type(packed ? YL_BF16 : x_dtype, [&](auto* t) {

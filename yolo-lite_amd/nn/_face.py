@@ -1,4 +1,5 @@
-"""What the Python faces of the direct C entry points (``nn/mx4.py``, ``nn/block_attention.py``) share."""
+"""What the Python faces of the direct C entry points (``nn/mx4.py``, ``nn/block_attention.py``) share.  A small call is bound by the
+host (an allocation and a launch are 2-4 us each), so the checks are a few attribute reads and the message is made when one fails."""
 from __future__ import annotations
 
 from typing import Optional
@@ -8,27 +9,34 @@ import torch
 from .. import _lib
 
 
-def on_gpu(what: str, *tensors: Optional[torch.Tensor]) -> torch.device:
-    dev = None
+def on_gpu(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """The index of the one GPU all of the tensors are on; raises for tensors elsewhere, on two GPUs, or that want a gradient."""
+    at = -1
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
-            raise RuntimeError(f"{what} runs on the GPU only (HIP kernel, no CPU fallback)")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on different devices ({dev} and {t.device})")
-        dev = t.device
-    return dev
+        d = t.get_device()
+        if d < 0 or (at >= 0 and d != at) or t.requires_grad:
+            _refuse(what, at, t)
+        at = d
+    return at
 
 
-def call(dev: torch.device, fn, what: str, *args) -> None:
+def _refuse(what: str, at: int, t: torch.Tensor) -> None:
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{what} runs on the GPU only (HIP kernel, no CPU fallback)")
+    if at >= 0 and t.device.index != at:
+        raise ValueError(f"{what}: tensors on different devices (cuda:{at} and {t.device})")
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
+
+
+def call(dev: int, fn, what: str, *args) -> None:
     """fn(*args, stream) with ``dev`` as the current device, on its current stream."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, what)

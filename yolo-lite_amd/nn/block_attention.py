@@ -46,10 +46,10 @@ def _check(what: str, q: torch.Tensor, k: torch.Tensor, mask: Optional[torch.Ten
     return mask
 
 
-def _workspace(what: str, nbytes: int, dev: torch.device):
+def _workspace(what: str, nbytes: int, like: torch.Tensor):
     if nbytes < 0:
         _lib.check(-3, what)
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def block_select(q: torch.Tensor, k: torch.Tensor, block: int = 64, topk: int = 8, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -62,10 +62,10 @@ def block_select(q: torch.Tensor, k: torch.Tensor, block: int = 64, topk: int = 
     nk, kv = k.shape[1], k.shape[2]
     L = _lib.lib()
     nbytes = L.yl_block_select_workspace_bytes(batch, nq, nk, heads, kv, dk, block)
-    work = _workspace("block_select", nbytes, dev)
+    work = _workspace("block_select", nbytes, q)
     q, qh = _heads(q)
     k, kh = _heads(k)
-    picked = torch.empty((batch, kv, nq, topk), dtype=torch.int32, device=dev)
+    picked = q.new_empty((batch, kv, nq, topk), dtype=torch.int32)
     call(dev, L.yl_block_select, "block_select", byref(qh), byref(kh), _TYPES[q.dtype], batch, nq, nk, heads, kv, dk, block, topk,
          mask.data_ptr() if mask is not None else None, mask.stride(0) if mask is not None else 0, picked.data_ptr(),
          work.data_ptr() if work is not None else None, nbytes)
@@ -89,12 +89,12 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, picked: t
     dv, topk = v.shape[3], picked.shape[3]
     L = _lib.lib()
     nbytes = L.yl_block_attention_workspace_bytes(batch, nq, nk, heads, kv, dk, dv, block, topk)
-    work = _workspace("block_attention", nbytes, dev)
+    work = _workspace("block_attention", nbytes, q)
     q, qh = _heads(q)
     k, kh = _heads(k)
     v, vh = _heads(v)
     picked = picked.contiguous()
-    out = torch.empty((batch, nq, heads, dv), dtype=q.dtype, device=dev)
+    out = q.new_empty((batch, nq, heads, dv))
     oh = _lib.Heads(out.data_ptr(), out.stride(0), out.stride(1), out.stride(2))
     call(dev, L.yl_block_attention, "block_attention", byref(qh), byref(kh), byref(vh), _TYPES[q.dtype], batch, nq, nk, heads, kv, dk, dv,
          block, topk, picked.data_ptr(), mask.data_ptr() if mask is not None else None, mask.stride(0) if mask is not None else 0,

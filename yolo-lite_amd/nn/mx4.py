@@ -47,7 +47,7 @@ def _dense(what: str, t: Mx4Tensor):
         raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold {cols} columns")
     if not codes.is_contiguous() or codes.data_ptr() % 16:
         codes = codes.clone(memory_format=torch.contiguous_format)
-    return codes, scales.contiguous()
+    return codes, scales if scales.is_contiguous() else scales.contiguous()
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
@@ -61,8 +61,8 @@ def mx4_quantize(x: torch.Tensor) -> Mx4Tensor:
     lead, cols = x.shape[:-1], x.shape[-1]
     kb = (cols + BLOCK - 1) // BLOCK
     x = _rows(x)
-    codes = torch.empty((*lead, kb * 16), dtype=torch.uint8, device=dev)
-    scales = torch.empty((*lead, kb), dtype=torch.uint8, device=dev)
+    codes = x.new_empty((*lead, kb * 16), dtype=torch.uint8)
+    scales = x.new_empty((*lead, kb), dtype=torch.uint8)
     _call(dev, _lib.lib().yl_mx4_quantize, "mx4_quantize", x.data_ptr(), _TYPES[x.dtype], x.shape[0], cols, max(x.stride(0), cols),
           codes.data_ptr(), scales.data_ptr())
     return Mx4Tensor(codes, scales, cols)
@@ -74,7 +74,7 @@ def mx4_dequantize(t: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
     if dtype not in _TYPES:
         raise TypeError(f"mx4_dequantize: bf16, fp16 or fp32 values, got {dtype}")
     codes, scales = _dense("mx4_dequantize", t)
-    y = torch.empty((*codes.shape[:-1], t.cols), dtype=dtype, device=dev)
+    y = codes.new_empty((*codes.shape[:-1], t.cols), dtype=dtype)
     _call(dev, _lib.lib().yl_mx4_dequantize, "mx4_dequantize", codes.data_ptr(), scales.data_ptr(), y.numel() // t.cols, t.cols,
           y.data_ptr(), _TYPES[dtype], t.cols)
     return y
@@ -121,17 +121,18 @@ def mx4_linear(x: Union[torch.Tensor, Mx4Tensor], w: Mx4Tensor, bias: Optional[t
     if bias is not None:
         if bias.shape != (n,):
             raise ValueError(f"mx4_linear: a bias of shape {tuple(bias.shape)} for {n} output columns")
-        bias = bias.float().contiguous()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
     if res is not None:
         if res.shape != (*lead, n) or res.dtype != dtype:
             raise ValueError(f"mx4_linear: a residual {tuple(res.shape)} in {res.dtype} for a result {(*lead, n)} in {dtype}")
         res = _rows(res)
-    y = torch.empty((*lead, n), dtype=dtype, device=dev)
+    y = wc.new_empty((*lead, n), dtype=dtype)
     L = _lib.lib()
     nbytes = L.yl_mx4_linear_workspace_bytes(in_type, rows, n, k)
     if nbytes < 0:
         _lib.check(-3, "mx4_linear")
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    work = wc.new_empty(nbytes) if nbytes else None
     _call(dev, L.yl_mx4_linear, "mx4_linear", xt.data_ptr(), xs.data_ptr() if xs is not None else None, in_type, rows, stride,
           wc.data_ptr(), ws.data_ptr(), n, k, bias.data_ptr() if bias is not None else None, int(bool(act)),
           res.data_ptr() if res is not None else None, max(res.stride(0), n) if res is not None else 0, y.data_ptr(), _TYPES[dtype], n,
