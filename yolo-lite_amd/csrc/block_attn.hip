@@ -34,46 +34,123 @@ struct BlockArgs {
   const uint8_t* mask;  // [batch][nk], row stride mask_stride; nullptr: every key may be read
   long long mask_stride;
   float scale;
-  double* mean;   // [batch][kv][dk][nb]
+  double* mean;   // [batch][kv][nb][dk]
+  double* score;  // few queries: [batch][kv][nq][nb]
+  __bf16* split;  // [batch][kv][nbp][2][dkp]: the means as two bf16; nbp = nb rounded up to 16, dkp = dk to 32
+  float* norm;    // [batch][kv][nb]: 2-norm of a mean
+  int nbp, dkp;
   int* count;     // [batch][nb]: unmasked keys of a block
   int* picked;    // [batch][kv][nq][topk]
 };
 
 // ------------------------------------------------------------------------------------------------ block means
-// One workgroup per (image, kv head, block): thread = (key lane, 8 dims).
-template <typename T>
+// value x as two bf16: x = hi + lo up to 2^-18 |x|
+__device__ __forceinline__ void split2(float x, __bf16* hi, __bf16* lo) {
+  *hi = (__bf16)x;
+  *lo = (__bf16)(x - (float)*hi);
+}
+__device__ __forceinline__ double shfl_xor_d(double x, int o) { return __shfl_xor(x, o); }
+
+// One wave per (image, kv head, block): lane = (key lane, 8 dims), 64 / CP key lanes (CP: dk / 8 rounded up to a power of two); the
+// lanes of a dim chunk exchange halves, then quarters, ... of their sums, so a wave reduces with 7 exchanges instead of 24.
+// SCORE: few queries -- the wave that has a block's mean also scores it, and no mean is stored.
+template <typename T, int CP, bool SCORE>
 __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
-  __shared__ double sum[256 * 8];
-  __shared__ int cnt;
-  const int j = blockIdx.x % a.nb, bh = blockIdx.x / a.nb, h = bh % a.kv, b = bh / a.kv;
-  const int C = a.dk >> 3, KL = 256 / C;
-  const int c = threadIdx.x % C, kl = threadIdx.x / C;
-  const int k0 = j * a.block, kn = min(a.block, a.nk - k0);
-  if (threadIdx.x == 0) cnt = 0;
-  __syncthreads();
-  double acc[8] = {};
-  int mine = 0;
   typedef T t8 __attribute__((ext_vector_type(8)));
-  if (kl < KL)
-    for (int i = kl; i < kn; i += KL) {
-      if (a.mask && !a.mask[b * a.mask_stride + k0 + i]) continue;
-      ++mine;
-      const t8 x = *reinterpret_cast<const t8*>(static_cast<const T*>(a.k.p) + b * a.k.sb + (long long)(k0 + i) * a.k.st + h * a.k.sh + c * 8);
+  constexpr int KL = 64 / CP;
+  const int lane = threadIdx.x & 63;
+  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= (long long)a.batch * a.kv * a.nb) return;
+  const int j = (int)(unit % a.nb), bh = (int)(unit / a.nb), h = bh % a.kv, b = bh / a.kv;
+  const int c = lane % CP, kl = lane / CP;
+  const int k0 = j * a.block, kn = min(a.block, a.nk - k0);
+  const T* kp = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh + c * 8;
+  const uint8_t* mp = a.mask ? a.mask + b * a.mask_stride + k0 : nullptr;
+  double acc[8] = {};
+  int n = 0;
+  for (int i0 = kl; i0 < kn; i0 += 8 * KL) {  // eight keys of a lane in flight
+    t8 x[8];
+    bool ok[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += (double)(float)x[e];
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * KL;
+      ok[u] = i < kn && (!mp || mp[i]);
+      x[u] = t8{};
+      if (ok[u] && c * 8 < a.dk) x[u] = *reinterpret_cast<const t8*>(kp + (long long)(k0 + i) * a.k.st);
     }
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (kl < KL) sum[(kl * C + c) * 8 + e] = acc[e];
-  if (c == 0 && mine) atomicAdd(&cnt, mine);  // (whole numbers: the order does not matter)
-  __syncthreads();
-  const int n = cnt;
-  for (int d = threadIdx.x; d < a.dk; d += 256) {
-    double s = 0;
-    for (int i = 0; i < KL; ++i) s += sum[i * a.dk + d];
-    a.mean[((long long)bh * a.dk + d) * a.nb + j] = n ? s / n : 0.0;
+    for (int u = 0; u < 8; ++u) {
+      n += ok[u];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += (double)(float)x[u][e];
+    }
   }
-  if (h == 0 && threadIdx.x == 0) a.count[b * a.nb + j] = n;
+#pragma unroll
+  for (int o = CP; o < 64; o <<= 1) n += __shfl_xor(n, o);
+  // lane bits CP, 2 CP, 4 CP: the partner's half of the dims comes here, the other half goes there
+  int d0 = 0;
+#pragma unroll
+  for (int step = 0; step < 3; ++step) {
+    const int o = CP << step, half = 4 >> step;
+    if (o < 64) {
+      const bool up = lane & o;
+#pragma unroll
+      for (int e = 0; e < half; ++e) {
+        const double give = up ? acc[e] : acc[half + e], keep = up ? acc[half + e] : acc[e];
+        acc[e] = keep + shfl_xor_d(give, o);
+      }
+      d0 += up ? half : 0;
+    }
+  }
+#pragma unroll
+  for (int o = CP * 8; o < 64; o <<= 1) acc[0] += shfl_xor_d(acc[0], o);  // (all eight dims are one per lane by now)
+  constexpr int LEFT = CP == 16 ? 2 : 1;  // dims a lane ends up with
+  const bool mine = kl < 8 && c * 8 < a.dk;
+  double mean[LEFT];
+#pragma unroll
+  for (int e = 0; e < LEFT; ++e) mean[e] = n ? acc[e] / n : 0.0;
+  if constexpr (SCORE) {
+    for (int i = 0; i < a.nq; ++i) {
+      double s = 0;
+      if (mine)
+#pragma unroll
+        for (int e = 0; e < LEFT; ++e) {
+          double q = 0;
+          for (int g = 0; g < a.group; ++g)
+            q += (double)(float)(static_cast<const T*>(a.q.p) + b * a.q.sb + i * a.q.st + (long long)(h * a.group + g) * a.q.sh)[c * 8 + d0 + e];
+          s += q * mean[e];
+        }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) s += shfl_xor_d(s, o);
+      if (lane == 0) a.score[((long long)bh * a.nq + i) * a.nb + j] = n ? s : __builtin_nan("");
+    }
+    if (lane == 0 && h == 0) a.count[b * a.nb + j] = n;
+  } else {
+    float norm = 0.f;
+    if (mine)
+#pragma unroll
+      for (int e = 0; e < LEFT; ++e) {
+        const int d = c * 8 + d0 + e;
+        a.mean[((long long)bh * a.nb + j) * a.dk + d] = mean[e];
+        const float f = (float)mean[e];
+        __bf16 hi, lo;
+        split2(f, &hi, &lo);
+        __bf16* at = a.split + ((long long)bh * a.nbp + j) * (2 * a.dkp) + d;
+        at[0] = hi;
+        at[a.dkp] = lo;
+        norm += f * f;
+      }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) norm += __shfl_xor(norm, o);
+    if (lane < a.dkp - a.dk) {  // the dims behind the last: zeros
+      __bf16* at = a.split + ((long long)bh * a.nbp + j) * (2 * a.dkp) + a.dk + lane;
+      at[0] = at[a.dkp] = (__bf16)0.f;
+    }
+    if (lane == 0) {
+      a.norm[(long long)bh * a.nb + j] = sqrtf(norm);
+      if (h == 0) a.count[b * a.nb + j] = n;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ selection
@@ -84,70 +161,324 @@ __device__ __forceinline__ unsigned long long order_key(double s, bool can) {
   const unsigned long long b = (unsigned long long)__double_as_longlong(s + 0.0);
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
+// sum over the 64 lanes, the same in all of them (row shifts, row broadcasts: no LDS round trips)
+__device__ __forceinline__ int wave_sum(int c) {
+  c += __builtin_amdgcn_update_dpp(0, c, 0x111, 0xF, 0xF, false);
+  c += __builtin_amdgcn_update_dpp(0, c, 0x112, 0xF, 0xF, false);
+  c += __builtin_amdgcn_update_dpp(0, c, 0x114, 0xF, 0xF, false);
+  c += __builtin_amdgcn_update_dpp(0, c, 0x118, 0xF, 0xF, false);
+  c += __builtin_amdgcn_update_dpp(0, c, 0x142, 0xA, 0xF, false);
+  c += __builtin_amdgcn_update_dpp(0, c, 0x143, 0xC, 0xF, false);
+  return __builtin_amdgcn_readlane(c, 63);
+}
 
-// One wave per (image, kv head, query): all scores in 64 bits, the topk-th largest by its bits, then the blocks at or over it.
+// One wave: key[nb] in LDS -> the n-th largest by its bits, then the blocks at or over it in ascending order.
+__device__ __forceinline__ void pick_row(const unsigned long long* key, int nb, int topk, int lane, int* out) {
+  int can = 0;
+  unsigned long long any = 0, all = ~0ull;
+  for (int j = lane; j < nb; j += 64) {
+    const unsigned long long k = key[j];
+    can += k != 0;
+    any |= k;
+    all &= k;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    any |= __shfl_xor(any, o);
+    all &= __shfl_xor(all, o);
+  }
+  const int n = min(topk, wave_sum(can));
+  // bits that all keys share need no decision
+  const unsigned long long differ = any & ~all;
+  const int top = differ ? 63 - __clzll(differ) : -1;
+  unsigned long long v = top == 63 ? 0 : all & ~((2ull << (top < 0 ? 0 : top)) - 1);
+  if (top < 0) v = all;
+  int over = 0;  // keys > v
+  if (n > 0) {
+    bool exact = false;
+    for (int bit = top; bit >= 0 && !exact; --bit) {
+      const unsigned long long t = v | 1ull << bit;
+      int c = 0;
+#pragma unroll 4
+      for (int j = lane; j < nb; j += 64) c += key[j] >= t;
+      c = wave_sum(c);
+      if (c >= n) v = t;
+      exact = c == n;
+    }
+    int c = 0;
+    for (int j = lane; j < nb; j += 64) c += key[j] > v;
+    over = wave_sum(c);
+  }
+  int at = 0, ties = n - over;  // of the keys equal to v the first `ties` belong to the set
+  for (int j0 = 0; j0 < nb && n > 0; j0 += 64) {
+    const int j = j0 + lane;
+    const unsigned long long k = j < nb ? key[j] : 0;
+    const unsigned long long below = (1ull << lane) - 1;
+    const unsigned long long eq = __ballot(j < nb && k == v);
+    const bool take = (j < nb && k > v) || (j < nb && k == v && __popcll(eq & below) < ties);
+    ties -= min(ties, (int)__popcll(eq));
+    const unsigned long long got = __ballot(take);
+    if (take) out[at + __popcll(got & below)] = j;
+    at += __popcll(got);
+  }
+  for (int t = n + lane; t < topk; t += 64) out[t] = -1;
+}
+
+// One wave: the exact scores of one (image, kv head, query) from the 64-bit means, then pick_row.  qs: dk doubles, key: nb words of LDS.
 template <typename T>
-__global__ __launch_bounds__(64) void block_select_kernel(BlockArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char sel_sm[];
-  double* qs = reinterpret_cast<double*>(sel_sm);                                   // [dk]
-  unsigned long long* key = reinterpret_cast<unsigned long long*>(sel_sm) + a.dk;   // [nb]
-  const int lane = threadIdx.x;
-  const long long row = blockIdx.x;  // (b * kv + h) * nq + i
-  const int i = (int)(row % a.nq);
-  const int bh = (int)(row / a.nq), h = bh % a.kv, b = bh / a.kv;
+__device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int lane, double* qs, unsigned long long* key) {
+  const int h = bh % a.kv, b = bh / a.kv;
   for (int d = lane; d < a.dk; d += 64) {
     double s = 0;
     for (int g = 0; g < a.group; ++g)
       s += (double)(float)(static_cast<const T*>(a.q.p) + b * a.q.sb + i * a.q.st + (long long)(h * a.group + g) * a.q.sh)[d];
     qs[d] = s;
   }
-  __syncthreads();
-  int can = 0;
+  __builtin_amdgcn_wave_barrier();
   for (int j = lane; j < a.nb; j += 64) {
     double s = 0;
-    const double* m = a.mean + (long long)bh * a.dk * a.nb + j;
-    for (int d = 0; d < a.dk; ++d) s += qs[d] * m[(long long)d * a.nb];
-    const bool ok = a.count[b * a.nb + j] > 0;
-    can += ok;
-    key[j] = order_key(s, ok);
+    const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
+    for (int d = 0; d < a.dk; ++d) s += qs[d] * m[d];
+    key[j] = order_key(s, a.count[b * a.nb + j] > 0);
   }
-  __syncthreads();
-  auto total = [&](int c) {
+  __builtin_amdgcn_wave_barrier();
+  pick_row(key, a.nb, a.topk, lane, a.picked + ((long long)bh * a.nq + i) * a.topk);
+}
+
+// SCORED: the scores are there (few queries); else from the means.  One wave per (image, kv head, query).
+template <typename T, bool SCORED>
+__global__ __launch_bounds__(64) void block_select_kernel(BlockArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char sel_sm[];
+  unsigned long long* key = reinterpret_cast<unsigned long long*>(sel_sm);  // [nb]
+  const int lane = threadIdx.x;
+  const long long row = blockIdx.x;  // (b * kv + h) * nq + i
+  const int i = (int)(row % a.nq), bh = (int)(row / a.nq);
+  if constexpr (SCORED) {
+#pragma unroll 4
+    for (int j = lane; j < a.nb; j += 64) key[j] = order_key(a.score[row * a.nb + j], a.count[bh / a.kv * a.nb + j] > 0);
+    __syncthreads();
+    pick_row(key, a.nb, a.topk, lane, a.picked + row * a.topk);
+  } else {
+    exact_row<T>(a, bh, i, lane, reinterpret_cast<double*>(key + a.nb), key);
+  }
+}
+
+// Many queries, up to 16 NT blocks: a wave scores 16 queries at once on the matrix pipe, in less than 64 bits, and decides only what
+// that can decide.  q (summed over the group) and the means are split into two bf16 each; hi hi + hi lo + lo hi leaves out less than
+//   err = (3 * 2^-18 + 4 dk 2^-24) |q| |c|     (two splits, the product lo lo, an fp32 sum of 3 dk terms; |.| the 2-norms)
+// of a score (and, where a part is not a normal number any more, dk 2^-126 times the other norm; near the ends of fp32's range nothing
+// is decided here).  Lane (query n, group g) holds the scores of blocks 16 t + 4 g + r; the cut that leaves topk of them over it is found by
+// bisection, 16 queries in step.  Where the last block over the cut and the first under it are more than 2 err apart -- all but a
+// few in a thousand -- the order is the exact one's; the other queries (ties, NaN and infinities among them) are scored in 64 bits.
+template <typename T, int NT>
+__global__ __launch_bounds__(256) void block_score_kernel(BlockArgs a, int qtiles) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char sel_sm[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  unsigned long long* key = reinterpret_cast<unsigned long long*>(sel_sm) + (size_t)wave * (a.nb + a.dk);
+  const long long unit = (long long)xcd_remap((int)blockIdx.x, (int)gridDim.x) * 4 + wave;
+  if (unit >= (long long)a.batch * a.kv * qtiles) return;  // (no barrier below: waves are on their own)
+  const int qt = (int)(unit % qtiles), bh = (int)(unit / qtiles), h = bh % a.kv, b = bh / a.kv;
+  const int i = qt * 16 + n;
+  const bool live = i < a.nq;
+  const float ninf = -__builtin_huge_valf();
+  // which of this lane's blocks can be selected, how many there are, the largest |c|
+  int can = 0;
+  float big = 0.f;
+  for (int j = lane; j < a.nb; j += 64) {
+    can += a.count[b * a.nb + j] > 0;
+    big = fmaxf(big, a.norm[(long long)bh * a.nb + j]);
+    if (!(a.norm[(long long)bh * a.nb + j] < __builtin_huge_valf())) big = __builtin_huge_valf();
+  }
+  can = wave_sum(can);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) c += __shfl_xor(c, o);
-    return c;
-  };
-  const int n = min(a.topk, total(can));
-  unsigned long long v = 0;
-  int over = 0;  // keys > v that are taken whatever their index
-  if (n > 0) {
-    bool exact = false;
-    for (int bit = 63; bit >= 0 && !exact; --bit) {
-      const unsigned long long t = v | 1ull << bit;
-      int c = 0;
-      for (int j = lane; j < a.nb; j += 64) c += key[j] >= t;
-      c = total(c);
-      if (c >= n) v = t;
-      exact = c == n;
+  for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
+  const int take = min(a.topk, can);
+
+  f32x4 s[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float qq = 0.f;
+  const __bf16* sp = a.split + (long long)bh * a.nbp * (2 * a.dkp);
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  for (int c0 = 0; c0 < a.dkp; c0 += 32) {
+    const int c = c0 + g * 8;
+    float q[8] = {};
+    if (c < a.dk) {
+      for (int e = 0; e < a.group; ++e) {
+        const t8 x = *reinterpret_cast<const t8*>(static_cast<const T*>(a.q.p) + b * a.q.sb + (live ? i : 0) * a.q.st +
+                                                  (long long)(h * a.group + e) * a.q.sh + c);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) q[d] += (float)x[d];
+      }
     }
+    bf16x8 qh, ql;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      __bf16 hi, lo;
+      split2(q[d], &hi, &lo);
+      qh[d] = hi, ql[d] = lo;
+      qq += q[d] * q[d];
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (t * 16 >= a.nb) break;
+      const __bf16* m = sp + (long long)(t * 16 + n) * (2 * a.dkp) + c;
+      const bf16x8 mh = *reinterpret_cast<const bf16x8*>(m), ml = *reinterpret_cast<const bf16x8*>(m + a.dkp);
+      s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh, qh, s[t], 0, 0, 0);
+      s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml, qh, s[t], 0, 0, 0);
+      s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh, ql, s[t], 0, 0, 0);
+    }
+  }
+  qq += __shfl_xor(qq, 16);
+  qq += __shfl_xor(qq, 32);
+  const float qn = sqrtf(qq);
+  const float err = (3.f / 262144.f + 4.f * a.dk / 16777216.f) * qn * big + (qn + big) * 2e-36f + 1e-30f;
+
+  // blocks that cannot be selected (and places behind the last) go under every cut
+  unsigned okw[(NT + 7) / 8] = {};  // four bits per tile
+  float lo = __builtin_huge_valf(), hi = ninf;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = t * 16 + 4 * g + r;
+      const bool ok = j < a.nb && a.count[b * a.nb + (j < a.nb ? j : 0)] > 0;
+      okw[t >> 3] |= (unsigned)ok << ((t & 7) * 4 + r);
+      lo = ok ? fminf(lo, s[t][r]) : lo;
+      hi = ok ? fmaxf(hi, s[t][r]) : hi;
+      s[t][r] = ok ? s[t][r] : ninf;
+    }
+  lo = fminf(lo, __shfl_xor(lo, 16));
+  lo = fminf(lo, __shfl_xor(lo, 32));
+  hi = fmaxf(hi, __shfl_xor(hi, 16));
+  hi = fmaxf(hi, __shfl_xor(hi, 32));
+  // cut: more than `take` scores over lo, fewer over hi
+  float cut = ninf;
+  bool found = take == can;  // (everything that can be selected is: the cut stays at -inf)
+  lo -= (hi - lo) * 0.01f + 1e-30f;
+  for (int it = 0; it < 32 && __ballot(!found && live); ++it) {
+    const float mid = 0.5f * (lo + hi);
     int c = 0;
-    for (int j = lane; j < a.nb; j += 64) c += key[j] > v;
-    over = total(c);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c += s[t][r] > mid;
+    c += __shfl_xor(c, 16);
+    c += __shfl_xor(c, 32);
+    if (!found) {
+      if (c == take) {
+        found = true;
+        cut = mid;
+      } else if (c > take) {
+        lo = mid;
+      } else {
+        hi = mid;
+      }
+    }
   }
-  int* out = a.picked + row * a.topk;
-  int at = 0, ties = n - over;  // of the keys equal to v the first `ties` belong to the set
-  for (int j0 = 0; j0 < a.nb && n > 0; j0 += 64) {
-    const int j = j0 + lane;
-    const unsigned long long k = j < a.nb ? key[j] : 0;
-    const unsigned long long below = (1ull << lane) - 1;
-    const unsigned long long eq = __ballot(j < a.nb && k == v);
-    const bool take = (j < a.nb && k > v) || (j < a.nb && k == v && __popcll(eq & below) < ties);
-    ties -= min(ties, (int)__popcll(eq));
-    const unsigned long long all = __ballot(take);
-    if (take) out[at + __popcll(all & below)] = j;
-    at += __popcll(all);
+  // how far apart the two sides of the cut are
+  float in = __builtin_huge_valf(), out = ninf;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      in = s[t][r] > cut ? fminf(in, s[t][r]) : in;
+      out = s[t][r] > cut ? out : fmaxf(out, s[t][r]);
+    }
+  in = fminf(in, __shfl_xor(in, 16));
+  in = fminf(in, __shfl_xor(in, 32));
+  out = fmaxf(out, __shfl_xor(out, 16));
+  out = fmaxf(out, __shfl_xor(out, 32));
+  const bool sure = take == can || (found && qn * big < 1e37f && in - out > 2.f * err);  // (not so where anything is NaN)
+  // ascending block indices: bits of a tile of 16 blocks, all of them in every lane of a query
+  const float up = (found ? out : hi) + 2.f * err, dn = (found ? in : lo) - 2.f * err;
+  int* const row = a.picked + ((long long)bh * a.nq + i) * a.topk;
+  unsigned inw[(NT + 1) / 2] = {}, mayw[(NT + 1) / 2] = {};  // 32 blocks to a word: picked; where the order is not sure, over it / next to it
+  int at = 0, may = 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (t * 16 >= a.nb) break;
+    unsigned bits = 0;  // low half: picked (or over the band), high half: in the band
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool ok = okw[t >> 3] >> ((t & 7) * 4 + r) & 1;
+      const bool pick = take == can ? ok : sure ? s[t][r] > cut : s[t][r] > up;
+      bits |= (unsigned)pick << (4 * g + r);
+      bits |= (unsigned)(!sure && ok && s[t][r] <= up && s[t][r] >= dn) << (16 + 4 * g + r);
+    }
+    const unsigned own = bits;
+    bits |= __shfl_xor(bits, 16);
+    bits |= __shfl_xor(bits, 32);
+    if (sure && live) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (own >> (4 * g + r) & 1) row[at + __popc(bits & ((1u << (4 * g + r)) - 1))] = t * 16 + 4 * g + r;
+    }
+    at += __popc(bits & 0xFFFF);
+    may += __popc(bits >> 16);
+    inw[t >> 1] |= (bits & 0xFFFF) << (t & 1) * 16;
+    mayw[t >> 1] |= (bits >> 16) << (t & 1) * 16;
   }
-  for (int t = n + lane; t < a.topk; t += 64) out[t] = -1;
+  if (sure && live)
+    for (int t = take + g; t < a.topk; t += 4) row[t] = -1;
+  // the other queries, one after another: 64-bit scores of the blocks next to the cut, or of all where that says too little
+  unsigned long long todo = __ballot(!sure && live) & 0xFFFF;
+  const bool few = qn * big < 1e37f && may <= 16 && at <= take && at + may >= take;
+  while (todo) {
+    const int k = __ffsll(todo) - 1;
+    todo &= todo - 1;
+    const int qi = qt * 16 + k;
+    if (!__builtin_amdgcn_readlane((int)few, k)) {
+      exact_row<T>(a, bh, qi, lane, reinterpret_cast<double*>(key + a.nb), key);
+      __builtin_amdgcn_wave_barrier();
+      continue;
+    }
+    double qd[2] = {0, 0};
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (lane + 64 * x < a.dk)
+        for (int e = 0; e < a.group; ++e)
+          qd[x] += (double)(float)(static_cast<const T*>(a.q.p) + b * a.q.sb + qi * a.q.st + (long long)(h * a.group + e) * a.q.sh)[lane + 64 * x];
+    const int nmay = __builtin_amdgcn_readlane(may, k), need = __builtin_amdgcn_readlane(take - at, k);
+    double mine = 0;
+    int mj = 0, c = 0;
+#pragma unroll
+    for (int w = 0; w < (NT + 1) / 2; ++w) {
+      unsigned bits = (unsigned)__builtin_amdgcn_readlane((int)mayw[w], k);
+      while (bits) {  // (the same in every lane)
+        const int j = w * 32 + __ffs(bits) - 1;
+        bits &= bits - 1;
+        double x = 0;
+        const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          if (lane + 64 * y < a.dk) x += qd[y] * m[lane + 64 * y];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) x += shfl_xor_d(x, o);
+        if (lane == c) mine = x, mj = j;
+        ++c;
+      }
+    }
+    int before = 0;  // candidates in front of this lane's
+    for (int x = 0; x < nmay; ++x) {
+      const double v = __shfl(mine, x);
+      before += v > mine || (v == mine && x < lane);
+    }
+    const unsigned long long chosen = __ballot(lane < nmay && before < need);
+    int* const to = a.picked + ((long long)bh * a.nq + qi) * a.topk;
+    int base = 0;
+#pragma unroll
+    for (int w = 0; w < (NT + 1) / 2; ++w) {
+      unsigned bits = (unsigned)__builtin_amdgcn_readlane((int)inw[w], k);
+      for (unsigned long long left = chosen; left; left &= left - 1) {
+        const int j = __builtin_amdgcn_readlane(mj, __ffsll(left) - 1);
+        if (j >> 5 == w) bits |= 1u << (j & 31);
+      }
+      if (lane < 32 && (bits >> lane & 1)) to[base + __popc(bits & ((1u << lane) - 1))] = w * 32 + lane;
+      base += __popc(bits);
+    }
+    for (int t = base + lane; t < a.topk; t += 64) to[t] = -1;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ attention
@@ -536,11 +867,61 @@ static int by_type16(int dtype, F f) {
 
 using namespace yl;
 
+// ---- how the selection runs, and where things lie in the workspace
+constexpr int SCORE_MAX_NQ = 4;       // so few queries are scored by the wave that has the mean
+constexpr int SCORE_MAX_BLOCKS = 512; // scores of 16 queries in a wave's registers
+struct SelectPlan {
+  long long mean, score, split, norm, count, all;  // byte offsets
+};
+static SelectPlan plan_select(BlockArgs* a) {
+  SelectPlan p{};
+  a->nbp = (a->nb + 15) / 16 * 16, a->dkp = (a->dk + 31) / 32 * 32;
+  const long long bh = (long long)a->batch * a->kv;
+  const bool few = a->nq <= SCORE_MAX_NQ;
+  long long at = 0;
+  auto take = [&](long long n) {
+    const long long o = at;
+    at += round256(n);
+    return o;
+  };
+  p.mean = take(few ? 0 : 8 * bh * a->nb * a->dk);
+  p.score = take(few ? 8 * bh * a->nq * a->nb : 0);
+  p.split = take(few ? 0 : 4 * bh * a->nbp * a->dkp);
+  p.norm = take(few ? 0 : 4 * bh * a->nb);
+  p.count = take(4LL * a->batch * a->nb);
+  p.all = at;
+  return p;
+}
+
 extern "C" int64_t yl_block_select_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dk, int block) {
   BlockArgs a{};
   yl_heads dummy{reinterpret_cast<void*>(16), 0, 0, 0};
   if (fill_args("block_select", &dummy, &dummy, YL_BF16, batch, nq, nk, heads, kv_heads, dk, block, 1, nullptr, 0, &a)) return -1;
-  return round256(8LL * batch * kv_heads * dk * a.nb) + round256(4LL * batch * a.nb);
+  return batch * (long long)nq == 0 ? 0 : plan_select(&a).all;
+}
+
+template <typename T, bool SCORE>
+static int mean_launch(const BlockArgs& a, hipStream_t s) {
+  const long long wg = ((long long)a.batch * a.kv * a.nb + 3) / 4;
+  const int c = a.dk / 8;
+#define BA_MEAN(CP) hipLaunchKernelGGL((block_mean_kernel<T, CP, SCORE>), dim3((unsigned)wg), dim3(256), 0, s, a)
+  if (c <= 1) BA_MEAN(1);
+  else if (c <= 2) BA_MEAN(2);
+  else if (c <= 4) BA_MEAN(4);
+  else if (c <= 8) BA_MEAN(8);
+  else BA_MEAN(16);
+#undef BA_MEAN
+  YL_HIP(hipGetLastError());
+  return 0;
+}
+
+template <typename T, int NT>
+static int score_launch(const BlockArgs& a, hipStream_t s) {
+  const int qtiles = (a.nq + 15) / 16;
+  const long long wg = ((long long)a.batch * a.kv * qtiles + 3) / 4;
+  hipLaunchKernelGGL((block_score_kernel<T, NT>), dim3((unsigned)wg), dim3(256), (size_t)4 * (a.nb + a.dk) * 8, s, a, qtiles);
+  YL_HIP(hipGetLastError());
+  return 0;
 }
 
 extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, int batch, int nq, int nk, int heads, int kv_heads,
@@ -551,18 +932,29 @@ extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, 
   if (int rc = fill_args("block_select", q, k, dtype, batch, nq, nk, heads, kv_heads, dk, block, topk, mask, mask_stride, &a)) return rc;
   if (batch * (long long)nq == 0) return 0;
   if (!picked) return fail(-1, "block_select: null pointer");
-  const long long need = yl_block_select_workspace_bytes(batch, nq, nk, heads, kv_heads, dk, block);
-  if (need > 0 && (!work || work_bytes < need || (reinterpret_cast<uintptr_t>(work) & 15)))
+  const SelectPlan p = plan_select(&a);
+  if (p.all > 0 && (!work || work_bytes < p.all || (reinterpret_cast<uintptr_t>(work) & 15)))
     return fail(-1, "block_select: workspace missing, too small or not 16-byte aligned");
+  char* const w = static_cast<char*>(work);
   a.picked = picked;
-  a.mean = static_cast<double*>(work);
-  a.count = reinterpret_cast<int*>(static_cast<char*>(work) + round256(8LL * batch * kv_heads * dk * a.nb));
+  a.mean = reinterpret_cast<double*>(w + p.mean), a.score = reinterpret_cast<double*>(w + p.score);
+  a.split = reinterpret_cast<__bf16*>(w + p.split), a.norm = reinterpret_cast<float*>(w + p.norm);
+  a.count = reinterpret_cast<int*>(w + p.count);
   return by_type16(dtype, [&](auto* t) {
-    if (a.nb > 0) {
-      hipLaunchKernelGGL(block_mean_kernel<BA_T(t)>, dim3(batch * kv_heads * a.nb), dim3(256), 0, s, a);
-      YL_HIP(hipGetLastError());
+    typedef BA_T(t) T;
+    const bool few = nq <= SCORE_MAX_NQ;
+    if (a.nb > 0)
+      if (int rc = few ? mean_launch<T, true>(a, s) : mean_launch<T, false>(a, s)) return rc;
+    if (!few && a.nb > 0 && a.nb <= SCORE_MAX_BLOCKS) {
+      if (a.nb <= 64) return score_launch<T, 4>(a, s);
+      if (a.nb <= 128) return score_launch<T, 8>(a, s);
+      return a.nb <= 256 ? score_launch<T, 16>(a, s) : score_launch<T, 32>(a, s);
     }
-    hipLaunchKernelGGL(block_select_kernel<BA_T(t)>, dim3(batch * kv_heads * nq), dim3(64), (size_t)(a.dk + a.nb) * 8, s, a);
+    const size_t lds = (size_t)(a.nb + a.dk) * 8;
+    if (few)
+      hipLaunchKernelGGL((block_select_kernel<T, true>), dim3(batch * kv_heads * nq), dim3(64), lds, s, a);
+    else
+      hipLaunchKernelGGL((block_select_kernel<T, false>), dim3(batch * kv_heads * nq), dim3(64), lds, s, a);
     YL_HIP(hipGetLastError());
     return 0;
   });
