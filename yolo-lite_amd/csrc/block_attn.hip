@@ -21,6 +21,32 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int BA_MAX_BLOCKS = 4096;  // key blocks per image: the exact selection keeps a row of 64-bit keys in LDS (32 KB)
 constexpr int BA_MAX_TOPK = 64;
 
+// Over the four lanes that share lane & 15 (an MFMA column): v_permlane32_swap / v_permlane16_swap of a register with itself leave
+// the two halves' (row pairs') values side by side -- no LDS round trip.
+template <typename F>
+__device__ __forceinline__ unsigned quad_bits(unsigned x, F f) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  u2 p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = f(p[0], p[1]);
+  p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return f(p[0], p[1]);
+}
+__device__ __forceinline__ float quad_max(float x) {
+  return __uint_as_float(quad_bits(__float_as_uint(x), [](unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+__device__ __forceinline__ float quad_min(float x) {
+  return __uint_as_float(quad_bits(__float_as_uint(x), [](unsigned a, unsigned b) { return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  return __uint_as_float(quad_bits(__float_as_uint(x), [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+__device__ __forceinline__ int quad_sum(int x) {
+  return (int)quad_bits((unsigned)x, [](unsigned a, unsigned b) { return a + b; });
+}
+__device__ __forceinline__ unsigned quad_or(unsigned x) {
+  return quad_bits(x, [](unsigned a, unsigned b) { return a | b; });
+}
+
 // element (b, t, h, c) of a tensor of heads: p + b * sb + t * st + h * sh + c
 struct Heads {
   const void* p;
@@ -271,8 +297,9 @@ __global__ __launch_bounds__(64) void block_select_kernel(BlockArgs a) {
 // bisection, 16 queries in step.  Where the last block over the cut and the first under it are more than 2 err apart -- all but a
 // few in a thousand -- the order is the exact one's; the other queries (ties, NaN and infinities among them) are scored in 64 bits.
 template <typename T, int NT>
-__global__ __launch_bounds__(256) void block_score_kernel(BlockArgs a, int qtiles) {
+__global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(BlockArgs a, int qtiles) {
   extern __shared__ __attribute__((aligned(16))) unsigned char sel_sm[];
+  constexpr int NWORD = (NT + 1) / 2;  // 32 blocks to a word
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   unsigned long long* key = reinterpret_cast<unsigned long long*>(sel_sm) + (size_t)wave * (a.nb + a.dk);
   const long long unit = (long long)xcd_remap((int)blockIdx.x, (int)gridDim.x) * 4 + wave;
@@ -281,32 +308,21 @@ __global__ __launch_bounds__(256) void block_score_kernel(BlockArgs a, int qtile
   const int i = qt * 16 + n;
   const bool live = i < a.nq;
   const float ninf = -__builtin_huge_valf();
-  // which of this lane's blocks can be selected, how many there are, the largest |c|
-  int can = 0;
-  float big = 0.f;
-  for (int j = lane; j < a.nb; j += 64) {
-    can += a.count[b * a.nb + j] > 0;
-    big = fmaxf(big, a.norm[(long long)bh * a.nb + j]);
-    if (!(a.norm[(long long)bh * a.nb + j] < __builtin_huge_valf())) big = __builtin_huge_valf();
-  }
-  can = wave_sum(can);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
-  const int take = min(a.topk, can);
+  typedef T t8 __attribute__((ext_vector_type(8)));
 
+  // ---- scores
   f32x4 s[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float qq = 0.f;
   const __bf16* sp = a.split + (long long)bh * a.nbp * (2 * a.dkp);
-  typedef T t8 __attribute__((ext_vector_type(8)));
+  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.sb + (live ? i : 0) * a.q.st + (long long)(h * a.group) * a.q.sh;
   for (int c0 = 0; c0 < a.dkp; c0 += 32) {
     const int c = c0 + g * 8;
     float q[8] = {};
     if (c < a.dk) {
       for (int e = 0; e < a.group; ++e) {
-        const t8 x = *reinterpret_cast<const t8*>(static_cast<const T*>(a.q.p) + b * a.q.sb + (live ? i : 0) * a.q.st +
-                                                  (long long)(h * a.group + e) * a.q.sh + c);
+        const t8 x = *reinterpret_cast<const t8*>(qp + e * a.q.sh + c);
 #pragma unroll
         for (int d = 0; d < 8; ++d) q[d] += (float)x[d];
       }
@@ -319,60 +335,87 @@ __global__ __launch_bounds__(256) void block_score_kernel(BlockArgs a, int qtile
       qh[d] = hi, ql[d] = lo;
       qq += q[d] * q[d];
     }
+    constexpr int TB = NT < 4 ? NT : 4;  // tiles whose loads are in flight together
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t * 16 >= a.nb) break;
-      const __bf16* m = sp + (long long)(t * 16 + n) * (2 * a.dkp) + c;
-      const bf16x8 mh = *reinterpret_cast<const bf16x8*>(m), ml = *reinterpret_cast<const bf16x8*>(m + a.dkp);
-      s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh, qh, s[t], 0, 0, 0);
-      s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml, qh, s[t], 0, 0, 0);
-      s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh, ql, s[t], 0, 0, 0);
+    for (int t0 = 0; t0 < NT; t0 += TB) {
+      if (t0 * 16 >= a.nb) break;
+      bf16x8 mh[TB], ml[TB];
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        const __bf16* m = sp + (long long)min((t0 + t) * 16 + n, a.nbp - 1) * (2 * a.dkp) + c;
+        mh[t] = *reinterpret_cast<const bf16x8*>(m);
+        ml[t] = *reinterpret_cast<const bf16x8*>(m + a.dkp);
+      }
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        s[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], qh, s[t0 + t], 0, 0, 0);
+        s[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml[t], qh, s[t0 + t], 0, 0, 0);
+        s[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], ql, s[t0 + t], 0, 0, 0);
+      }
     }
   }
-  qq += __shfl_xor(qq, 16);
-  qq += __shfl_xor(qq, 32);
-  const float qn = sqrtf(qq);
+  // ---- which blocks can be selected, how many there are, the largest |c|
+  unsigned okw[NWORD];
+  int can = 0;
+  float big = 0.f;
+#pragma unroll
+  for (int w = 0; w < NWORD; w += 2) {
+    const int j = w * 16 * 2 + lane;
+    const bool in = j < a.nb;
+    const float x = in ? a.norm[(long long)bh * a.nb + j] : 0.f;
+    const unsigned long long ok = __ballot(in && a.count[b * a.nb + (in ? j : 0)] > 0);
+    okw[w] = (unsigned)ok;
+    if (w + 1 < NWORD) okw[w + 1] = (unsigned)(ok >> 32);
+    can += __popcll(ok);
+    big = fmaxf(big, x < __builtin_huge_valf() ? x : __builtin_huge_valf());  // (NaN: no bound)
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
+  big = quad_max(big);
+  const int take = min(a.topk, can);
+  const float qn = sqrtf(quad_sum(qq));
   const float err = (3.f / 262144.f + 4.f * a.dk / 16777216.f) * qn * big + (qn + big) * 2e-36f + 1e-30f;
 
-  // blocks that cannot be selected (and places behind the last) go under every cut
-  unsigned okw[(NT + 7) / 8] = {};  // four bits per tile
+  // ---- the cut.  Blocks that cannot be selected (and places behind the last) go under every cut
   float lo = __builtin_huge_valf(), hi = ninf;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t) {
+    const unsigned m = okw[t >> 1] >> ((t & 1) * 16 + 4 * g);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int j = t * 16 + 4 * g + r;
-      const bool ok = j < a.nb && a.count[b * a.nb + (j < a.nb ? j : 0)] > 0;
-      okw[t >> 3] |= (unsigned)ok << ((t & 7) * 4 + r);
+      const bool ok = m >> r & 1;
       lo = ok ? fminf(lo, s[t][r]) : lo;
-      hi = ok ? fmaxf(hi, s[t][r]) : hi;
       s[t][r] = ok ? s[t][r] : ninf;
+      hi = fmaxf(hi, s[t][r]);
     }
-  lo = fminf(lo, __shfl_xor(lo, 16));
-  lo = fminf(lo, __shfl_xor(lo, 32));
-  hi = fmaxf(hi, __shfl_xor(hi, 16));
-  hi = fmaxf(hi, __shfl_xor(hi, 32));
-  // cut: more than `take` scores over lo, fewer over hi
+  }
+  lo = quad_min(lo);
+  hi = quad_max(hi);
+  // more than `take` scores over lo, fewer over hi; the next one where a straight line between the two counts meets `take` (scores lie
+  // dense around the cut), every third time half way
   float cut = ninf;
   bool found = take == can;  // (everything that can be selected is: the cut stays at -inf)
   lo -= (hi - lo) * 0.01f + 1e-30f;
-  for (int it = 0; it < 32 && __ballot(!found && live); ++it) {
-    const float mid = 0.5f * (lo + hi);
+  float over_lo = (float)can, over_hi = 0.f;
+  for (int it = 0; it < 40 && __ballot(!found && live); ++it) {
+    const float f = it % 3 == 2 ? 0.5f : fminf(0.98f, fmaxf(0.02f, (over_lo - (float)take) / (over_lo - over_hi)));
+    const float mid = lo + f * (hi - lo);
     int c = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) c += s[t][r] > mid;
-    c += __shfl_xor(c, 16);
-    c += __shfl_xor(c, 32);
+    c = quad_sum(c);
     if (!found) {
       if (c == take) {
         found = true;
         cut = mid;
       } else if (c > take) {
         lo = mid;
+        over_lo = (float)c;
       } else {
         hi = mid;
+        over_hi = (float)c;
       }
     }
   }
@@ -382,47 +425,58 @@ __global__ __launch_bounds__(256) void block_score_kernel(BlockArgs a, int qtile
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      in = s[t][r] > cut ? fminf(in, s[t][r]) : in;
-      out = s[t][r] > cut ? out : fmaxf(out, s[t][r]);
+      const bool over = s[t][r] > cut;
+      in = over ? fminf(in, s[t][r]) : in;
+      out = over ? out : fmaxf(out, s[t][r]);
     }
-  in = fminf(in, __shfl_xor(in, 16));
-  in = fminf(in, __shfl_xor(in, 32));
-  out = fmaxf(out, __shfl_xor(out, 16));
-  out = fmaxf(out, __shfl_xor(out, 32));
+  in = quad_min(in);
+  out = quad_max(out);
   const bool sure = take == can || (found && qn * big < 1e37f && in - out > 2.f * err);  // (not so where anything is NaN)
-  // ascending block indices: bits of a tile of 16 blocks, all of them in every lane of a query
-  const float up = (found ? out : hi) + 2.f * err, dn = (found ? in : lo) - 2.f * err;
+  const float up = (found ? out : hi) + 2.f * err, dn = (found ? in : lo) - 2.f * err;   // the band around a cut that is not sure
+  const float floor_ = sure ? cut : up;
+
+  // ---- picked blocks as words of 32, the same in every lane of a query; each lane writes its own, by rank
   int* const row = a.picked + ((long long)bh * a.nq + i) * a.topk;
-  unsigned inw[(NT + 1) / 2] = {}, mayw[(NT + 1) / 2] = {};  // 32 blocks to a word: picked; where the order is not sure, over it / next to it
-  int at = 0, may = 0;
+  const unsigned own = 0x000F000Fu << (4 * g);
+  unsigned inw[NWORD];
+  int at = 0;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    if (t * 16 >= a.nb) break;
-    unsigned bits = 0;  // low half: picked (or over the band), high half: in the band
+  for (int w = 0; w < NWORD; ++w) {
+    unsigned bits = 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool ok = okw[t >> 3] >> ((t & 7) * 4 + r) & 1;
-      const bool pick = take == can ? ok : sure ? s[t][r] > cut : s[t][r] > up;
-      bits |= (unsigned)pick << (4 * g + r);
-      bits |= (unsigned)(!sure && ok && s[t][r] <= up && s[t][r] >= dn) << (16 + 4 * g + r);
+    for (int t = 2 * w; t < 2 * w + 2 && t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bits |= (unsigned)(s[t][r] > floor_) << ((t & 1) * 16 + r);
+    bits = quad_or(bits << (4 * g));
+    if (take == can) bits = okw[w];
+    inw[w] = bits;
+    unsigned left = sure && live ? bits & own : 0;
+    while (__ballot(left)) {
+      if (left) {
+        const int x = __ffs(left) - 1;
+        left &= left - 1;
+        row[at + __popc(bits & ((1u << x) - 1))] = w * 32 + x;
+      }
     }
-    const unsigned own = bits;
-    bits |= __shfl_xor(bits, 16);
-    bits |= __shfl_xor(bits, 32);
-    if (sure && live) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (own >> (4 * g + r) & 1) row[at + __popc(bits & ((1u << (4 * g + r)) - 1))] = t * 16 + 4 * g + r;
-    }
-    at += __popc(bits & 0xFFFF);
-    may += __popc(bits >> 16);
-    inw[t >> 1] |= (bits & 0xFFFF) << (t & 1) * 16;
-    mayw[t >> 1] |= (bits >> 16) << (t & 1) * 16;
+    at += __popc(bits);
   }
   if (sure && live)
     for (int t = take + g; t < a.topk; t += 4) row[t] = -1;
   // the other queries, one after another: 64-bit scores of the blocks next to the cut, or of all where that says too little
   unsigned long long todo = __ballot(!sure && live) & 0xFFFF;
+  if (!todo) return;
+  unsigned mayw[NWORD];
+  int may = 0;
+#pragma unroll
+  for (int w = 0; w < NWORD; ++w) {
+    unsigned bits = 0;
+#pragma unroll
+    for (int t = 2 * w; t < 2 * w + 2 && t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bits |= (unsigned)(s[t][r] <= up && s[t][r] >= dn) << ((t & 1) * 16 + r);
+    mayw[w] = quad_or(bits << (4 * g)) & okw[w];
+    may += __popc(mayw[w]);
+  }
   const bool few = qn * big < 1e37f && may <= 16 && at <= take && at + may >= take;
   while (todo) {
     const int k = __ffsll(todo) - 1;
@@ -443,7 +497,7 @@ __global__ __launch_bounds__(256) void block_score_kernel(BlockArgs a, int qtile
     double mine = 0;
     int mj = 0, c = 0;
 #pragma unroll
-    for (int w = 0; w < (NT + 1) / 2; ++w) {
+    for (int w = 0; w < NWORD; ++w) {
       unsigned bits = (unsigned)__builtin_amdgcn_readlane((int)mayw[w], k);
       while (bits) {  // (the same in every lane)
         const int j = w * 32 + __ffs(bits) - 1;
@@ -468,7 +522,7 @@ __global__ __launch_bounds__(256) void block_score_kernel(BlockArgs a, int qtile
     int* const to = a.picked + ((long long)bh * a.nq + qi) * a.topk;
     int base = 0;
 #pragma unroll
-    for (int w = 0; w < (NT + 1) / 2; ++w) {
+    for (int w = 0; w < NWORD; ++w) {
       unsigned bits = (unsigned)__builtin_amdgcn_readlane((int)inw[w], k);
       for (unsigned long long left = chosen; left; left &= left - 1) {
         const int j = __builtin_amdgcn_readlane(mj, __ffsll(left) - 1);
@@ -509,16 +563,6 @@ struct Vec<_Float16> {
   typedef _Float16 t4 __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ f32x4 mfma(t8 a, t8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
-
-// the four lanes that share lane & 15: maximum, sum
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
 
 struct AttendArgs {
   BlockArgs a;
