@@ -18,7 +18,7 @@ namespace yl {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int BA_MAX_BLOCKS = 4096;  // key blocks per image: the exact selection keeps a row of 64-bit keys in LDS (32 KB)
+constexpr int BA_MAX_BLOCKS = 4096;  // key blocks per image: the exact selection keeps a row of 64-bit keys in a wave's registers
 constexpr int BA_MAX_TOPK = 64;
 
 // Over the four lanes that share lane & 15 (an MFMA column): v_permlane32_swap / v_permlane16_swap of a register with itself leave
@@ -65,6 +65,7 @@ struct BlockArgs {
   __bf16* split;  // [batch][kv][nbp][2][dkp]: the means as two bf16; nbp = nb rounded up to 16, dkp = dk to 32
   float* norm;    // [batch][kv][nb]: 2-norm of a mean
   int nbp, dkp;
+  unsigned magic; // 2^32 / group, rounded up: f / group = mulhi(f, magic) for f * group < 2^32
   int* count;     // [batch][nb]: unmasked keys of a block
   int* picked;    // [batch][kv][nq][topk]
 };
@@ -198,61 +199,75 @@ __device__ __forceinline__ int wave_sum(int c) {
   return __builtin_amdgcn_readlane(c, 63);
 }
 
-// One wave: key[nb] in LDS -> the n-th largest by its bits, then the blocks at or over it in ascending order.
-__device__ __forceinline__ void pick_row(const unsigned long long* key, int nb, int topk, int lane, int* out) {
+__device__ __forceinline__ unsigned wave_or(unsigned c) {
+  c |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)c, 0x111, 0xF, 0xF, false);
+  c |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)c, 0x112, 0xF, 0xF, false);
+  c |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)c, 0x114, 0xF, 0xF, false);
+  c |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)c, 0x118, 0xF, 0xF, false);
+  c |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)c, 0x142, 0xA, 0xF, false);
+  c |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)c, 0x143, 0xC, 0xF, false);
+  return (unsigned)__builtin_amdgcn_readlane((int)c, 63);
+}
+
+// One wave: lane holds the keys of blocks 64 i + lane (0 behind the last) -> the n-th largest by its bits, upper word first (the lower
+// words are looked at where the upper ones leave it open: ties), then the blocks at or over it in ascending order.
+template <int NI>
+__device__ __forceinline__ void pick_row(const unsigned long long (&key)[NI], int topk, int lane, int* out) {
   int can = 0;
-  unsigned long long any = 0, all = ~0ull;
-  for (int j = lane; j < nb; j += 64) {
-    const unsigned long long k = key[j];
-    can += k != 0;
-    any |= k;
-    all &= k;
-  }
+  unsigned any = 0, none = 0;  // bits set in some key, clear in some key
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    any |= __shfl_xor(any, o);
-    all &= __shfl_xor(all, o);
+  for (int i = 0; i < NI; ++i) {
+    can += key[i] != 0;
+    any |= (unsigned)(key[i] >> 32);
+    none |= ~(unsigned)(key[i] >> 32);
   }
   const int n = min(topk, wave_sum(can));
-  // bits that all keys share need no decision
-  const unsigned long long differ = any & ~all;
-  const int top = differ ? 63 - __clzll(differ) : -1;
-  unsigned long long v = top == 63 ? 0 : all & ~((2ull << (top < 0 ? 0 : top)) - 1);
-  if (top < 0) v = all;
-  int over = 0;  // keys > v
   if (n > 0) {
+    any = wave_or(any);
+    const unsigned differ = any & wave_or(none);  // bits that all keys share need no decision
+    unsigned vh = any & ~differ, vl = 0;
     bool exact = false;
-    for (int bit = top; bit >= 0 && !exact; --bit) {
-      const unsigned long long t = v | 1ull << bit;
+    for (unsigned left = differ; left && !exact;) {
+      const unsigned bit = 1u << (31 - __clz(left));
+      left &= ~bit;
       int c = 0;
-#pragma unroll 4
-      for (int j = lane; j < nb; j += 64) c += key[j] >= t;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) c += (unsigned)(key[i] >> 32) >= (vh | bit);
       c = wave_sum(c);
-      if (c >= n) v = t;
+      if (c >= n) vh |= bit;
       exact = c == n;
     }
-    int c = 0;
-    for (int j = lane; j < nb; j += 64) c += key[j] > v;
-    over = wave_sum(c);
-  }
-  int at = 0, ties = n - over;  // of the keys equal to v the first `ties` belong to the set
-  for (int j0 = 0; j0 < nb && n > 0; j0 += 64) {
-    const int j = j0 + lane;
-    const unsigned long long k = j < nb ? key[j] : 0;
+    for (int bit = 31; bit >= 0 && !exact; --bit) {
+      const unsigned long long t = (unsigned long long)vh << 32 | vl | 1u << bit;
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) c += key[i] >= t;
+      c = wave_sum(c);
+      if (c >= n) vl |= 1u << bit;
+      exact = c == n;
+    }
+    const unsigned long long v = (unsigned long long)vh << 32 | vl;
+    int over = 0;  // keys > v
+#pragma unroll
+    for (int i = 0; i < NI; ++i) over += key[i] > v;
+    int at = 0, ties = n - wave_sum(over);  // of the keys equal to v the first `ties` belong to the set
     const unsigned long long below = (1ull << lane) - 1;
-    const unsigned long long eq = __ballot(j < nb && k == v);
-    const bool take = (j < nb && k > v) || (j < nb && k == v && __popcll(eq & below) < ties);
-    ties -= min(ties, (int)__popcll(eq));
-    const unsigned long long got = __ballot(take);
-    if (take) out[at + __popcll(got & below)] = j;
-    at += __popcll(got);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const unsigned long long eq = __ballot(key[i] == v);
+      const bool take = key[i] > v || (key[i] == v && __popcll(eq & below) < ties);
+      ties -= min(ties, (int)__popcll(eq));
+      const unsigned long long got = __ballot(take);
+      if (take) out[at + __popcll(got & below)] = i * 64 + lane;
+      at += __popcll(got);
+    }
   }
   for (int t = n + lane; t < topk; t += 64) out[t] = -1;
 }
 
-// One wave: the exact scores of one (image, kv head, query) from the 64-bit means, then pick_row.  qs: dk doubles, key: nb words of LDS.
-template <typename T>
-__device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int lane, double* qs, unsigned long long* key) {
+// One wave: the exact scores of one (image, kv head, query) from the 64-bit means, then pick_row.  qs: dk doubles of LDS.
+template <typename T, int NI>
+__device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int lane, double* qs) {
   const int h = bh % a.kv, b = bh / a.kv;
   for (int d = lane; d < a.dk; d += 64) {
     double s = 0;
@@ -261,31 +276,44 @@ __device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int
     qs[d] = s;
   }
   __builtin_amdgcn_wave_barrier();
-  for (int j = lane; j < a.nb; j += 64) {
-    double s = 0;
-    const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
-    for (int d = 0; d < a.dk; ++d) s += qs[d] * m[d];
-    key[j] = order_key(s, a.count[b * a.nb + j] > 0);
+  unsigned long long key[NI];
+#pragma unroll
+  for (int x = 0; x < NI; ++x) {
+    const int j = x * 64 + lane;
+    key[x] = 0;
+    if (j < a.nb) {
+      double s = 0;
+      const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
+#pragma unroll 8
+      for (int d = 0; d < a.dk; ++d) s += qs[d] * m[d];
+      key[x] = order_key(s, a.count[b * a.nb + j] > 0);
+    }
   }
-  __builtin_amdgcn_wave_barrier();
-  pick_row(key, a.nb, a.topk, lane, a.picked + ((long long)bh * a.nq + i) * a.topk);
+  pick_row<NI>(key, a.topk, lane, a.picked + ((long long)bh * a.nq + i) * a.topk);
 }
 
-// SCORED: the scores are there (few queries); else from the means.  One wave per (image, kv head, query).
-template <typename T, bool SCORED>
+// SCORED: the scores are there (few queries); else from the means.  One wave per (image, kv head, query); up to 64 NI blocks.
+template <typename T, int NI, bool SCORED>
 __global__ __launch_bounds__(64) void block_select_kernel(BlockArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char sel_sm[];
-  unsigned long long* key = reinterpret_cast<unsigned long long*>(sel_sm);  // [nb]
+  __shared__ double qs[SCORED ? 1 : 128];
   const int lane = threadIdx.x;
   const long long row = blockIdx.x;  // (b * kv + h) * nq + i
   const int i = (int)(row % a.nq), bh = (int)(row / a.nq);
   if constexpr (SCORED) {
-#pragma unroll 4
-    for (int j = lane; j < a.nb; j += 64) key[j] = order_key(a.score[row * a.nb + j], a.count[bh / a.kv * a.nb + j] > 0);
-    __syncthreads();
-    pick_row(key, a.nb, a.topk, lane, a.picked + row * a.topk);
+    unsigned long long key[NI];
+    double s[NI];
+    int n[NI];
+#pragma unroll
+    for (int x = 0; x < NI; ++x) {  // (all in flight together)
+      const int j = min(x * 64 + lane, a.nb - 1);
+      s[x] = a.nb ? a.score[row * a.nb + j] : 0.0;
+      n[x] = a.nb && x * 64 + lane < a.nb ? a.count[bh / a.kv * a.nb + j] : 0;
+    }
+#pragma unroll
+    for (int x = 0; x < NI; ++x) key[x] = order_key(s[x], n[x] > 0);
+    pick_row<NI>(key, a.topk, lane, a.picked + row * a.topk);
   } else {
-    exact_row<T>(a, bh, i, lane, reinterpret_cast<double*>(key + a.nb), key);
+    exact_row<T, NI>(a, bh, i, lane, qs);
   }
 }
 
@@ -298,10 +326,9 @@ __global__ __launch_bounds__(64) void block_select_kernel(BlockArgs a) {
 // few in a thousand -- the order is the exact one's; the other queries (ties, NaN and infinities among them) are scored in 64 bits.
 template <typename T, int NT>
 __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(BlockArgs a, int qtiles) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char sel_sm[];
+  __shared__ double qs[4][128];
   constexpr int NWORD = (NT + 1) / 2;  // 32 blocks to a word
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
-  unsigned long long* key = reinterpret_cast<unsigned long long*>(sel_sm) + (size_t)wave * (a.nb + a.dk);
   const long long unit = (long long)xcd_remap((int)blockIdx.x, (int)gridDim.x) * 4 + wave;
   if (unit >= (long long)a.batch * a.kv * qtiles) return;  // (no barrier below: waves are on their own)
   const int qt = (int)(unit % qtiles), bh = (int)(unit / qtiles), h = bh % a.kv, b = bh / a.kv;
@@ -342,9 +369,9 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
       bf16x8 mh[TB], ml[TB];
 #pragma unroll
       for (int t = 0; t < TB; ++t) {
-        const __bf16* m = sp + (long long)min((t0 + t) * 16 + n, a.nbp - 1) * (2 * a.dkp) + c;
-        mh[t] = *reinterpret_cast<const bf16x8*>(m);
-        ml[t] = *reinterpret_cast<const bf16x8*>(m + a.dkp);
+        const unsigned m = (unsigned)min((t0 + t) * 16 + n, a.nbp - 1) * (unsigned)(2 * a.dkp) + (unsigned)c;  // (at most 2^18)
+        mh[t] = *reinterpret_cast<const bf16x8*>(sp + m);
+        ml[t] = *reinterpret_cast<const bf16x8*>(sp + m + (unsigned)a.dkp);
       }
 #pragma unroll
       for (int t = 0; t < TB; ++t) {
@@ -391,33 +418,22 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   }
   lo = quad_min(lo);
   hi = quad_max(hi);
-  // more than `take` scores over lo, fewer over hi; the next one where a straight line between the two counts meets `take` (scores lie
-  // dense around the cut), every third time half way
+  // more than `take` scores over lo, fewer over hi.  (Half way: about 11 steps until all 16 queries are done; a straight line between
+  // the two counts took 14-16, the counts fall too steeply towards the cut.)
   float cut = ninf;
   bool found = take == can;  // (everything that can be selected is: the cut stays at -inf)
   lo -= (hi - lo) * 0.01f + 1e-30f;
-  float over_lo = (float)can, over_hi = 0.f;
-  for (int it = 0; it < 40 && __ballot(!found && live); ++it) {
-    const float f = it % 3 == 2 ? 0.5f : fminf(0.98f, fmaxf(0.02f, (over_lo - (float)take) / (over_lo - over_hi)));
-    const float mid = lo + f * (hi - lo);
+  for (int it = 0; it < 32 && __ballot(!found && live); ++it) {
+    const float mid = 0.5f * (lo + hi);
     int c = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) c += s[t][r] > mid;
     c = quad_sum(c);
-    if (!found) {
-      if (c == take) {
-        found = true;
-        cut = mid;
-      } else if (c > take) {
-        lo = mid;
-        over_lo = (float)c;
-      } else {
-        hi = mid;
-        over_hi = (float)c;
-      }
-    }
+    if (c == take) cut = found ? cut : mid, found = true;
+    lo = c > take && !found ? mid : lo;
+    hi = c < take && !found ? mid : hi;
   }
   // how far apart the two sides of the cut are
   float in = __builtin_huge_valf(), out = ninf;
@@ -483,7 +499,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
     todo &= todo - 1;
     const int qi = qt * 16 + k;
     if (!__builtin_amdgcn_readlane((int)few, k)) {
-      exact_row<T>(a, bh, qi, lane, reinterpret_cast<double*>(key + a.nb), key);
+      exact_row<T, (NT + 3) / 4>(a, bh, qi, lane, qs[wave]);
       __builtin_amdgcn_wave_barrier();
       continue;
     }
@@ -634,7 +650,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   constexpr int NT = DIRECT ? 64 : 256;
   constexpr int KT = KEYS / 16, KS = KEYS / 32, DVP = DV16 * 16, VP = KEYS + 8;
   __shared__ __attribute__((aligned(16))) T sVt[DVP * VP];
-  __shared__ unsigned rows[DIRECT ? 1 : 4096];
+  extern __shared__ unsigned rows[];  // [64 * range]: group in the range << 12 | query << 6 | slot
   __shared__ int total;
   const BlockArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -736,16 +752,22 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       const t4 lo = *reinterpret_cast<const t4*>(vr), hi = *reinterpret_cast<const t4*>(vr + 16);
       vf[d][s] = t8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     }
-  const float scale = a.scale * 1.44269504088896340736f;
+  // scores are scaled by |scale| inside the exponential's fma; a negative scale flips the queries' signs
+  const float scale = fabsf(a.scale) * 1.44269504088896340736f;
+  const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
+  const bool all = ok == (KEYS == 64 ? ~0ull : (1ull << KEYS) - 1);  // no key is masked: uniform
   const bool alone = DIRECT && p.slots == 1;  // a row has this one result: it is the output
+  t8 one;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
 
   // a tile's queries: lane column n is (query, head) row f
   struct Row {
-    long long q;  // query of the image
-    int head, slot;
+    int q, head, slot;  // query of the image
     bool live;
     t8 f[DK32];
   };
+  const T* const qb = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)(h * a.group) * a.q.sh;
   auto fetch = [&](int tile, Row& w) __attribute__((always_inline)) {
     const int f = tile * 16 + n;
     w.live = f < nrows;
@@ -753,7 +775,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     int e = fc;
     w.head = 0;
     if (a.group > 1) {
-      e = fc / a.group;
+      e = (int)__umulhi((unsigned)fc, a.magic);
       w.head = fc - e * a.group;
     }
     if constexpr (DIRECT) {
@@ -761,14 +783,17 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       w.slot = tdirect;
     } else {
       const unsigned x = rows[e];
-      w.q = (long long)(grp0 + (int)(x >> 12)) * 64 + (x >> 6 & 63);
+      w.q = (grp0 + (int)(x >> 12)) * 64 + (int)(x >> 6 & 63);
       w.slot = (int)(x & 63);
     }
-    const T* qp = static_cast<const T*>(a.q.p) + b * a.q.sb + w.q * a.q.st + (long long)(h * a.group + w.head) * a.q.sh;
+    const T* qp = qb + w.q * a.q.st + w.head * a.q.sh;
 #pragma unroll
     for (int c = 0; c < DK32; ++c) {
-      w.f[c] = t8{};
-      if ((c * 4 + g) * 8 < a.dk) w.f[c] = *reinterpret_cast<const t8*>(qp + (c * 4 + g) * 8);
+      u32x4 x = {0, 0, 0, 0};
+      if ((c * 4 + g) * 8 < a.dk) x = *reinterpret_cast<const u32x4*>(qp + (c * 4 + g) * 8);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) x[d] ^= flip;
+      w.f[c] = __builtin_bit_cast(t8, x);
     }
   };
   const int ntiles = (nrows + 15) >> 4;
@@ -786,27 +811,37 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       for (int c = 0; c < DK32; ++c) s[t] = Vec<T>::mfma(kf[t][c], w.f[c], s[t]);
     }
     float m = ninf;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[t][r] = okt >> (4 * t + r) & 1 ? s[t][r] * scale : ninf;
-        m = fmaxf(m, s[t][r]);
-      }
-    m = quad_max(m);
-    const float base = m == ninf ? 0.f : m;  // (no key, or every score -inf: all weights 0)
-    float l = 0.f;
     t8 pf[KS];
+    if (all) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(s[t][r] - base);
-        l += e;
-        pf[t >> 1][(t & 1) * 4 + r] = (T)e;
-      }
-    l = quad_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, s[t][r]);
+      m = quad_max(m) * scale;
+      const float base = m == ninf ? 0.f : m;  // (every score -inf: all weights 0)
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pf[t >> 1][(t & 1) * 4 + r] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -base));
+    } else {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = okt >> (4 * t + r) & 1 ? fmaxf(m, s[t][r]) : m;
+      m = quad_max(m);
+      m = m == ninf ? m : m * scale;  // (no key: -inf, also where the scale is 0)
+      const float base = m == ninf ? 0.f : m;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          pf[t >> 1][(t & 1) * 4 + r] = okt >> (4 * t + r) & 1 ? (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -base)) : (T)0.f;
+    }
+    // the weights' sum by the matrix pipe too: a row of ones; every lane of a query gets it, and it is the sum of what multiplies v
+    f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < KS; ++x) lsum = Vec<T>::mfma(one, pf[x], lsum);
+    const float l = lsum[0];
     f32x4 o[DV16];
 #pragma unroll
     for (int d = 0; d < DV16; ++d) {
@@ -814,11 +849,12 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
 #pragma unroll
       for (int x = 0; x < KS; ++x) o[d] = Vec<T>::mfma(vf[d][x], pf[x], o[d]);
     }
+    const float inv = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);
     if (!w.live) continue;
-    const long long row = (((long long)bh) * a.nq + w.q) * a.group + w.head;
-    const int slot = w.slot * p.subs + sub;
+    const unsigned row = ((unsigned)bh * (unsigned)a.nq + (unsigned)w.q) * (unsigned)a.group + (unsigned)w.head;  // (below 2^31)
+    const long long at = (long long)row * p.slots + w.slot * p.subs + sub;
     T* dst = alone ? static_cast<T*>(const_cast<void*>(a.o.p)) + b * a.o.sb + w.q * a.o.st + (long long)(h * a.group + w.head) * a.o.sh
-                   : static_cast<T*>(p.part) + (row * p.slots + slot) * DVP;
+                   : static_cast<T*>(p.part) + at * DVP;
 #pragma unroll
     for (int d = 0; d < DV16; d += 2) {
       const int c = g * (DVP / 4) + d * 4;
@@ -826,7 +862,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
                     (T)(o[d + 1][0] * inv), (T)(o[d + 1][1] * inv), (T)(o[d + 1][2] * inv), (T)(o[d + 1][3] * inv)};
       if (!alone || c < a.dv) *reinterpret_cast<t8*>(dst + c) = y;
     }
-    if (!alone && g == 0) p.ml[row * p.slots + slot] = float2{m, l};
+    if (!alone && g == 0) p.ml[at] = float2{m, l};
   }
 }
 
@@ -841,17 +877,35 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   const long long row = item / C;
   if (row >= (long long)a.batch * a.nq * a.heads || c >= a.dv) return;
   const float2* ml = p.ml + row * p.slots;
+  const T* part = static_cast<const T*>(p.part) + row * p.slots * DVP + c;
+  constexpr int U = 8;  // slots whose loads are in flight together
   float m = -__builtin_huge_valf();
-  for (int t = 0; t < p.slots; ++t) m = fmaxf(m, ml[t].x);
+  for (int t0 = 0; t0 < p.slots; t0 += U) {
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = ml[min(t0 + u, p.slots - 1)].x;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = fmaxf(m, x[u]);
+  }
   const float base = m == -__builtin_huge_valf() ? 0.f : m;
   float acc[8] = {}, sum = 0.f;
-  for (int t = 0; t < p.slots; ++t) {
-    const float w = ml[t].y * __builtin_amdgcn_exp2f(ml[t].x - base);
-    if (w == 0.f) continue;  // (nothing was stored for a slot without a block)
-    sum += w;
-    const t8 y = *reinterpret_cast<const t8*>(static_cast<const T*>(p.part) + (row * p.slots + t) * DVP + c);
+  for (int t0 = 0; t0 < p.slots; t0 += U) {
+    float w[U];
+    t8 y[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += w * (float)y[e];
+    for (int u = 0; u < U; ++u) {
+      const int t = min(t0 + u, p.slots - 1);
+      const float2 x = ml[t];
+      y[u] = *reinterpret_cast<const t8*>(part + t * DVP);  // (whatever lies there where the slot has no block: not used)
+      w[u] = t0 + u < p.slots ? x.y * __builtin_amdgcn_exp2f(x.x - base) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (w[u] == 0.f) continue;
+      sum += w[u];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += w[u] * (float)y[u][e];
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int gh = (int)(row % a.group);
@@ -881,6 +935,7 @@ static int fill_args(const std::string& who, const yl_heads* q, const yl_heads* 
   if (dtype != YL_BF16 && dtype != YL_F16) return fail(-1, who + ": bf16 or fp16 tensors");
   if (batch < 0 || nq < 0 || nk < 0) return fail(-1, who + ": a negative size");
   if (heads < 1 || kv_heads < 1 || heads % kv_heads) return fail(-1, who + ": the query heads must be a multiple of the kv heads");
+  if (heads / kv_heads > 1000) return fail(-3, who + ": more than 1000 query heads to a kv head");
   if (dk < 8 || dk > 128 || dk % 8) return fail(-3, who + ": key widths are multiples of 8 up to 128");
   if (block != 32 && block != 64 && block != 128) return fail(-3, who + ": blocks of 32, 64 or 128 keys");
   if (topk < 1 || topk > BA_MAX_TOPK) return fail(-3, who + ": 1 to 64 blocks for a query");
@@ -896,6 +951,7 @@ static int fill_args(const std::string& who, const yl_heads* q, const yl_heads* 
   a->q = Heads{q->data, q->batch, q->token, q->head};
   if (nk > 0) a->k = Heads{k->data, k->batch, k->token, k->head};
   a->batch = batch, a->nq = nq, a->nk = nk, a->heads = heads, a->kv = kv_heads, a->group = heads / kv_heads;
+  a->magic = (unsigned)((1ULL << 32) / a->group + 1);
   a->dk = dk, a->block = block, a->nb = (int)nb, a->topk = topk, a->mask = mask, a->mask_stride = mask_stride;
   return 0;
 }
@@ -963,7 +1019,7 @@ template <typename T, int NT>
 static int score_launch(const BlockArgs& a, hipStream_t s) {
   const int qtiles = (a.nq + 15) / 16;
   const long long wg = ((long long)a.batch * a.kv * qtiles + 3) / 4;
-  hipLaunchKernelGGL((block_score_kernel<T, NT>), dim3((unsigned)wg), dim3(256), (size_t)4 * (a.nb + a.dk) * 8, s, a, qtiles);
+  hipLaunchKernelGGL((block_score_kernel<T, NT>), dim3((unsigned)wg), dim3(256), 0, s, a, qtiles);
   YL_HIP(hipGetLastError());
   return 0;
 }
@@ -994,11 +1050,15 @@ extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, 
       if (a.nb <= 128) return score_launch<T, 8>(a, s);
       return a.nb <= 256 ? score_launch<T, 16>(a, s) : score_launch<T, 32>(a, s);
     }
-    const size_t lds = (size_t)(a.nb + a.dk) * 8;
-    if (few)
-      hipLaunchKernelGGL((block_select_kernel<T, true>), dim3(batch * kv_heads * nq), dim3(64), lds, s, a);
-    else
-      hipLaunchKernelGGL((block_select_kernel<T, false>), dim3(batch * kv_heads * nq), dim3(64), lds, s, a);
+#define BA_SELECT(NI)                                                                                                  \
+  do {                                                                                                                 \
+    if (few) hipLaunchKernelGGL((block_select_kernel<T, NI, true>), dim3(batch * kv_heads * nq), dim3(64), 0, s, a);   \
+    else hipLaunchKernelGGL((block_select_kernel<T, NI, false>), dim3(batch * kv_heads * nq), dim3(64), 0, s, a);      \
+  } while (0)
+    if (a.nb <= 256) BA_SELECT(4);
+    else if (a.nb <= 1024) BA_SELECT(16);
+    else BA_SELECT(64);
+#undef BA_SELECT
     YL_HIP(hipGetLastError());
     return 0;
   });
@@ -1048,7 +1108,7 @@ static int attend_launch(const AttendArgs& p, bool direct, hipStream_t s) {
   if (direct)
     hipLaunchKernelGGL((block_attend_kernel<T, KEYS, DK32, DV16, true>), dim3((unsigned)wg), dim3(64), 0, s, p);
   else
-    hipLaunchKernelGGL((block_attend_kernel<T, KEYS, DK32, DV16, false>), dim3((unsigned)wg), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((block_attend_kernel<T, KEYS, DK32, DV16, false>), dim3((unsigned)wg), dim3(256), (size_t)256 * p.range, s, p);
   YL_HIP(hipGetLastError());
   return 0;
 }
