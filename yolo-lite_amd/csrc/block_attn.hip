@@ -284,7 +284,7 @@ __device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int
     if (j < a.nb) {
       double s = 0;
       const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
-#pragma unroll 8
+#pragma unroll 2
       for (int d = 0; d < a.dk; ++d) s += qs[d] * m[d];
       key[x] = order_key(s, a.count[b * a.nb + j] > 0);
     }
@@ -572,12 +572,17 @@ struct Vec<__bf16> {
   typedef bf16x8 t8;
   typedef bf16x4 t4;
   static __device__ __forceinline__ f32x4 mfma(t8 a, t8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ unsigned pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
 };
 template <>
 struct Vec<_Float16> {
   typedef f16x8 t8;
   typedef _Float16 t4 __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ f32x4 mfma(t8 a, t8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ unsigned pack(float lo, float hi) {  // (round to nearest even)
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, h2{(_Float16)lo, (_Float16)hi});
+  }
 };
 
 struct AttendArgs {
@@ -586,8 +591,11 @@ struct AttendArgs {
   int groups, range, nrange;  // groups of 64 queries per image; groups of a workgroup's range; ranges
   unsigned short* starts;   // [batch * kv][groups][nb + 1]
   unsigned short* lists;    // [batch * kv][groups][64 * topk]: query (6 bits) << 6 | slot
-  void* part;               // [row][slots][DVP], row = ((b * kv + h) * nq + i) * group + head in the group
-  float2* ml;               // [row][slots]: maximum (log2), sum
+  int g0, gn, cq;           // this launch's groups of queries [g0, g0 + gn), and how many queries `part` has room for
+  long long mlrow;          // nq * group
+  int q32;                  // offsets of q inside a range of queries fit 32 bits, its strides 24
+  void* part;               // [row][slots][DVP], row = ((b * kv + h) * cq + i - 64 g0) * group + head in the group
+  float2* ml;               // [b * kv + h][slots][nq * group]: maximum (log2), sum -- rows together: a unit's neighbours share lines
 };
 
 // One wave per (image, kv head, 64 queries): the group's picks sorted by block.  A block counts once per query; slots that name no
@@ -611,8 +619,9 @@ __global__ __launch_bounds__(64) void block_lists_kernel(AttendArgs p) {
         atomicOr(&word[j], 1ull << lane);
         first |= 1ull << t;
       } else {
-        for (int g = 0; g < p.a.group * p.subs; ++g)
-          p.ml[(q * p.a.group + g / p.subs) * p.slots + t * p.subs + g % p.subs] = float2{-__builtin_huge_valf(), 0.f};
+        for (int u = 0; u < p.subs; ++u)
+          for (int g = 0; g < p.a.group; ++g)
+            p.ml[((long long)bh * p.slots + t * p.subs + u) * p.mlrow + (long long)i * p.a.group + g] = float2{-__builtin_huge_valf(), 0.f};
       }
     }
   __syncthreads();
@@ -651,7 +660,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   constexpr int KT = KEYS / 16, KS = KEYS / 32, DVP = DV16 * 16, VP = KEYS + 8;
   __shared__ __attribute__((aligned(16))) T sVt[DVP * VP];
   extern __shared__ unsigned rows[];  // [64 * range]: group in the range << 12 | query << 6 | slot
-  __shared__ int total;
+  __shared__ int first[DIRECT ? 1 : 65], from[DIRECT ? 1 : 64];  // per group of the range: its place in `rows`, in its list
   const BlockArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int g = lane >> 4, n = lane & 15;
@@ -673,8 +682,8 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     bool use = j >= 0 && j < a.nb;
     for (int t = 0; t < tdirect; ++t) use = use && pick[t] != j;
     if (!use) {
-      const long long row = ((long long)bh * a.nq + qdirect) * a.group;
-      for (int e = lane; e < a.group; e += 64) p.ml[(row + e) * p.slots + tdirect * p.subs + sub] = float2{ninf, 0.f};
+      const long long at = ((long long)bh * p.slots + tdirect * p.subs + sub) * p.mlrow + (long long)qdirect * a.group;
+      for (int e = lane; e < a.group; e += 64) p.ml[at + e] = float2{ninf, 0.f};
       if (p.slots == 1) {  // (nothing is joined: the result itself is zeros)
         const int b0 = bh / a.kv, h0 = bh % a.kv;
         for (int e = lane; e < a.group * a.dv; e += 64)
@@ -686,15 +695,15 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   } else {
     j = unit % a.nb;
     unit /= a.nb;
-    grp0 = unit % p.nrange * p.range;
+    grp0 = p.g0 + unit % p.nrange * p.range;
     bh = unit / p.nrange;
-    const int ng = min(p.range, p.groups - grp0);
-    if (wave == 0) {  // a lane per group: its share of the list, copied behind the ones before it
-      int from = 0, cnt = 0;
+    const int ng = min(p.range, p.g0 + p.gn - grp0);
+    if (wave == 0) {  // a lane per group: where its share of the list begins, here and there
+      int lo = 0, cnt = 0;
       const long long at = (long long)bh * p.groups + grp0 + lane;
       if (lane < ng) {
-        from = p.starts[at * (a.nb + 1) + j];
-        cnt = p.starts[at * (a.nb + 1) + j + 1] - from;
+        lo = p.starts[at * (a.nb + 1) + j];
+        cnt = p.starts[at * (a.nb + 1) + j + 1] - lo;
       }
       int x = cnt;
 #pragma unroll
@@ -702,12 +711,21 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
         const int y = __shfl_up(x, o);
         if (lane >= o) x += y;
       }
-      if (lane == 63) total = x;
-      for (int e = 0; e < cnt; ++e) rows[x - cnt + e] = (unsigned)lane << 12 | p.lists[at * (64 * a.topk) + from + e];
+      first[lane] = x - cnt;
+      from[lane] = lo;
+      if (lane == 63) first[64] = x;
     }
     __syncthreads();
+    const int total = first[64];
     nrows = total * a.group;
     if (nrows == 0) return;
+    for (int e = tid; e < total; e += NT) {  // the group that holds entry e: the last one that begins at or before it
+      int x = 0;
+#pragma unroll
+      for (int o = 32; o; o >>= 1) x += first[x + o] <= e ? o : 0;
+      const long long at = ((long long)bh * p.groups + grp0 + x) * (64 * a.topk);
+      rows[e] = (unsigned)x << 12 | p.lists[at + from[x] + e - first[x]];
+    }
   }
   const int h = bh % a.kv, b = bh / a.kv;
   const int k0 = j * a.block + sub * KEYS;
@@ -761,13 +779,17 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
 #pragma unroll
   for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
 
-  // a tile's queries: lane column n is (query, head) row f
+  // a tile's queries: lane column n is (query, head) row f.  q0: the first query that this unit may have; everything per row is a
+  // 24-bit product from there (a full 32-bit one takes four times as long)
   struct Row {
-    int q, head, slot;  // query of the image
+    int q, head, slot;  // query behind q0
     bool live;
     t8 f[DK32];
   };
-  const T* const qb = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)(h * a.group) * a.q.sh;
+  const int q0 = DIRECT ? qdirect : grp0 * 64;
+  const T* const qb = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)q0 * a.q.st + (long long)(h * a.group) * a.q.sh;
+  T* const pb = static_cast<T*>(p.part) + ((long long)bh * p.cq + (q0 - p.g0 * 64)) * a.group * p.slots * DVP;
+  float2* const mlb = p.ml + (long long)bh * p.slots * p.mlrow + (long long)q0 * a.group;
   auto fetch = [&](int tile, Row& w) __attribute__((always_inline)) {
     const int f = tile * 16 + n;
     w.live = f < nrows;
@@ -776,24 +798,25 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     w.head = 0;
     if (a.group > 1) {
       e = (int)__umulhi((unsigned)fc, a.magic);
-      w.head = fc - e * a.group;
+      w.head = fc - __mul24(e, a.group);
     }
     if constexpr (DIRECT) {
-      w.q = qdirect;
-      w.slot = tdirect;
+      w.q = 0;
+      w.slot = tdirect * p.subs + sub;
     } else {
       const unsigned x = rows[e];
-      w.q = (grp0 + (int)(x >> 12)) * 64 + (int)(x >> 6 & 63);
-      w.slot = (int)(x & 63);
+      w.q = (int)(x >> 6);
+      w.slot = __mul24((int)(x & 63), p.subs) + sub;
     }
-    const T* qp = qb + w.q * a.q.st + w.head * a.q.sh;
+    const T* qp;
+    if (p.q32)
+      qp = qb + (unsigned)(__umul24((unsigned)w.q, (unsigned)a.q.st) + __umul24((unsigned)w.head, (unsigned)a.q.sh));
+    else
+      qp = qb + w.q * a.q.st + w.head * a.q.sh;
 #pragma unroll
     for (int c = 0; c < DK32; ++c) {
-      u32x4 x = {0, 0, 0, 0};
-      if ((c * 4 + g) * 8 < a.dk) x = *reinterpret_cast<const u32x4*>(qp + (c * 4 + g) * 8);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) x[d] ^= flip;
-      w.f[c] = __builtin_bit_cast(t8, x);
+      w.f[c] = t8{};
+      if ((c * 4 + g) * 8 < a.dk) w.f[c] = *reinterpret_cast<const t8*>(qp + (c * 4 + g) * 8);
     }
   };
   const int ntiles = (nrows + 15) >> 4;
@@ -801,8 +824,16 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   Row next;
   if (wave < ntiles) fetch(wave, next);
   for (int tile = wave; tile < ntiles; tile += NW) {
-    const Row w = next;
+    Row w = next;
     if (tile + NW < ntiles) fetch(tile + NW, next);
+    if (flip)
+#pragma unroll
+      for (int c = 0; c < DK32; ++c) {
+        u32x4 x = __builtin_bit_cast(u32x4, w.f[c]);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) x[d] ^= flip;
+        w.f[c] = __builtin_bit_cast(t8, x);
+      }
     f32x4 s[KT];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
@@ -811,18 +842,21 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       for (int c = 0; c < DK32; ++c) s[t] = Vec<T>::mfma(kf[t][c], w.f[c], s[t]);
     }
     float m = ninf;
-    t8 pf[KS];
+    u32x4 pw[KS];
     if (all) {
+      // max(x, y) = med3(x, y, inf): one instruction where fmaxf first quiets a possible signalling NaN (a NaN score makes NaN below)
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m = fmaxf(m, s[t][r]);
+        for (int r = 0; r < 4; ++r) m = __builtin_amdgcn_fmed3f(m, s[t][r], __builtin_huge_valf());
       m = quad_max(m) * scale;
       const float base = m == ninf ? 0.f : m;  // (every score -inf: all weights 0)
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) pf[t >> 1][(t & 1) * 4 + r] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -base));
+        for (int r = 0; r < 4; r += 2)
+          pw[t >> 1][(t & 1) * 2 + r / 2] = Vec<T>::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -base)),
+                                                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + 1], scale, -base)));
     } else {
 #pragma unroll
       for (int t = 0; t < KT; ++t)
@@ -834,9 +868,14 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          pf[t >> 1][(t & 1) * 4 + r] = okt >> (4 * t + r) & 1 ? (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -base)) : (T)0.f;
+        for (int r = 0; r < 4; r += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], scale, -base)), e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r + 1], scale, -base));
+          pw[t >> 1][(t & 1) * 2 + r / 2] = Vec<T>::pack(okt >> (4 * t + r) & 1 ? e0 : 0.f, okt >> (4 * t + r + 1) & 1 ? e1 : 0.f);
+        }
     }
+    t8 pf[KS];
+#pragma unroll
+    for (int x = 0; x < KS; ++x) pf[x] = __builtin_bit_cast(t8, pw[x]);
     // the weights' sum by the matrix pipe too: a row of ones; every lane of a query gets it, and it is the sum of what multiplies v
     f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -851,18 +890,17 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     }
     const float inv = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);
     if (!w.live) continue;
-    const unsigned row = ((unsigned)bh * (unsigned)a.nq + (unsigned)w.q) * (unsigned)a.group + (unsigned)w.head;  // (below 2^31)
-    const long long at = (long long)row * p.slots + w.slot * p.subs + sub;
-    T* dst = alone ? static_cast<T*>(const_cast<void*>(a.o.p)) + b * a.o.sb + w.q * a.o.st + (long long)(h * a.group + w.head) * a.o.sh
-                   : static_cast<T*>(p.part) + at * DVP;
+    const unsigned local = __umul24((unsigned)w.q, (unsigned)a.group) + (unsigned)w.head;  // row behind q0's first: below 4096 * 1000
+    T* dst = alone ? static_cast<T*>(const_cast<void*>(a.o.p)) + b * a.o.sb + (long long)(q0 + w.q) * a.o.st + (long long)(h * a.group + w.head) * a.o.sh
+                   : pb + (long long)(__umul24(local, (unsigned)p.slots) + (unsigned)w.slot) * DVP;
 #pragma unroll
     for (int d = 0; d < DV16; d += 2) {
       const int c = g * (DVP / 4) + d * 4;
-      const t8 y = {(T)(o[d][0] * inv), (T)(o[d][1] * inv), (T)(o[d][2] * inv), (T)(o[d][3] * inv),
-                    (T)(o[d + 1][0] * inv), (T)(o[d + 1][1] * inv), (T)(o[d + 1][2] * inv), (T)(o[d + 1][3] * inv)};
-      if (!alone || c < a.dv) *reinterpret_cast<t8*>(dst + c) = y;
+      const u32x4 y = {Vec<T>::pack(o[d][0] * inv, o[d][1] * inv), Vec<T>::pack(o[d][2] * inv, o[d][3] * inv),
+                       Vec<T>::pack(o[d + 1][0] * inv, o[d + 1][1] * inv), Vec<T>::pack(o[d + 1][2] * inv, o[d + 1][3] * inv)};
+      if (!alone || c < a.dv) *reinterpret_cast<u32x4*>(dst + c) = y;
     }
-    if (!alone && g == 0) p.ml[at] = float2{m, l};
+    if (!alone && g == 0) mlb[(long long)w.slot * p.mlrow + local] = float2{m, l};
   }
 }
 
@@ -874,16 +912,19 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   constexpr int C = DVP / 8;
   const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
   const int c = (int)(item % C) * 8;
-  const long long row = item / C;
-  if (row >= (long long)a.batch * a.nq * a.heads || c >= a.dv) return;
-  const float2* ml = p.ml + row * p.slots;
-  const T* part = static_cast<const T*>(p.part) + row * p.slots * DVP + c;
+  const long long prow = item / C;  // rows of this launch's queries
+  const int cq = min(p.gn * 64, a.nq - p.g0 * 64);
+  if (prow >= (long long)a.batch * a.kv * cq * a.group || c >= a.dv) return;
+  const int gh = (int)(prow % a.group);
+  const int i = p.g0 * 64 + (int)(prow / a.group % cq), bh = (int)(prow / a.group / cq);
+  const float2* ml = p.ml + (long long)bh * p.slots * p.mlrow + (long long)i * a.group + gh;
+  const T* part = static_cast<const T*>(p.part) + (((long long)bh * p.cq + i - p.g0 * 64) * a.group + gh) * p.slots * DVP + c;
   constexpr int U = 8;  // slots whose loads are in flight together
   float m = -__builtin_huge_valf();
   for (int t0 = 0; t0 < p.slots; t0 += U) {
     float x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = ml[min(t0 + u, p.slots - 1)].x;
+    for (int u = 0; u < U; ++u) x[u] = ml[min(t0 + u, p.slots - 1) * p.mlrow].x;
 #pragma unroll
     for (int u = 0; u < U; ++u) m = fmaxf(m, x[u]);
   }
@@ -895,7 +936,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int t = min(t0 + u, p.slots - 1);
-      const float2 x = ml[t];
+      const float2 x = ml[t * p.mlrow];
       y[u] = *reinterpret_cast<const t8*>(part + t * DVP);  // (whatever lies there where the slot has no block: not used)
       w[u] = t0 + u < p.slots ? x.y * __builtin_amdgcn_exp2f(x.x - base) : 0.f;
     }
@@ -908,9 +949,6 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int gh = (int)(row % a.group);
-  const long long q = row / a.group;
-  const int i = (int)(q % a.nq), bh = (int)(q / a.nq);
   t8 y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv);
@@ -1067,10 +1105,12 @@ extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, 
 // ---- how the attention runs: sizes, and where things lie in the workspace
 struct AttendPlan {
   bool direct;
-  int subs, slots, groups, range, nrange, dvp;
+  int subs, slots, groups, range, dvp;
+  int chunk;               // groups of queries whose block results are in memory together
   long long starts, lists, part, ml, all;  // byte offsets
 };
 
+constexpr long long CHUNK_BYTES = 256LL << 20;  // block results in memory at once (measured: 128 MB and more the same time, 64 MB 15 % more, 16 MB twice)
 static AttendPlan plan_attend(const BlockArgs& a, int dv) {
   AttendPlan p{};
   p.subs = a.block == 128 ? 2 : 1;
@@ -1079,12 +1119,16 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv) {
   p.groups = (a.nq + 63) / 64;
   // the lists pay where a block is picked often; below that, a wave per (query, block)
   p.direct = a.nq <= 4 || (long long)a.nq * a.topk <= 2LL * a.nb;
-  // a workgroup's range of queries: about 256 (query, head) rows, 16 tiles, for an average block
+  // a workgroup's range of queries: about 512 (query, head) rows, 32 tiles, for an average block
   const long long per64 = 64LL * a.topk * a.group;
-  p.range = (int)std::min<long long>(64, std::max<long long>(1, 256LL * std::max(1, a.nb) / per64));
-  p.range = std::min(p.range, p.groups);
-  p.nrange = p.range ? (p.groups + p.range - 1) / p.range : 0;
+  p.range = (int)std::min<long long>(64, std::max<long long>(1, 512LL * std::max(1, a.nb) / per64));
   const long long rows = (long long)a.batch * a.nq * a.heads, bg = (long long)a.batch * a.kv * p.groups;
+  p.chunk = p.groups;
+  if (!p.direct) {
+    const long long group_bytes = 2LL * a.batch * a.heads * 64 * p.slots * p.dvp;
+    p.chunk = (int)std::min<long long>(p.groups, std::max<long long>(1, CHUNK_BYTES / group_bytes));
+  }
+  p.range = std::min(p.range, p.chunk);
   long long at = 0;
   auto take = [&](long long n) {
     const long long o = at;
@@ -1094,7 +1138,8 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv) {
   p.starts = take(p.direct ? 0 : 2 * bg * (a.nb + 1));
   p.lists = take(p.direct ? 0 : 2 * bg * 64 * a.topk);
   p.ml = take(8 * rows * p.slots);
-  p.part = take(p.slots == 1 && p.direct ? 0 : 2 * rows * p.slots * p.dvp);
+  const long long cq = p.direct ? a.nq : 64LL * p.chunk;
+  p.part = take(p.slots == 1 && p.direct ? 0 : 2LL * a.batch * a.heads * cq * p.slots * p.dvp);
   p.all = at;
   return p;
 }
@@ -1153,7 +1198,10 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
   a.o = Heads{out->data, out->batch, out->token, out->head};
   a.dv = dv, a.scale = scale, a.picked = const_cast<int32_t*>(picked);
   char* const w = static_cast<char*>(work);
-  p.subs = pl.subs, p.slots = pl.slots, p.groups = pl.groups, p.range = pl.range, p.nrange = pl.nrange;
+  p.subs = pl.subs, p.slots = pl.slots, p.groups = pl.groups, p.range = pl.range;
+  p.gn = pl.groups, p.cq = pl.direct ? nq : 64 * pl.chunk;
+  p.mlrow = (long long)nq * a.group;
+  p.q32 = a.q.st < (1 << 24) && a.q.sh < (1 << 24) && 4096 * a.q.st + 1024 * a.q.sh < (1LL << 31);
   p.starts = reinterpret_cast<unsigned short*>(w + pl.starts), p.lists = reinterpret_cast<unsigned short*>(w + pl.lists);
   p.part = w + pl.part, p.ml = reinterpret_cast<float2*>(w + pl.ml);
   if (!pl.direct) {
@@ -1162,15 +1210,19 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
   }
   return by_type16(dtype, [&](auto* t) {
     typedef BA_T(t) T;
-    if (a.nb > 0 || pl.direct)
-      if (int rc = block == 32 ? attend_by_width<T, 32>(p, pl.direct, s) : attend_by_width<T, 64>(p, pl.direct, s)) return rc;
-    if (pl.slots == 1 && pl.direct) return 0;
-    const long long items = (long long)batch * nq * heads * (pl.dvp / 8);
-    if (pl.dvp == 64)
-      hipLaunchKernelGGL((block_join_kernel<T, 64>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
-    else
-      hipLaunchKernelGGL((block_join_kernel<T, 128>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
-    YL_HIP(hipGetLastError());
+    for (int g0 = 0; g0 < pl.groups; g0 += pl.chunk) {
+      p.g0 = g0, p.gn = std::min(pl.chunk, pl.groups - g0);
+      p.nrange = (p.gn + pl.range - 1) / pl.range;
+      if (a.nb > 0 || pl.direct)
+        if (int rc = block == 32 ? attend_by_width<T, 32>(p, pl.direct, s) : attend_by_width<T, 64>(p, pl.direct, s)) return rc;
+      if (pl.slots == 1 && pl.direct) return 0;
+      const long long items = (long long)batch * std::min(64 * p.gn, nq - 64 * g0) * heads * (pl.dvp / 8);
+      if (pl.dvp == 64)
+        hipLaunchKernelGGL((block_join_kernel<T, 64>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
+      else
+        hipLaunchKernelGGL((block_join_kernel<T, 128>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
+      YL_HIP(hipGetLastError());
+    }
     return 0;
   });
 }
