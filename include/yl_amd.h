@@ -392,7 +392,8 @@ int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, int batch, 
 /* out[b][i][h] = softmax over the readable keys of the blocks picked[b][h's kv head][i] of (scale * q . k), times v.  Entries of
  * `picked` outside [0, blocks) are no block; a block named twice counts once; the order does not matter.  fp32 accumulation.
  * `work` as above, yl_block_attention_workspace_bytes bytes. */
-int64_t yl_block_attention_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block, int topk);
+int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block,
+                                           int topk);
 int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl_heads* v, int dtype, int batch, int nq, int nk, int heads,
                        int kv_heads, int dk, int dv, int block, int topk, const int32_t* picked, const uint8_t* mask,
                        int64_t mask_stride, float scale, const yl_heads* out, void* work, int64_t work_bytes, void* stream);

@@ -92,7 +92,7 @@ def test_workspace_refusals():
     assert need > 0 and _run("select", dict(work_bytes=need - 1)) == -1 and _run("select", dict(work=None)) == -1
     assert _run("select", dict(work=8200)) == -1
     assert L.yl_block_select_workspace_bytes(1, 4, 100, 4, 3, 32, 64) == -1
-    assert L.yl_block_attention_workspace_bytes(1, 4, 100, 4, 2, 32, 62, 64, 2) == -1
+    assert L.yl_block_attention_workspace_bytes(0, 1, 4, 100, 4, 2, 32, 62, 64, 2) == -1
 
 
 def test_nothing_to_do_is_no_error():

@@ -279,7 +279,7 @@ def lib() -> C.CDLL:
     L.yl_block_select.restype = i32
     L.yl_block_select.argtypes = [hp, hp] + [i32] * 9 + [vp, i64, vp, vp, i64, vp]
     L.yl_block_attention_workspace_bytes.restype = i64
-    L.yl_block_attention_workspace_bytes.argtypes = [i32] * 9
+    L.yl_block_attention_workspace_bytes.argtypes = [i32] * 10
     L.yl_block_attention.restype = i32
     L.yl_block_attention.argtypes = [hp, hp, hp] + [i32] * 10 + [vp, vp, i64, f32, hp, vp, i64, vp]
     if L.yl_abi_version() != 21:

@@ -559,8 +559,10 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
 // joins a row's blocks.  Keys are read once per block and range of queries instead of once per query; the price is that every (row,
 // block) result passes through memory, which is what bounds the stage (2 (dv + 4) bytes written and read per row and block).
 //
-// Results of a block are rounded to the tensors' type between the launches: as exact as the weights P themselves, which the matrix
-// pipe takes in that type, and half the traffic; maxima, sums and the joining are fp32.
+// A block's results pass unnormalised (sum of p v; the maximum and sum of p beside them in fp32).  For fp16 tensors they are fp32.  For
+// bf16 tensors they are fp16, toward zero (2^-10 at most, a quarter of a bf16 step; fp32 took 278 instead of 150 us on the 128x128
+// map): the unit's values are scaled by a power of two, exact in bf16, that puts their largest at 2^8, so that the sums fill fp16's
+// range from the top and what lies up to 2^23 below the largest value still has all its bits; the join scales back.
 //
 // Lists: 64 queries form a group; lists[group] holds its (query, slot) pairs sorted by block, starts[group][j] where block j's begin.
 // A block of 128 keys is two units of 64 (two results per slot): one unit's fragments fill the registers.
@@ -569,6 +571,7 @@ template <typename T>
 struct Vec;
 template <>
 struct Vec<__bf16> {
+  typedef _Float16 part;  // a block's results between the launches
   typedef bf16x8 t8;
   typedef bf16x4 t4;
   static __device__ __forceinline__ f32x4 mfma(t8 a, t8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -576,6 +579,7 @@ struct Vec<__bf16> {
 };
 template <>
 struct Vec<_Float16> {
+  typedef float part;
   typedef f16x8 t8;
   typedef _Float16 t4 __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ f32x4 mfma(t8 a, t8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -594,6 +598,7 @@ struct AttendArgs {
   int g0, gn, cq;           // this launch's groups of queries [g0, g0 + gn), and how many queries `part` has room for
   long long mlrow;          // nq * group
   int q32;                  // offsets of q inside a range of queries fit 32 bits, its strides 24
+  signed char* vexp;        // [b * kv + h][nb * subs]: bf16 tensors: a unit's results are times 2^vexp
   void* part;               // [row][slots][DVP], row = ((b * kv + h) * cq + i - 64 g0) * group + head in the group
   float2* ml;               // [b * kv + h][slots][nq * group]: maximum (log2), sum -- rows together: a unit's neighbours share lines
 };
@@ -657,6 +662,8 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   typedef typename Vec<T>::t8 t8;
   typedef typename Vec<T>::t4 t4;
   constexpr int NT = DIRECT ? 64 : 256;
+  typedef typename Vec<T>::part part_t;
+  constexpr bool HALF = sizeof(part_t) == 2;
   constexpr int KT = KEYS / 16, KS = KEYS / 32, DVP = DV16 * 16, VP = KEYS + 8;
   __shared__ __attribute__((aligned(16))) T sVt[DVP * VP];
   extern __shared__ unsigned rows[];  // [64 * range]: group in the range << 12 | query << 6 | slot
@@ -732,19 +739,55 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   const int kn = min(min(KEYS, a.block - sub * KEYS), a.nk - k0);  // keys of this unit; <= 0: none
   const bool lok = lane < kn && (!a.mask || a.mask[b * a.mask_stride + k0 + lane]);
   const unsigned long long ok = __ballot(lok);  // the keys that may be read
+  const bool alone = DIRECT && p.slots == 1;  // a row has this one result: it is the output
   // ---- values, transposed, keys in a row; a masked value counts as 0 whatever it holds
+  __shared__ unsigned vmax;
+  if (HALF && !alone) {
+    if (tid == 0) vmax = 0;
+    __syncthreads();
+  }
   const T* vb = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh;
-  for (int it = tid; it < KEYS / 8 * (DVP / 8); it += NT) {
-    const int c8 = it % (DVP / 8), kg = it / (DVP / 8);
-    t8 v[8];
+  constexpr int NV = (KEYS / 8 * (DVP / 8) + NT - 1) / NT;  // 8 x 8 pieces of a thread
+  t8 v[NV][8];
+  unsigned big = 0;  // bits of the largest finite |v|
+#pragma unroll
+  for (int x = 0; x < NV; ++x) {
+    const int it = tid + x * NT, c8 = it % (DVP / 8), kg = it / (DVP / 8);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      v[u] = t8{};
-      if (c8 * 8 < a.dv && (ok >> (kg * 8 + u) & 1)) v[u] = *reinterpret_cast<const t8*>(vb + (long long)(k0 + kg * 8 + u) * a.v.st + c8 * 8);
+      v[x][u] = t8{};
+      if (it < KEYS / 8 * (DVP / 8) && c8 * 8 < a.dv && (ok >> (kg * 8 + u) & 1))
+        v[x][u] = *reinterpret_cast<const t8*>(vb + (long long)(k0 + kg * 8 + u) * a.v.st + c8 * 8);
     }
+    if (HALF && !alone)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      *reinterpret_cast<t8*>(sVt + (c8 * 8 + e) * VP + kg * 8) = t8{v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned m = __float_as_uint((float)v[x][u][e]) & 0x7FFFFFFFu;
+          big = max(big, m < 0x7F800000u ? m : 0u);
+        }
+  }
+  float vscale = 1.f;
+  if (HALF && !alone) {
+    if (big) atomicMax(&vmax, big);
+    __syncthreads();
+    const int e = (int)(vmax >> 23) - 127;                // floor(log2 of the largest); -127: zeros, or not normal
+    const int up = vmax ? min(8 - e, 126) : 0;            // 2^up puts it at 2^8: sums of 64 weighted values stay under 2^15
+    vscale = up > -127 ? __uint_as_float((unsigned)(up + 127) << 23) : 0.f;
+    if (tid == 0) p.vexp[((long long)bh * a.nb + j) * p.subs + sub] = (signed char)-up;
+  }
+#pragma unroll
+  for (int x = 0; x < NV; ++x) {
+    const int it = tid + x * NT, c8 = it % (DVP / 8), kg = it / (DVP / 8);
+    if (it < KEYS / 8 * (DVP / 8))
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        t8 y;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[u] = HALF ? (T)((float)v[x][u][e] * vscale) : v[x][u][e];
+        *reinterpret_cast<t8*>(sVt + (c8 * 8 + e) * VP + kg * 8) = y;
+      }
   }
   // ---- keys: fragments of the first product (row = key, 8 dims of group g)
   t8 kf[KT][DK32];
@@ -760,13 +803,14 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
 #pragma unroll
   for (int t = 0; t < KT; ++t) okt |= (unsigned)(ok >> (t * 16 + 4 * g) & 15) << (4 * t);
   __syncthreads();
-  // values: row i of tile d is channel (i / 4) (DVP / 4) + 4 d + i % 4, so that a lane ends up with DVP / 4 neighbouring channels
+  // values: which channel is row i of tile d -- one that lets the four lanes of a query store 64 neighbouring bytes at a time
+  auto channel = [](int d, int i) { return HALF ? (d >> 1) * 32 + (i >> 2) * 8 + (d & 1) * 4 + (i & 3) : d * 16 + i; };
   t8 vf[DV16][KS];
 #pragma unroll
   for (int d = 0; d < DV16; ++d)
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const T* vr = sVt + ((n >> 2) * (DVP / 4) + d * 4 + (n & 3)) * VP + s * 32 + 4 * g;
+      const T* vr = sVt + channel(d, n) * VP + s * 32 + 4 * g;
       const t4 lo = *reinterpret_cast<const t4*>(vr), hi = *reinterpret_cast<const t4*>(vr + 16);
       vf[d][s] = t8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     }
@@ -774,7 +818,6 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   const float scale = fabsf(a.scale) * 1.44269504088896340736f;
   const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
   const bool all = ok == (KEYS == 64 ? ~0ull : (1ull << KEYS) - 1);  // no key is masked: uniform
-  const bool alone = DIRECT && p.slots == 1;  // a row has this one result: it is the output
   t8 one;
 #pragma unroll
   for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
@@ -788,7 +831,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   };
   const int q0 = DIRECT ? qdirect : grp0 * 64;
   const T* const qb = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)q0 * a.q.st + (long long)(h * a.group) * a.q.sh;
-  T* const pb = static_cast<T*>(p.part) + ((long long)bh * p.cq + (q0 - p.g0 * 64)) * a.group * p.slots * DVP;
+  part_t* const pb = static_cast<part_t*>(p.part) + ((long long)bh * p.cq + (q0 - p.g0 * 64)) * a.group * p.slots * DVP;
   float2* const mlb = p.ml + (long long)bh * p.slots * p.mlrow + (long long)q0 * a.group;
   auto fetch = [&](int tile, Row& w) __attribute__((always_inline)) {
     const int f = tile * 16 + n;
@@ -888,19 +931,31 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
 #pragma unroll
       for (int x = 0; x < KS; ++x) o[d] = Vec<T>::mfma(vf[d][x], pf[x], o[d]);
     }
-    const float inv = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);
     if (!w.live) continue;
     const unsigned local = __umul24((unsigned)w.q, (unsigned)a.group) + (unsigned)w.head;  // row behind q0's first: below 4096 * 1000
-    T* dst = alone ? static_cast<T*>(const_cast<void*>(a.o.p)) + b * a.o.sb + (long long)(q0 + w.q) * a.o.st + (long long)(h * a.group + w.head) * a.o.sh
-                   : pb + (long long)(__umul24(local, (unsigned)p.slots) + (unsigned)w.slot) * DVP;
+    if (alone) {
+      T* const dst = static_cast<T*>(const_cast<void*>(a.o.p)) + b * a.o.sb + (long long)(q0 + w.q) * a.o.st + (long long)(h * a.group + w.head) * a.o.sh;
+      const float inv = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);
 #pragma unroll
-    for (int d = 0; d < DV16; d += 2) {
-      const int c = g * (DVP / 4) + d * 4;
-      const u32x4 y = {Vec<T>::pack(o[d][0] * inv, o[d][1] * inv), Vec<T>::pack(o[d][2] * inv, o[d][3] * inv),
-                       Vec<T>::pack(o[d + 1][0] * inv, o[d + 1][1] * inv), Vec<T>::pack(o[d + 1][2] * inv, o[d + 1][3] * inv)};
-      if (!alone || c < a.dv) *reinterpret_cast<u32x4*>(dst + c) = y;
+      for (int d = 0; d < DV16; ++d) {
+        const int c = channel(d, 4 * g);
+        const u32x2 y = {Vec<T>::pack(o[d][0] * inv, o[d][1] * inv), Vec<T>::pack(o[d][2] * inv, o[d][3] * inv)};
+        if (c < a.dv) *reinterpret_cast<u32x2*>(dst + c) = y;
+      }
+      continue;
     }
-    if (!alone && g == 0) mlb[(long long)w.slot * p.mlrow + local] = float2{m, l};
+    part_t* const dst = pb + (long long)(__umul24(local, (unsigned)p.slots) + (unsigned)w.slot) * DVP;
+    if constexpr (HALF) {
+      auto pk = [](float lo, float hi) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(lo, hi)); };
+#pragma unroll
+      for (int d = 0; d < DV16; d += 2)
+        *reinterpret_cast<u32x4*>(dst + channel(d, 4 * g)) =
+            u32x4{pk(o[d][0], o[d][1]), pk(o[d][2], o[d][3]), pk(o[d + 1][0], o[d + 1][1]), pk(o[d + 1][2], o[d + 1][3])};
+    } else {
+#pragma unroll
+      for (int d = 0; d < DV16; ++d) *reinterpret_cast<f32x4*>(dst + channel(d, 4 * g)) = o[d];
+    }
+    if (g == 0) mlb[(long long)w.slot * p.mlrow + local] = float2{m, l};
   }
 }
 
@@ -918,7 +973,11 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   const int gh = (int)(prow % a.group);
   const int i = p.g0 * 64 + (int)(prow / a.group % cq), bh = (int)(prow / a.group / cq);
   const float2* ml = p.ml + (long long)bh * p.slots * p.mlrow + (long long)i * a.group + gh;
-  const T* part = static_cast<const T*>(p.part) + (((long long)bh * p.cq + i - p.g0 * 64) * a.group + gh) * p.slots * DVP + c;
+  typedef typename Vec<T>::part part_t;
+  typedef part_t p8 __attribute__((ext_vector_type(8)));
+  constexpr bool HALF = sizeof(part_t) == 2;
+  const int* pick = a.picked + ((long long)bh * a.nq + i) * a.topk;
+  const part_t* part = static_cast<const part_t*>(p.part) + (((long long)bh * p.cq + i - p.g0 * 64) * a.group + gh) * p.slots * DVP + c;
   constexpr int U = 8;  // slots whose loads are in flight together
   float m = -__builtin_huge_valf();
   for (int t0 = 0; t0 < p.slots; t0 += U) {
@@ -931,21 +990,29 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   const float base = m == -__builtin_huge_valf() ? 0.f : m;
   float acc[8] = {}, sum = 0.f;
   for (int t0 = 0; t0 < p.slots; t0 += U) {
-    float w[U];
-    t8 y[U];
+    float w[U], l[U];
+    int ve[U];
+    p8 y[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int t = min(t0 + u, p.slots - 1);
       const float2 x = ml[t * p.mlrow];
-      y[u] = *reinterpret_cast<const t8*>(part + t * DVP);  // (whatever lies there where the slot has no block: not used)
-      w[u] = t0 + u < p.slots ? x.y * __builtin_amdgcn_exp2f(x.x - base) : 0.f;
+      y[u] = *reinterpret_cast<const p8*>(part + t * DVP);  // (whatever lies there where the slot has no block: not used)
+      ve[u] = 0;
+      if constexpr (HALF) {
+        const int j = pick[p.subs == 2 ? t >> 1 : t];
+        ve[u] = p.vexp[((long long)bh * a.nb + (j >= 0 && j < a.nb ? j : 0)) * p.subs + (p.subs == 2 ? t & 1 : 0)];
+      }
+      w[u] = __builtin_amdgcn_exp2f(x.x - base);
+      l[u] = t0 + u < p.slots ? x.y : 0.f;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (w[u] == 0.f) continue;
-      sum += w[u];
+      if (l[u] == 0.f) continue;
+      sum += w[u] * l[u];
+      const float x = HALF ? __builtin_amdgcn_ldexpf(w[u], ve[u]) : w[u];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += w[u] * (float)y[u][e];
+      for (int e = 0; e < 8; ++e) acc[e] += x * (float)y[u][e];
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -1107,11 +1174,12 @@ struct AttendPlan {
   bool direct;
   int subs, slots, groups, range, dvp;
   int chunk;               // groups of queries whose block results are in memory together
-  long long starts, lists, part, ml, all;  // byte offsets
+  long long starts, lists, vexp, part, ml, all;  // byte offsets
 };
 
 constexpr long long CHUNK_BYTES = 256LL << 20;  // block results in memory at once (measured: 128 MB and more the same time, 64 MB 15 % more, 16 MB twice)
-static AttendPlan plan_attend(const BlockArgs& a, int dv) {
+static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
+  const int part_bytes = dtype == YL_BF16 ? 2 : 4;
   AttendPlan p{};
   p.subs = a.block == 128 ? 2 : 1;
   p.slots = a.topk * p.subs;
@@ -1125,7 +1193,7 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv) {
   const long long rows = (long long)a.batch * a.nq * a.heads, bg = (long long)a.batch * a.kv * p.groups;
   p.chunk = p.groups;
   if (!p.direct) {
-    const long long group_bytes = 2LL * a.batch * a.heads * 64 * p.slots * p.dvp;
+    const long long group_bytes = (long long)part_bytes * a.batch * a.heads * 64 * p.slots * p.dvp;
     p.chunk = (int)std::min<long long>(p.groups, std::max<long long>(1, CHUNK_BYTES / group_bytes));
   }
   p.range = std::min(p.range, p.chunk);
@@ -1137,9 +1205,10 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv) {
   };
   p.starts = take(p.direct ? 0 : 2 * bg * (a.nb + 1));
   p.lists = take(p.direct ? 0 : 2 * bg * 64 * a.topk);
+  p.vexp = take((long long)a.batch * a.kv * std::max(1, a.nb) * p.subs);
   p.ml = take(8 * rows * p.slots);
   const long long cq = p.direct ? a.nq : 64LL * p.chunk;
-  p.part = take(p.slots == 1 && p.direct ? 0 : 2LL * a.batch * a.heads * cq * p.slots * p.dvp);
+  p.part = take(p.slots == 1 && p.direct ? 0 : (long long)part_bytes * a.batch * a.heads * cq * p.slots * p.dvp);
   p.all = at;
   return p;
 }
@@ -1165,16 +1234,16 @@ static int attend_by_width(const AttendArgs& p, bool direct, hipStream_t s) {
   return dk <= 32 ? attend_launch<T, KEYS, 1, 8>(p, direct, s) : dk <= 64 ? attend_launch<T, KEYS, 2, 8>(p, direct, s) : attend_launch<T, KEYS, 4, 8>(p, direct, s);
 }
 
-extern "C" int64_t yl_block_attention_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block,
+extern "C" int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block,
                                                       int topk) {
   BlockArgs a{};
   yl_heads dummy{reinterpret_cast<void*>(16), 0, 0, 0};
-  if (fill_args("block_attention", &dummy, &dummy, YL_BF16, batch, nq, nk, heads, kv_heads, dk, block, topk, nullptr, 0, &a)) return -1;
+  if (fill_args("block_attention", &dummy, &dummy, dtype, batch, nq, nk, heads, kv_heads, dk, block, topk, nullptr, 0, &a)) return -1;
   if (dv < 8 || dv > 128 || dv % 8) {
     fail(-3, "block_attention: value widths are multiples of 8 up to 128");
     return -1;
   }
-  return batch * (long long)nq == 0 ? 0 : plan_attend(a, dv).all;
+  return batch * (long long)nq == 0 ? 0 : plan_attend(a, dv, dtype).all;
 }
 
 extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl_heads* v, int dtype, int batch, int nq, int nk,
@@ -1191,7 +1260,7 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
     if (int rc = check_heads("block_attention", "v", v)) return rc;
   if (int rc = check_heads("block_attention", "out", out)) return rc;
   if (!picked) return fail(-1, "block_attention: null pointer");
-  const AttendPlan pl = plan_attend(a, dv);
+  const AttendPlan pl = plan_attend(a, dv, dtype);
   if (!work || work_bytes < pl.all || (reinterpret_cast<uintptr_t>(work) & 15))
     return fail(-1, "block_attention: workspace missing, too small or not 16-byte aligned");
   if (nk > 0) a.v = Heads{v->data, v->batch, v->token, v->head};
@@ -1203,7 +1272,7 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
   p.mlrow = (long long)nq * a.group;
   p.q32 = a.q.st < (1 << 24) && a.q.sh < (1 << 24) && 4096 * a.q.st + 1024 * a.q.sh < (1LL << 31);
   p.starts = reinterpret_cast<unsigned short*>(w + pl.starts), p.lists = reinterpret_cast<unsigned short*>(w + pl.lists);
-  p.part = w + pl.part, p.ml = reinterpret_cast<float2*>(w + pl.ml);
+  p.vexp = reinterpret_cast<signed char*>(w + pl.vexp), p.part = w + pl.part, p.ml = reinterpret_cast<float2*>(w + pl.ml);
   if (!pl.direct) {
     hipLaunchKernelGGL(block_lists_kernel, dim3((unsigned)(batch * kv_heads * pl.groups)), dim3(64), (size_t)a.nb * 10 + 16, s, p);
     YL_HIP(hipGetLastError());

@@ -88,7 +88,7 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, picked: t
         raise ValueError(f"block_attention: picked (batch, kv heads, nq, topk) in int32 is needed, got {tuple(picked.shape)} in {picked.dtype}")
     dv, topk = v.shape[3], picked.shape[3]
     L = _lib.lib()
-    nbytes = L.yl_block_attention_workspace_bytes(batch, nq, nk, heads, kv, dk, dv, block, topk)
+    nbytes = L.yl_block_attention_workspace_bytes(_TYPES[q.dtype], batch, nq, nk, heads, kv, dk, dv, block, topk)
     work = _workspace("block_attention", nbytes, q)
     q, qh = _heads(q)
     k, kh = _heads(k)
