@@ -109,3 +109,24 @@ def test_python_face_refuses_without_a_gpu_tensor():
         ya.block_select(q, q)
     with pytest.raises(RuntimeError, match="GPU only"):
         ya.block_attention(q, q, q, torch.zeros(1, 2, 4, 1, dtype=torch.int32))
+
+
+def test_lowering_takes_blocks_on_long_maps(monkeypatch):
+    """YL_PSA_TOPK: the attention of maps with more blocks than it reads, with its scratch in the arena; nothing else changes."""
+    from yololite_amd import _lib
+    from yololite_amd.nn import arch
+    from yololite_amd.nn.lower import OP_ATTENTION, OP_PSA, lower
+    from yololite_amd.nn.synth import synth_state_dict
+
+    specs, _ = arch.parse_model(arch.yolo11_dict("n"))
+    sd = synth_state_dict("n", 0)
+    before = lower(specs, sd, 8, 640, 640)
+    monkeypatch.setenv("YL_PSA_TOPK", "7")  # a 20x20 map has seven blocks: all of them, so the dense form stays
+    assert [o["kind"] for o in lower(specs, sd, 8, 640, 640).ops] == [o["kind"] for o in before.ops]
+    monkeypatch.setenv("YL_PSA_TOPK", "3")
+    prog = lower(specs, sd, 8, 640, 640)
+    att = [o for o in prog.ops if o["kind"] == OP_ATTENTION]
+    assert [(o["grp"], o["topk"]) for o in att] == [(64, 3)] and not [o for o in prog.ops if o["kind"] == OP_PSA]
+    need = _lib.lib().yl_attention_scratch_bytes(8, 2, 400, 64, 3)
+    assert need > 0 and att[0]["scratch"] % 256 == 0 and att[0]["scratch"] + need <= prog.ws_bytes
+    assert _lib.lib().yl_attention_scratch_bytes(8, 2, 400, 48, 3) == -1 and _lib.lib().yl_attention_scratch_bytes(8, 2, 0, 64, 3) == -1

@@ -304,3 +304,76 @@ def test_together_as_an_attention_stage(gpu_device):
     o = _check_attend(q, k, v, picked, 64, mask)
     y = ya.mx4_linear(o.view(b, n, -1), ya.mx4_quantize(w2), bias=bias, res=x)
     _check_product(y.view(b * n, c), mx4_ref.rounded(_np(o).reshape(b * n, -1)), mx4_ref.rounded(_np(w2)), bias, False, x.view(b * n, c))
+
+
+@pytest.mark.parametrize("b, nh, h, w, block, topk", [(2, 2, 20, 20, 64, 3), (1, 1, 7, 5, 32, 1), (3, 4, 13, 7, 32, 2), (2, 1, 40, 40, 128, 4),
+                                                      (1, 2, 20, 1, 32, 1), (1, 6, 40, 40, 64, 8), (2, 1, 2, 2, 32, 2)])
+def test_engine_op_on_the_networks_maps(gpu_device, b, nh, h, w, block, topk):
+    """YL_OP_ATTENTION with grp != 0 on planar guarded maps: the bits of the direct calls on the same tokens, guards untouched."""
+    from tests.hip_util import Mini
+    from yololite_amd import _lib
+    from yololite_amd.nn.lower import OP_ATTENTION
+
+    g = torch.Generator().manual_seed(h * w)
+    qkv = torch.randn(b, nh * 128, h, w, generator=g).bfloat16()
+    m = Mini(b, gpu_device)
+    xin, out = m.buf(h, w, nh * 128 + 16).slice(16, nh * 128), m.buf(h, w, nh * 64 + 8).slice(8, nh * 64)
+    m.fill(xin, qkv.float())
+    scratch = m.ar.alloc_bytes(_lib.lib().yl_attention_scratch_bytes(b, nh, h * w, block, topk))
+    m.op(kind=OP_ATTENTION, name="attn", heads=nh, key_dim=32, head_dim=64, scale=32 ** -0.5, inp=xin, out=out, grp=block, topk=topk,
+         scratch=scratch)
+    m.run()
+    assert m.eng.op_kernel(0) == "block_attention"
+    got = m.read(out)
+    t = qkv.to(gpu_device).view(b, nh, 128, h * w).permute(0, 3, 1, 2).contiguous()
+    q, k, v = t.split((32, 32, 64), -1)
+    picked = _check_select(q, k, block, topk)
+    want = _check_attend(q, k, v, picked, block, rows=np.arange(0, h * w, 13))
+    assert torch.equal(got, want.permute(0, 2, 3, 1).reshape(b, nh * 64, h, w).float().cpu())
+
+
+def test_engine_op_refusals(gpu_device):
+    from tests.hip_util import Mini
+    from yololite_amd.nn.lower import OP_ATTENTION
+
+    for change in (dict(grp=48), dict(topk=65), dict(scratch=1 << 40), dict(scratch=100), dict(scratch=-1)):
+        m = Mini(1, gpu_device)
+        xin, out = m.buf(20, 20, 128), m.buf(20, 20, 64)
+        m.op(**(dict(kind=OP_ATTENTION, name="attn", heads=1, key_dim=32, head_dim=64, scale=1.0, inp=xin, out=out, grp=64, topk=2,
+                     scratch=m.ar.alloc_bytes(1 << 20)) | change))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            m.run()
+
+
+def test_network_with_selected_blocks(gpu_device, monkeypatch):
+    """YL_PSA_TOPK through the whole network: eager and replayed graphs agree on changing inputs; with the knob unset nothing has
+    changed."""
+    from yololite_amd.nn import arch
+    from yololite_amd.nn.engine import HipEngine
+    from yololite_amd.nn.synth import synth_state_dict
+
+    specs, _ = arch.parse_model(arch.yolo11_dict("n"))
+    sd = synth_state_dict("n", 0)
+    g = torch.Generator().manual_seed(5)
+    xs = [torch.rand(2, 3, 640, 640, generator=g).to(gpu_device) for _ in range(2)]
+
+    def engine():
+        return HipEngine.from_model(specs, sd, 2, 640, 640, gpu_device)
+
+    dense = engine()
+    y_dense = [dense.forward(x).clone() for x in xs]
+    monkeypatch.setenv("YL_PSA_TOPK", "3")
+    eng = engine()
+    want = [eng.forward(x).clone() for x in xs]
+    assert not torch.equal(want[0], y_dense[0]) and bool(torch.isfinite(want[0]).all())
+    buf, y = torch.empty_like(xs[0]), torch.empty_like(want[0])
+    for k in (0, 1, 0, 1):
+        buf.copy_(xs[k])
+        eng.forward(buf, y=y, graph=True)
+        eng.forward(xs[1 - k])  # eager work between the replays
+        buf.copy_(xs[k])
+        eng.forward(buf, y=y, graph=True)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[k])
+    monkeypatch.delenv("YL_PSA_TOPK")
+    assert torch.equal(engine().forward(xs[0]), y_dense[0])

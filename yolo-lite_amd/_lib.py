@@ -115,6 +115,7 @@ EXPORTS = (  # include/yl_amd.h: the product ABI
     "yl_comm_get_unique_id", "yl_comm_create", "yl_comm_destroy", "yl_comm_rank", "yl_comm_world", "yl_comm_scatter",
     "yl_comm_gather", "yl_comm_barrier", "yl_mx4_quantize", "yl_mx4_dequantize", "yl_mx4_linear_workspace_bytes", "yl_mx4_linear",
     "yl_block_select_workspace_bytes", "yl_block_select", "yl_block_attention_workspace_bytes", "yl_block_attention",
+    "yl_attention_scratch_bytes",
 )
 COMM_ID_BYTES = 128  # YL_COMM_ID_BYTES
 DIAG_EXPORTS = (  # include/yl_amd_diag.h: probes for tools/ and the runtime self-checks, not part of the product ABI
@@ -281,6 +282,8 @@ def lib() -> C.CDLL:
     L.yl_block_attention_workspace_bytes.restype = i64
     L.yl_block_attention_workspace_bytes.argtypes = [i32] * 10
     L.yl_block_attention.restype = i32
+    L.yl_attention_scratch_bytes.restype = i64
+    L.yl_attention_scratch_bytes.argtypes = [i32] * 5
     L.yl_block_attention.argtypes = [hp, hp, hp] + [i32] * 10 + [vp, vp, i64, f32, hp, vp, i64, vp]
     if L.yl_abi_version() != 21:
         raise RuntimeError("libyl_amd.so ABI version mismatch; rebuild it")

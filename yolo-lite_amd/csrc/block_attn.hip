@@ -47,14 +47,16 @@ __device__ __forceinline__ unsigned quad_or(unsigned x) {
   return quad_bits(x, [](unsigned a, unsigned b) { return a | b; });
 }
 
-// element (b, t, h, c) of a tensor of heads: p + b * sb + t * st + h * sh + c
+// Element (b, t, h, c) of a tensor of heads: p + b sb + token(t) st + h sh + (c / 8) sc + c % 8.  Dense tensors: sc = 8, token(t) = t.
+// The network's maps (yl_internal.h): a plane per 8 channels, st = 8, sc = a plane, and a guard pixel behind every W tokens.
 struct Heads {
   const void* p;
-  long long sb, st, sh;
+  long long sb, st, sh, sc;
 };
 
 struct BlockArgs {
   Heads q, k, v, o;
+  int W;  // tokens of a row of the map, 0: no rows
   int batch, nq, nk, heads, kv, group;  // group = heads / kv
   int dk, dv, block, nb, topk;
   const uint8_t* mask;  // [batch][nk], row stride mask_stride; nullptr: every key may be read
@@ -69,6 +71,13 @@ struct BlockArgs {
   int* count;     // [batch][nb]: unmasked keys of a block
   int* picked;    // [batch][kv][nq][topk]
 };
+
+__device__ __forceinline__ int token(const BlockArgs& a, int t) { return a.W ? t + t / a.W : t; }
+// channels 0..7 of (b, t, h); chunk c of eight lies c * x.sc further on
+template <typename T>
+__device__ __forceinline__ T* head_ptr(const BlockArgs& a, const Heads& x, int b, int t, int h) {
+  return static_cast<T*>(const_cast<void*>(x.p)) + b * x.sb + token(a, t) * x.st + h * x.sh;
+}
 
 // ------------------------------------------------------------------------------------------------ block means
 // value x as two bf16: x = hi + lo up to 2^-18 |x|
@@ -91,7 +100,7 @@ __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
   const int j = (int)(unit % a.nb), bh = (int)(unit / a.nb), h = bh % a.kv, b = bh / a.kv;
   const int c = lane % CP, kl = lane / CP;
   const int k0 = j * a.block, kn = min(a.block, a.nk - k0);
-  const T* kp = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh + c * 8;
+  const T* kp = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh + c * a.k.sc;
   const uint8_t* mp = a.mask ? a.mask + b * a.mask_stride + k0 : nullptr;
   double acc[8] = {};
   int n = 0;
@@ -103,7 +112,7 @@ __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
       const int i = i0 + u * KL;
       ok[u] = i < kn && (!mp || mp[i]);
       x[u] = t8{};
-      if (ok[u] && c * 8 < a.dk) x[u] = *reinterpret_cast<const t8*>(kp + (long long)(k0 + i) * a.k.st);
+      if (ok[u] && c * 8 < a.dk) x[u] = *reinterpret_cast<const t8*>(kp + token(a, k0 + i) * a.k.st);
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -144,7 +153,7 @@ __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
         for (int e = 0; e < LEFT; ++e) {
           double q = 0;
           for (int g = 0; g < a.group; ++g)
-            q += (double)(float)(static_cast<const T*>(a.q.p) + b * a.q.sb + i * a.q.st + (long long)(h * a.group + g) * a.q.sh)[c * 8 + d0 + e];
+            q += (double)(float)head_ptr<const T>(a, a.q, b, i, h * a.group + g)[c * a.q.sc + d0 + e];
           s += q * mean[e];
         }
 #pragma unroll
@@ -272,7 +281,7 @@ __device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int
   for (int d = lane; d < a.dk; d += 64) {
     double s = 0;
     for (int g = 0; g < a.group; ++g)
-      s += (double)(float)(static_cast<const T*>(a.q.p) + b * a.q.sb + i * a.q.st + (long long)(h * a.group + g) * a.q.sh)[d];
+      s += (double)(float)head_ptr<const T>(a, a.q, b, i, h * a.group + g)[(d >> 3) * a.q.sc + (d & 7)];
     qs[d] = s;
   }
   __builtin_amdgcn_wave_barrier();
@@ -343,13 +352,13 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   for (int t = 0; t < NT; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float qq = 0.f;
   const __bf16* sp = a.split + (long long)bh * a.nbp * (2 * a.dkp);
-  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.sb + (live ? i : 0) * a.q.st + (long long)(h * a.group) * a.q.sh;
+  const T* qp = head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group);
   for (int c0 = 0; c0 < a.dkp; c0 += 32) {
     const int c = c0 + g * 8;
     float q[8] = {};
     if (c < a.dk) {
       for (int e = 0; e < a.group; ++e) {
-        const t8 x = *reinterpret_cast<const t8*>(qp + e * a.q.sh + c);
+        const t8 x = *reinterpret_cast<const t8*>(qp + e * a.q.sh + (c >> 3) * a.q.sc);
 #pragma unroll
         for (int d = 0; d < 8; ++d) q[d] += (float)x[d];
       }
@@ -508,7 +517,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
     for (int x = 0; x < 2; ++x)
       if (lane + 64 * x < a.dk)
         for (int e = 0; e < a.group; ++e)
-          qd[x] += (double)(float)(static_cast<const T*>(a.q.p) + b * a.q.sb + qi * a.q.st + (long long)(h * a.group + e) * a.q.sh)[lane + 64 * x];
+          qd[x] += (double)(float)head_ptr<const T>(a, a.q, b, qi, h * a.group + e)[(lane >> 3) * a.q.sc + x * 8 * a.q.sc + (lane & 7)];
     const int nmay = __builtin_amdgcn_readlane(may, k), need = __builtin_amdgcn_readlane(take - at, k);
     double mine = 0;
     int mj = 0, c = 0;
@@ -694,7 +703,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       if (p.slots == 1) {  // (nothing is joined: the result itself is zeros)
         const int b0 = bh / a.kv, h0 = bh % a.kv;
         for (int e = lane; e < a.group * a.dv; e += 64)
-          (static_cast<T*>(const_cast<void*>(a.o.p)) + b0 * a.o.sb + qdirect * a.o.st + (long long)(h0 * a.group + e / a.dv) * a.o.sh)[e % a.dv] = (T)0.f;
+          head_ptr<T>(a, a.o, b0, qdirect, h0 * a.group + e / a.dv)[e % a.dv / 8 * a.o.sc + (e & 7)] = (T)0.f;
       }
       return;
     }
@@ -757,7 +766,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     for (int u = 0; u < 8; ++u) {
       v[x][u] = t8{};
       if (it < KEYS / 8 * (DVP / 8) && c8 * 8 < a.dv && (ok >> (kg * 8 + u) & 1))
-        v[x][u] = *reinterpret_cast<const t8*>(vb + (long long)(k0 + kg * 8 + u) * a.v.st + c8 * 8);
+        v[x][u] = *reinterpret_cast<const t8*>(vb + token(a, k0 + kg * 8 + u) * a.v.st + c8 * a.v.sc);
     }
     if (HALF && !alone)
 #pragma unroll
@@ -797,7 +806,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
 #pragma unroll
     for (int c = 0; c < DK32; ++c) {
       kf[t][c] = t8{};
-      if (t * 16 + n < kn && (c * 4 + g) * 8 < a.dk) kf[t][c] = *reinterpret_cast<const t8*>(kb + (long long)(k0 + t * 16 + n) * a.k.st + (c * 4 + g) * 8);
+      if (t * 16 + n < kn && (c * 4 + g) * 8 < a.dk) kf[t][c] = *reinterpret_cast<const t8*>(kb + token(a, k0 + t * 16 + n) * a.k.st + (c * 4 + g) * a.k.sc);
     }
   unsigned okt = 0;  // this lane's keys t * 16 + 4 g + r, four bits per tile
 #pragma unroll
@@ -817,7 +826,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   // scores are scaled by |scale| inside the exponential's fma; a negative scale flips the queries' signs
   const float scale = fabsf(a.scale) * 1.44269504088896340736f;
   const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
-  const bool all = ok == (KEYS == 64 ? ~0ull : (1ull << KEYS) - 1);  // no key is masked: uniform
+  const bool all = ok == ~0ull >> (64 - KEYS);  // no key is masked: uniform
   t8 one;
 #pragma unroll
   for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
@@ -830,7 +839,8 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     t8 f[DK32];
   };
   const int q0 = DIRECT ? qdirect : grp0 * 64;
-  const T* const qb = static_cast<const T*>(a.q.p) + b * a.q.sb + (long long)q0 * a.q.st + (long long)(h * a.group) * a.q.sh;
+  const T* const qb = head_ptr<const T>(a, a.q, b, q0, h * a.group);
+  const int qtok = token(a, q0);
   part_t* const pb = static_cast<part_t*>(p.part) + ((long long)bh * p.cq + (q0 - p.g0 * 64)) * a.group * p.slots * DVP;
   float2* const mlb = p.ml + (long long)bh * p.slots * p.mlrow + (long long)q0 * a.group;
   auto fetch = [&](int tile, Row& w) __attribute__((always_inline)) {
@@ -852,14 +862,16 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       w.slot = __mul24((int)(x & 63), p.subs) + sub;
     }
     const T* qp;
-    if (p.q32)
+    if (a.W)
+      qp = qb + (token(a, q0 + w.q) - qtok) * a.q.st + w.head * a.q.sh;
+    else if (p.q32)
       qp = qb + (unsigned)(__umul24((unsigned)w.q, (unsigned)a.q.st) + __umul24((unsigned)w.head, (unsigned)a.q.sh));
     else
       qp = qb + w.q * a.q.st + w.head * a.q.sh;
 #pragma unroll
     for (int c = 0; c < DK32; ++c) {
       w.f[c] = t8{};
-      if ((c * 4 + g) * 8 < a.dk) w.f[c] = *reinterpret_cast<const t8*>(qp + (c * 4 + g) * 8);
+      if ((c * 4 + g) * 8 < a.dk) w.f[c] = *reinterpret_cast<const t8*>(qp + (c * 4 + g) * a.q.sc);
     }
   };
   const int ntiles = (nrows + 15) >> 4;
@@ -934,13 +946,13 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     if (!w.live) continue;
     const unsigned local = __umul24((unsigned)w.q, (unsigned)a.group) + (unsigned)w.head;  // row behind q0's first: below 4096 * 1000
     if (alone) {
-      T* const dst = static_cast<T*>(const_cast<void*>(a.o.p)) + b * a.o.sb + (long long)(q0 + w.q) * a.o.st + (long long)(h * a.group + w.head) * a.o.sh;
+      T* const dst = head_ptr<T>(a, a.o, b, q0 + w.q, h * a.group + w.head);
       const float inv = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);
 #pragma unroll
       for (int d = 0; d < DV16; ++d) {
         const int c = channel(d, 4 * g);
         const u32x2 y = {Vec<T>::pack(o[d][0] * inv, o[d][1] * inv), Vec<T>::pack(o[d][2] * inv, o[d][3] * inv)};
-        if (c < a.dv) *reinterpret_cast<u32x2*>(dst + c) = y;
+        if (c < a.dv) *reinterpret_cast<u32x2*>(dst + (c >> 3) * a.o.sc + (c & 7)) = y;
       }
       continue;
     }
@@ -1019,8 +1031,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   t8 y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv);
-  *reinterpret_cast<t8*>(static_cast<T*>(const_cast<void*>(a.o.p)) + bh / a.kv * a.o.sb + i * a.o.st +
-                         (long long)(bh % a.kv * a.group + gh) * a.o.sh + c) = y;
+  *reinterpret_cast<t8*>(head_ptr<T>(a, a.o, bh / a.kv, i, bh % a.kv * a.group + gh) + (c >> 3) * a.o.sc) = y;
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -1053,8 +1064,8 @@ static int fill_args(const std::string& who, const yl_heads* q, const yl_heads* 
   if (nk > 0)
     if (int rc = check_heads(who, "k", k)) return rc;
   if (mask && batch > 1 && mask_stride < nk) return fail(-1, who + ": the mask's row stride is smaller than a row");
-  a->q = Heads{q->data, q->batch, q->token, q->head};
-  if (nk > 0) a->k = Heads{k->data, k->batch, k->token, k->head};
+  a->q = Heads{q->data, q->batch, q->token, q->head, 8};
+  if (nk > 0) a->k = Heads{k->data, k->batch, k->token, k->head, 8};
   a->batch = batch, a->nq = nq, a->nk = nk, a->heads = heads, a->kv = kv_heads, a->group = heads / kv_heads;
   a->magic = (unsigned)((1ULL << 32) / a->group + 1);
   a->dk = dk, a->block = block, a->nb = (int)nb, a->topk = topk, a->mask = mask, a->mask_stride = mask_stride;
@@ -1129,19 +1140,9 @@ static int score_launch(const BlockArgs& a, hipStream_t s) {
   return 0;
 }
 
-extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, int batch, int nq, int nk, int heads, int kv_heads,
-                               int dk, int block, int topk, const uint8_t* mask, int64_t mask_stride, int32_t* picked, void* work,
-                               int64_t work_bytes, void* stream) {
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  BlockArgs a{};
-  if (int rc = fill_args("block_select", q, k, dtype, batch, nq, nk, heads, kv_heads, dk, block, topk, mask, mask_stride, &a)) return rc;
-  if (batch * (long long)nq == 0) return 0;
-  if (!picked) return fail(-1, "block_select: null pointer");
-  const SelectPlan p = plan_select(&a);
-  if (p.all > 0 && (!work || work_bytes < p.all || (reinterpret_cast<uintptr_t>(work) & 15)))
-    return fail(-1, "block_select: workspace missing, too small or not 16-byte aligned");
-  char* const w = static_cast<char*>(work);
-  a.picked = picked;
+// the selection of `a` (sizes and tensors filled in) into a.picked, with plan `p` and its workspace
+static int select_run(BlockArgs& a, const SelectPlan& p, int dtype, char* w, hipStream_t s) {
+  const int batch = a.batch, nq = a.nq, kv_heads = a.kv;
   a.mean = reinterpret_cast<double*>(w + p.mean), a.score = reinterpret_cast<double*>(w + p.score);
   a.split = reinterpret_cast<__bf16*>(w + p.split), a.norm = reinterpret_cast<float*>(w + p.norm);
   a.count = reinterpret_cast<int*>(w + p.count);
@@ -1167,6 +1168,21 @@ extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, 
     YL_HIP(hipGetLastError());
     return 0;
   });
+}
+
+extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, int batch, int nq, int nk, int heads, int kv_heads,
+                               int dk, int block, int topk, const uint8_t* mask, int64_t mask_stride, int32_t* picked, void* work,
+                               int64_t work_bytes, void* stream) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  BlockArgs a{};
+  if (int rc = fill_args("block_select", q, k, dtype, batch, nq, nk, heads, kv_heads, dk, block, topk, mask, mask_stride, &a)) return rc;
+  if (batch * (long long)nq == 0) return 0;
+  if (!picked) return fail(-1, "block_select: null pointer");
+  const SelectPlan p = plan_select(&a);
+  if (p.all > 0 && (!work || work_bytes < p.all || (reinterpret_cast<uintptr_t>(work) & 15)))
+    return fail(-1, "block_select: workspace missing, too small or not 16-byte aligned");
+  a.picked = picked;
+  return select_run(a, p, dtype, static_cast<char*>(work), s);
 }
 
 // ---- how the attention runs: sizes, and where things lie in the workspace
@@ -1246,27 +1262,10 @@ extern "C" int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int 
   return batch * (long long)nq == 0 ? 0 : plan_attend(a, dv, dtype).all;
 }
 
-extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl_heads* v, int dtype, int batch, int nq, int nk,
-                                  int heads, int kv_heads, int dk, int dv, int block, int topk, const int32_t* picked,
-                                  const uint8_t* mask, int64_t mask_stride, float scale, const yl_heads* out, void* work,
-                                  int64_t work_bytes, void* stream) {
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  AttendArgs p{};
+// the attention of `p.a` (sizes, tensors, picked and scale filled in), with plan `pl` and its workspace
+static int attend_run(AttendArgs& p, const AttendPlan& pl, int dtype, char* w, hipStream_t s) {
   BlockArgs& a = p.a;
-  if (int rc = fill_args("block_attention", q, k, dtype, batch, nq, nk, heads, kv_heads, dk, block, topk, mask, mask_stride, &a)) return rc;
-  if (dv < 8 || dv > 128 || dv % 8) return fail(-3, "block_attention: value widths are multiples of 8 up to 128");
-  if (batch * (long long)nq == 0) return 0;
-  if (nk > 0)
-    if (int rc = check_heads("block_attention", "v", v)) return rc;
-  if (int rc = check_heads("block_attention", "out", out)) return rc;
-  if (!picked) return fail(-1, "block_attention: null pointer");
-  const AttendPlan pl = plan_attend(a, dv, dtype);
-  if (!work || work_bytes < pl.all || (reinterpret_cast<uintptr_t>(work) & 15))
-    return fail(-1, "block_attention: workspace missing, too small or not 16-byte aligned");
-  if (nk > 0) a.v = Heads{v->data, v->batch, v->token, v->head};
-  a.o = Heads{out->data, out->batch, out->token, out->head};
-  a.dv = dv, a.scale = scale, a.picked = const_cast<int32_t*>(picked);
-  char* const w = static_cast<char*>(work);
+  const int batch = a.batch, nq = a.nq, heads = a.heads, kv_heads = a.kv, block = a.block;
   p.subs = pl.subs, p.slots = pl.slots, p.groups = pl.groups, p.range = pl.range;
   p.gn = pl.groups, p.cq = pl.direct ? nq : 64 * pl.chunk;
   p.mlrow = (long long)nq * a.group;
@@ -1294,4 +1293,66 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
     }
     return 0;
   });
+}
+
+extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl_heads* v, int dtype, int batch, int nq, int nk,
+                                  int heads, int kv_heads, int dk, int dv, int block, int topk, const int32_t* picked,
+                                  const uint8_t* mask, int64_t mask_stride, float scale, const yl_heads* out, void* work,
+                                  int64_t work_bytes, void* stream) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  AttendArgs p{};
+  BlockArgs& a = p.a;
+  if (int rc = fill_args("block_attention", q, k, dtype, batch, nq, nk, heads, kv_heads, dk, block, topk, mask, mask_stride, &a)) return rc;
+  if (dv < 8 || dv > 128 || dv % 8) return fail(-3, "block_attention: value widths are multiples of 8 up to 128");
+  if (batch * (long long)nq == 0) return 0;
+  if (nk > 0)
+    if (int rc = check_heads("block_attention", "v", v)) return rc;
+  if (int rc = check_heads("block_attention", "out", out)) return rc;
+  if (!picked) return fail(-1, "block_attention: null pointer");
+  const AttendPlan pl = plan_attend(a, dv, dtype);
+  if (!work || work_bytes < pl.all || (reinterpret_cast<uintptr_t>(work) & 15))
+    return fail(-1, "block_attention: workspace missing, too small or not 16-byte aligned");
+  if (nk > 0) a.v = Heads{v->data, v->batch, v->token, v->head, 8};
+  a.o = Heads{out->data, out->batch, out->token, out->head, 8};
+  a.dv = dv, a.scale = scale, a.picked = const_cast<int32_t*>(picked);
+  return attend_run(p, pl, dtype, static_cast<char*>(work), s);
+}
+
+// ---- YL_OP_ATTENTION on the network's maps: q (32) | k (32) | v (64) channels of every head, all tokens of an image
+static BlockArgs map_args(int batch, int heads, int n, int block, int topk) {
+  BlockArgs a{};
+  a.batch = batch, a.nq = a.nk = n, a.heads = a.kv = heads, a.group = 1, a.magic = 1;
+  a.dk = 32, a.dv = 64, a.block = block, a.nb = (n + block - 1) / block, a.topk = topk;
+  return a;
+}
+namespace yl {
+long long block_attention_map_bytes(int batch, int heads, int n, int block, int topk) {
+  BlockArgs a = map_args(batch, heads, n, block, topk);
+  return round256(4LL * batch * heads * n * topk) + std::max(plan_select(&a).all, plan_attend(a, a.dv, YL_BF16).all);
+}
+int block_attention_map_launch(const AttnArgs& t, int block, int topk, char* work, hipStream_t s) {
+  AttendArgs p{};
+  BlockArgs& a = p.a;
+  a = map_args(t.batch, t.heads, t.N, block, topk);
+  a.W = t.W;
+  auto heads = [&](const PView& v, int plane, int per_head) {
+    return Heads{v.base + plane * v.plane + v.g0 * 8LL, v.img * 8LL, 8, per_head * v.plane, v.plane};
+  };
+  a.q = heads(t.in, 0, 16), a.k = heads(t.in, 4, 16), a.v = heads(t.in, 8, 16), a.o = heads(t.out, 0, 8);
+  a.scale = t.scale;
+  a.picked = reinterpret_cast<int*>(work);
+  char* const w = work + round256(4LL * a.batch * a.kv * a.nq * a.topk);
+  const SelectPlan sp = plan_select(&a);
+  if (int rc = select_run(a, sp, YL_BF16, w, s)) return rc;
+  return attend_run(p, plan_attend(a, a.dv, YL_BF16), YL_BF16, w, s);
+}
+}  // namespace yl
+
+extern "C" int64_t yl_attention_scratch_bytes(int batch, int heads, int tokens, int block, int topk) {
+  if (batch < 1 || heads < 1 || tokens < 1 || (block != 32 && block != 64 && block != 128) || topk < 1 || topk > BA_MAX_TOPK ||
+      ((long long)tokens + block - 1) / block > BA_MAX_BLOCKS || (long long)batch * heads * tokens > 0x7FFFFFFFLL) {
+    fail(-3, "attention: blocks of 32, 64 or 128 tokens, at most 4096 of them, 1 to 64 for a token");
+    return -1;
+  }
+  return yl::block_attention_map_bytes(batch, heads, tokens, block, topk);
 }

@@ -895,6 +895,19 @@ extern "C" int yl_engine_create(const yl_op* ops, int n_ops, int batch, int in_h
         if (o.key_dim != 32 || o.head_dim != 64)
           return fail(-3, tag + ": attention supports key_dim 32 / head_dim 64 (every YOLO11 scale)");
         if (o.in.C != o.heads * 128 || o.out.C != o.heads * 64) return fail(-1, tag + ": attention channel mismatch");
+        if (o.grp != 0) {  // over the blocks a score selects (yl_amd.h)
+          const int n = o.in.H * o.in.W;
+          if ((o.grp != 32 && o.grp != 64 && o.grp != 128) || o.reserved2 < 1 || o.reserved2 > 64 || (n + o.grp - 1) / o.grp > 4096)
+            return fail(-3, tag + ": blocks of 32, 64 or 128 tokens (grp), at most 4096 of them, 1 to 64 for a token (reserved2)");
+          const long long need = block_attention_map_bytes(batch, o.heads, n, o.grp, o.reserved2);
+          if (o.out8.offset < 0 || o.out8.offset % 256 || o.out8.offset + need > workspace_bytes)
+            return fail(-1, tag + ": no room for " + std::to_string(need) + " bytes of scratch at out8.offset");
+          const double keys = std::min<double>(n, (double)o.reserved2 * o.grp), nb = (n + o.grp - 1) / o.grp;
+          r.flops = 2.0 * batch * o.heads * (double)n * (nb * 32 + keys * (32 + 64));
+          r.bytes = px_in * o.in.C * 2 + px_out * o.out.C * 2;
+          r.name = "block_attention";
+          break;
+        }
         r.flops = 2.0 * batch * o.heads * (double)(o.in.H * o.in.W) * (o.in.H * o.in.W) * (32 + 64);
         r.bytes = px_in * o.in.C * 2 + px_out * o.out.C * 2;
         r.name = "attention";
@@ -1503,6 +1516,7 @@ static int run_op(const yl_engine* e, const OpRec& r, char* ws, hipStream_t s, c
       a.heads = o.heads;
       a.batch = B;
       a.scale = o.scale;
+      if (o.grp != 0) return block_attention_map_launch(a, o.grp, o.reserved2, ws + o.out8.offset, s);
       return attention_launch(a, s);
     }
   }

@@ -266,6 +266,9 @@ struct AttnArgs {
   float scale;
 };
 int attention_launch(const AttnArgs& a, hipStream_t s);
+// the same over `topk` blocks of `block` tokens that a mean-key score selects for every token (block_attn.hip); scratch of _bytes
+long long block_attention_map_bytes(int batch, int heads, int n, int block, int topk);
+int block_attention_map_launch(const AttnArgs& a, int block, int topk, char* work, hipStream_t s);
 
 struct StemArgs {
   const void* in;     // NCHW [B][3][H][W]

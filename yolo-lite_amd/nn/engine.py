@@ -59,6 +59,8 @@ class HipEngine:
             c.in_scale, c.out_scale, c.res_scale = (float(o.get(k, 0.0)) for k in ("in_scale", "out_scale", "res_scale"))
             c.out8, c.out8_c0 = _cview(o.get("out8")), int(o.get("out8_c0", 0))
             c.out8_scale, c.out8_only = float(o.get("out8_scale", 0.0)), int(o.get("out8_only", 0))
+            if o.get("topk"):  # YL_OP_ATTENTION over selected blocks of o["grp"] tokens: its scratch is raw bytes
+                c.reserved2, c.out8.offset = int(o["topk"]), int(o["scratch"])
             if "weight" in o:
                 w = np.ascontiguousarray(o["weight"], dtype=np.float32)
                 b = np.ascontiguousarray(o["bias"], dtype=np.float32)

@@ -18,6 +18,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from .. import _lib
 from .arch import LayerSpec, detect_mid_channels
 
 BN_EPS = 1e-3
@@ -1001,13 +1002,17 @@ def lower(specs: Sequence[LayerSpec], sd: Dict[str, torch.Tensor], batch: int, i
                 conv(p + ".cv1", src, u, 1, 1)
             b = u.slice(c, c)
             psa_tail_done = False
+            # YL_PSA_TOPK=n: attention over the n blocks of 64 tokens that a mean-key score selects for each token, where the map has
+            # more (csrc/block_attn.hip); not the trained network's function any more, opt-in
+            topk = int(os.environ.get("YL_PSA_TOPK", "0"))
+            sparse = 0 < topk and src.H * src.W > 64 * topk
             for j in range(sp.n):
                 q = f"{p}.m.{j}"
                 # the whole PSABlock in ONE launch, one workgroup per image (csrc/resident.hip psa_resident_kernel: 6 launches ->
                 # 1, bit-identical); small batches keep the six launches, like the resident C3k block
                 # (the one-batch profile keeps the six launches: 69.8 us in sequence against 71 us; with FOUR workgroups per image --
                 # YL_LAT_PSA=1 -- the one-launch form measures the same there, 34.4 against 34.5 k one batch at a time)
-                if (fuse_post and os.environ.get("YL_FUSE_PSA", "1") != "0" and not (one_batch and os.environ.get("YL_LAT_PSA", "0") != "1")
+                if (fuse_post and not sparse and os.environ.get("YL_FUSE_PSA", "1") != "0" and not (one_batch and os.environ.get("YL_LAT_PSA", "0") != "1")
                         and psa_resident_fits(c, nh, kd, hd, src.H, src.W)
                         and batch >= int(os.environ.get("YL_FUSE_C3K_MIN_BATCH", "8")) and not fp8_scales):
                     wq, bq = fold_conv_bn(sd, q + ".attn.qkv")
@@ -1030,6 +1035,11 @@ def lower(specs: Sequence[LayerSpec], sd: Dict[str, torch.Tensor], batch: int, i
                 o = ar.alloc(src.H, src.W, c)
                 ops.append(dict(kind=OP_ATTENTION, name=q + ".attn", heads=nh, key_dim=kd, head_dim=hd,
                                 scale=float(kd ** -0.5), inp=qkv, out=o, res=None))
+                if sparse:
+                    nbytes = _lib.lib().yl_attention_scratch_bytes(batch, nh, src.H * src.W, 64, topk)
+                    if nbytes < 0:
+                        _lib.check(-3, "YL_PSA_TOPK")
+                    ops[-1].update(grp=64, topk=topk, scratch=ar.alloc_bytes(nbytes))
                 dwconv(q + ".attn.pe", qkv, o, act=False, accumulate=True, grp=hd, grp_stride=2 * kd + hd,
                        grp_off=2 * kd)
                 # everything behind the attention is pointwise: proj, ffn.0, ffn.1 and C2PSA.cv2 in ONE launch over the pixels
