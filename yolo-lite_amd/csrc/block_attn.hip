@@ -413,25 +413,24 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   const float err = (3.f / 262144.f + 4.f * a.dk / 16777216.f) * qn * big + (qn + big) * 2e-36f + 1e-30f;
 
   // ---- the cut.  Blocks that cannot be selected (and places behind the last) go under every cut
-  float lo = __builtin_huge_valf(), hi = ninf;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
+    if ((okw[t >> 1] >> ((t & 1) * 16) & 0xFFFFu) == 0xFFFFu) continue;  // (the same in every lane)
     const unsigned m = okw[t >> 1] >> ((t & 1) * 16 + 4 * g);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool ok = m >> r & 1;
-      lo = ok ? fminf(lo, s[t][r]) : lo;
-      s[t][r] = ok ? s[t][r] : ninf;
-      hi = fmaxf(hi, s[t][r]);
-    }
+    for (int r = 0; r < 4; ++r) s[t][r] = m >> r & 1 ? s[t][r] : ninf;
   }
-  lo = quad_min(lo);
+  float hi = ninf;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) hi = __builtin_amdgcn_fmed3f(hi, s[t][r], __builtin_huge_valf());
   hi = quad_max(hi);
-  // more than `take` scores over lo, fewer over hi.  (Half way: about 11 steps until all 16 queries are done; a straight line between
+  float lo = -1.01f * qn * big - 1e-30f;  // under every score
+  // more than `take` scores over lo, fewer over hi.  (Half way: about 12 steps until all 16 queries are done; a straight line between
   // the two counts took 14-16, the counts fall too steeply towards the cut.)
   float cut = ninf;
   bool found = take == can;  // (everything that can be selected is: the cut stays at -inf)
-  lo -= (hi - lo) * 0.01f + 1e-30f;
   for (int it = 0; it < 32 && __ballot(!found && live); ++it) {
     const float mid = 0.5f * (lo + hi);
     int c = 0;
@@ -444,19 +443,30 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
     lo = c > take && !found ? mid : lo;
     hi = c < take && !found ? mid : hi;
   }
-  // how far apart the two sides of the cut are
-  float in = __builtin_huge_valf(), out = ninf;
+  // Sure where no score lies within err of the cut: the two sides are more than 2 err apart.  (Not so where anything is NaN.)  Only
+  // where that fails for some query are the two sides themselves looked for.
+  float near = __builtin_huge_valf();
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool over = s[t][r] > cut;
-      in = over ? fminf(in, s[t][r]) : in;
-      out = over ? out : fmaxf(out, s[t][r]);
-    }
-  in = quad_min(in);
-  out = quad_max(out);
-  const bool sure = take == can || (found && qn * big < 1e37f && in - out > 2.f * err);  // (not so where anything is NaN)
+    for (int r = 0; r < 4; ++r) near = fminf(near, fabsf(s[t][r] - cut));
+  near = quad_min(near);
+  const bool fine = qn * big < 1e37f;
+  bool sure = take == can || (found && fine && near > err);
+  float in = __builtin_huge_valf(), out = ninf;
+  if (__ballot(!sure && live)) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool over = s[t][r] > cut;
+        in = over ? fminf(in, s[t][r]) : in;
+        out = over ? out : fmaxf(out, s[t][r]);
+      }
+    in = quad_min(in);
+    out = quad_max(out);
+    sure = sure || (found && fine && in - out > 2.f * err);
+  }
   const float up = (found ? out : hi) + 2.f * err, dn = (found ? in : lo) - 2.f * err;   // the band around a cut that is not sure
   const float floor_ = sure ? cut : up;
 
@@ -502,7 +512,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
     mayw[w] = quad_or(bits << (4 * g)) & okw[w];
     may += __popc(mayw[w]);
   }
-  const bool few = qn * big < 1e37f && may <= 16 && at <= take && at + may >= take;
+  const bool few = fine && may <= 16 && at <= take && at + may >= take;
   while (todo) {
     const int k = __ffsll(todo) - 1;
     todo &= todo - 1;
@@ -671,7 +681,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   typedef typename Vec<T>::t8 t8;
   typedef typename Vec<T>::t4 t4;
   constexpr int NT = DIRECT ? 64 : 256;
-  typedef typename Vec<T>::part part_t;
+  typedef std::conditional_t<DIRECT, float, typename Vec<T>::part> part_t;  // (few rows: nothing to save)
   constexpr bool HALF = sizeof(part_t) == 2;
   constexpr int KT = KEYS / 16, KS = KEYS / 32, DVP = DV16 * 16, VP = KEYS + 8;
   __shared__ __attribute__((aligned(16))) T sVt[DVP * VP];
@@ -972,7 +982,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
 }
 
 // out = the slots' results weighted by their sums; one thread per (row, 8 channels)
-template <typename T, int DVP>
+template <typename T, typename P, int DVP>
 __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   typedef typename Vec<T>::t8 t8;
   const BlockArgs& a = p.a;
@@ -985,11 +995,10 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   const int gh = (int)(prow % a.group);
   const int i = p.g0 * 64 + (int)(prow / a.group % cq), bh = (int)(prow / a.group / cq);
   const float2* ml = p.ml + (long long)bh * p.slots * p.mlrow + (long long)i * a.group + gh;
-  typedef typename Vec<T>::part part_t;
-  typedef part_t p8 __attribute__((ext_vector_type(8)));
-  constexpr bool HALF = sizeof(part_t) == 2;
+  typedef P p8 __attribute__((ext_vector_type(8)));
+  constexpr bool HALF = sizeof(P) == 2;
   const int* pick = a.picked + ((long long)bh * a.nq + i) * a.topk;
-  const part_t* part = static_cast<const part_t*>(p.part) + (((long long)bh * p.cq + i - p.g0 * 64) * a.group + gh) * p.slots * DVP + c;
+  const P* part = static_cast<const P*>(p.part) + (((long long)bh * p.cq + i - p.g0 * 64) * a.group + gh) * p.slots * DVP + c;
   constexpr int U = 8;  // slots whose loads are in flight together
   float m = -__builtin_huge_valf();
   for (int t0 = 0; t0 < p.slots; t0 += U) {
@@ -1195,7 +1204,7 @@ struct AttendPlan {
 
 constexpr long long CHUNK_BYTES = 256LL << 20;  // block results in memory at once (measured: 128 MB and more the same time, 64 MB 15 % more, 16 MB twice)
 static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
-  const int part_bytes = dtype == YL_BF16 ? 2 : 4;
+
   AttendPlan p{};
   p.subs = a.block == 128 ? 2 : 1;
   p.slots = a.topk * p.subs;
@@ -1207,6 +1216,7 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
   const long long per64 = 64LL * a.topk * a.group;
   p.range = (int)std::min<long long>(64, std::max<long long>(1, 512LL * std::max(1, a.nb) / per64));
   const long long rows = (long long)a.batch * a.nq * a.heads, bg = (long long)a.batch * a.kv * p.groups;
+  const int part_bytes = dtype == YL_BF16 && !p.direct ? 2 : 4;
   p.chunk = p.groups;
   if (!p.direct) {
     const long long group_bytes = (long long)part_bytes * a.batch * a.heads * 64 * p.slots * p.dvp;
@@ -1285,10 +1295,12 @@ static int attend_run(AttendArgs& p, const AttendPlan& pl, int dtype, char* w, h
         if (int rc = block == 32 ? attend_by_width<T, 32>(p, pl.direct, s) : attend_by_width<T, 64>(p, pl.direct, s)) return rc;
       if (pl.slots == 1 && pl.direct) return 0;
       const long long items = (long long)batch * std::min(64 * p.gn, nq - 64 * g0) * heads * (pl.dvp / 8);
-      if (pl.dvp == 64)
-        hipLaunchKernelGGL((block_join_kernel<T, 64>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
-      else
-        hipLaunchKernelGGL((block_join_kernel<T, 128>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p);
+      const dim3 grid((unsigned)((items + 255) / 256));
+      typedef typename Vec<T>::part P;
+      if (pl.direct && pl.dvp == 64) hipLaunchKernelGGL((block_join_kernel<T, float, 64>), grid, dim3(256), 0, s, p);
+      else if (pl.direct) hipLaunchKernelGGL((block_join_kernel<T, float, 128>), grid, dim3(256), 0, s, p);
+      else if (pl.dvp == 64) hipLaunchKernelGGL((block_join_kernel<T, P, 64>), grid, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((block_join_kernel<T, P, 128>), grid, dim3(256), 0, s, p);
       YL_HIP(hipGetLastError());
     }
     return 0;
