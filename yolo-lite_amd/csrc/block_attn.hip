@@ -64,7 +64,7 @@ struct BlockArgs {
   float scale;
   double* mean;   // [batch][kv][nb][dk]
   double* score;  // few queries: [batch][kv][nq][nb]
-  __bf16* split;  // [batch][kv][nbp][2][dkp]: the means as two bf16; nbp = nb rounded up to 16, dkp = dk to 32
+  __bf16* split;  // the means as two bf16, in the order the matrix pipe takes them (split_at); nbp = nb rounded up to 16, dkp = dk to 32
   float* norm;    // [batch][kv][nb]: 2-norm of a mean
   int nbp, dkp;
   unsigned magic; // 2^32 / group, rounded up: f / group = mulhi(f, magic) for f * group < 2^32
@@ -86,6 +86,13 @@ __device__ __forceinline__ void split2(float x, __bf16* hi, __bf16* lo) {
   *lo = (__bf16)(x - (float)*hi);
 }
 __device__ __forceinline__ double shfl_xor_d(double x, int o) { return __shfl_xor(x, o); }
+
+// Where the upper half of dim d of block j's mean lies among [batch][kv][nbp / 16][dkp / 32][2][64 lanes][8]: lane (block j % 16, dims
+// 8 g .. of 32) of an MFMA operand; the lower half 512 further.  A wave's fragment is then 1 KiB in a row (row by row, 64 bytes of each
+// row, the fragment reads took 18 of 34 us of a selection on 80x80 maps).
+__device__ __forceinline__ long long split_at(const BlockArgs& a, int bh, int j, int d) {
+  return (((long long)bh * (a.nbp >> 4) + (j >> 4)) * (a.dkp >> 5) + (d >> 5)) * 1024 + (((d >> 3) & 3) * 16 + (j & 15)) * 8 + (d & 7);
+}
 
 // One wave per (image, kv head, block): lane = (key lane, 8 dims), 64 / CP key lanes (CP: dk / 8 rounded up to a power of two); the
 // lanes of a dim chunk exchange halves, then quarters, ... of their sums, so a wave reduces with 7 exchanges instead of 24.
@@ -171,16 +178,16 @@ __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
         const float f = (float)mean[e];
         __bf16 hi, lo;
         split2(f, &hi, &lo);
-        __bf16* at = a.split + ((long long)bh * a.nbp + j) * (2 * a.dkp) + d;
+        __bf16* at = a.split + split_at(a, bh, j, d);
         at[0] = hi;
-        at[a.dkp] = lo;
+        at[512] = lo;
         norm += f * f;
       }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) norm += __shfl_xor(norm, o);
     if (lane < a.dkp - a.dk) {  // the dims behind the last: zeros
-      __bf16* at = a.split + ((long long)bh * a.nbp + j) * (2 * a.dkp) + a.dk + lane;
-      at[0] = at[a.dkp] = (__bf16)0.f;
+      __bf16* at = a.split + split_at(a, bh, j, a.dk + lane);
+      at[0] = at[512] = (__bf16)0.f;
     }
     if (lane == 0) {
       a.norm[(long long)bh * a.nb + j] = sqrtf(norm);
@@ -338,29 +345,44 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   __shared__ double qs[4][128];
   constexpr int NWORD = (NT + 1) / 2;  // 32 blocks to a word
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
-  const long long unit = (long long)xcd_remap((int)blockIdx.x, (int)gridDim.x) * 4 + wave;
-  if (unit >= (long long)a.batch * a.kv * qtiles) return;  // (no barrier below: waves are on their own)
-  const int qt = (int)(unit % qtiles), bh = (int)(unit / qtiles), h = bh % a.kv, b = bh / a.kv;
+  const unsigned unit = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x) * 4u + (unsigned)wave;  // (below 2^31: the rows are)
+  if (unit >= (unsigned)(a.batch * a.kv) * (unsigned)qtiles) return;  // (no barrier below: waves are on their own)
+  const int bh = (int)(unit / (unsigned)qtiles), qt = (int)(unit - (unsigned)bh * (unsigned)qtiles), h = bh % a.kv, b = bh / a.kv;
   const int i = qt * 16 + n;
   const bool live = i < a.nq;
   const float ninf = -__builtin_huge_valf();
   typedef T t8 __attribute__((ext_vector_type(8)));
 
+  // how many keys each block has to read, |c| -- asked for ahead of everything else
+  int cnt[(NWORD + 1) / 2];
+  float norm[(NWORD + 1) / 2];
+#pragma unroll
+  for (int w = 0; w < (NWORD + 1) / 2; ++w) {
+    const int j = min(w * 64 + lane, a.nb - 1);
+    cnt[w] = a.count[b * a.nb + j];
+    norm[w] = a.norm[(long long)bh * a.nb + j];
+    if (w * 64 + lane >= a.nb) cnt[w] = 0, norm[w] = 0.f;
+  }
   // ---- scores
   f32x4 s[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float qq = 0.f;
-  const __bf16* sp = a.split + (long long)bh * a.nbp * (2 * a.dkp);
+  const __bf16* sp = a.split + split_at(a, bh, 0, 0) + lane * 8;
   const T* qp = head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group);
   for (int c0 = 0; c0 < a.dkp; c0 += 32) {
     const int c = c0 + g * 8;
     float q[8] = {};
     if (c < a.dk) {
-      for (int e = 0; e < a.group; ++e) {
-        const t8 x = *reinterpret_cast<const t8*>(qp + e * a.q.sh + (c >> 3) * a.q.sc);
+      for (int e0 = 0; e0 < a.group; e0 += 4) {  // four heads' loads in flight together
+        t8 x[4];
 #pragma unroll
-        for (int d = 0; d < 8; ++d) q[d] += (float)x[d];
+        for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const t8*>(qp + min(e0 + e, a.group - 1) * a.q.sh + (c >> 3) * a.q.sc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e0 + e < a.group)
+#pragma unroll
+            for (int d = 0; d < 8; ++d) q[d] += (float)x[e][d];
       }
     }
     bf16x8 qh, ql;
@@ -371,16 +393,16 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
       qh[d] = hi, ql[d] = lo;
       qq += q[d] * q[d];
     }
-    constexpr int TB = NT < 4 ? NT : 4;  // tiles whose loads are in flight together
+    constexpr int TB = NT < 8 ? NT : 8;  // tiles whose loads are in flight together
 #pragma unroll
     for (int t0 = 0; t0 < NT; t0 += TB) {
       if (t0 * 16 >= a.nb) break;
       bf16x8 mh[TB], ml[TB];
 #pragma unroll
       for (int t = 0; t < TB; ++t) {
-        const unsigned m = (unsigned)min((t0 + t) * 16 + n, a.nbp - 1) * (unsigned)(2 * a.dkp) + (unsigned)c;  // (at most 2^18)
+        const unsigned m = ((unsigned)min(t0 + t, (a.nbp >> 4) - 1) * (unsigned)(a.dkp >> 5) + (unsigned)(c0 >> 5)) * 1024u;
         mh[t] = *reinterpret_cast<const bf16x8*>(sp + m);
-        ml[t] = *reinterpret_cast<const bf16x8*>(sp + m + (unsigned)a.dkp);
+        ml[t] = *reinterpret_cast<const bf16x8*>(sp + m + 512);
       }
 #pragma unroll
       for (int t = 0; t < TB; ++t) {
@@ -396,14 +418,11 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   float big = 0.f;
 #pragma unroll
   for (int w = 0; w < NWORD; w += 2) {
-    const int j = w * 16 * 2 + lane;
-    const bool in = j < a.nb;
-    const float x = in ? a.norm[(long long)bh * a.nb + j] : 0.f;
-    const unsigned long long ok = __ballot(in && a.count[b * a.nb + (in ? j : 0)] > 0);
+    const unsigned long long ok = __ballot(cnt[w / 2] > 0);
     okw[w] = (unsigned)ok;
     if (w + 1 < NWORD) okw[w + 1] = (unsigned)(ok >> 32);
     can += __popcll(ok);
-    big = fmaxf(big, x < __builtin_huge_valf() ? x : __builtin_huge_valf());  // (NaN: no bound)
+    big = fmaxf(big, norm[w / 2] < __builtin_huge_valf() ? norm[w / 2] : __builtin_huge_valf());  // (NaN: no bound)
   }
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
@@ -470,9 +489,9 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   const float up = (found ? out : hi) + 2.f * err, dn = (found ? in : lo) - 2.f * err;   // the band around a cut that is not sure
   const float floor_ = sure ? cut : up;
 
-  // ---- picked blocks as words of 32, the same in every lane of a query; each lane writes its own, by rank
+  // ---- picked blocks as words of 32, the same in every lane of a query; lane g writes the ranks g, g + 4, ... (a lane that wrote its own
+  // blocks had up to eight of a word where neighbours are picked together: 9 us of 33)
   int* const row = a.picked + ((long long)bh * a.nq + i) * a.topk;
-  const unsigned own = 0x000F000Fu << (4 * g);
   unsigned inw[NWORD];
   int at = 0;
 #pragma unroll
@@ -483,20 +502,29 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
 #pragma unroll
       for (int r = 0; r < 4; ++r) bits |= (unsigned)(s[t][r] > floor_) << ((t & 1) * 16 + r);
     bits = quad_or(bits << (4 * g));
-    if (take == can) bits = okw[w];
-    inw[w] = bits;
-    unsigned left = sure && live ? bits & own : 0;
-    while (__ballot(left)) {
-      if (left) {
-        const int x = __ffs(left) - 1;
-        left &= left - 1;
-        row[at + __popc(bits & ((1u << x) - 1))] = w * 32 + x;
-      }
-    }
-    at += __popc(bits);
+    inw[w] = take == can ? okw[w] : bits;
+    at += __popc(inw[w]);
   }
   if (sure && live)
-    for (int t = take + g; t < a.topk; t += 4) row[t] = -1;
+    for (int t = g; t < a.topk; t += 4) {
+      int k = t, j = -1;
+      unsigned bits = 0;
+#pragma unroll
+      for (int w = 0; w < NWORD; ++w) {  // the word that holds rank t
+        const int n = __popc(inw[w]);
+        if (j < 0) {
+          if (k < n) j = w * 32, bits = inw[w];
+          else k -= n;
+        }
+      }
+      if (j >= 0)
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {  // its k-th set bit
+          const int n = __popc(bits & ((1u << o) - 1));
+          if (k >= n) k -= n, j += o, bits >>= o;
+        }
+      row[t] = j;
+    }
   // the other queries, one after another: 64-bit scores of the blocks next to the cut, or of all where that says too little
   unsigned long long todo = __ballot(!sure && live) & 0xFFFF;
   if (!todo) return;
@@ -522,32 +550,40 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
       __builtin_amdgcn_wave_barrier();
       continue;
     }
-    double qd[2] = {0, 0};
+    double* const qsum = qs[wave];
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (lane + 64 * x < a.dk)
-        for (int e = 0; e < a.group; ++e)
-          qd[x] += (double)(float)head_ptr<const T>(a, a.q, b, qi, h * a.group + e)[(lane >> 3) * a.q.sc + x * 8 * a.q.sc + (lane & 7)];
+    for (int x = 0; x < 2; ++x) {
+      const int d = lane + 64 * x;
+      if (d < a.dk) {
+        double q = 0;
+        for (int e = 0; e < a.group; ++e) q += (double)(float)head_ptr<const T>(a, a.q, b, qi, h * a.group + e)[(d >> 3) * a.q.sc + (d & 7)];
+        qsum[d] = q;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
     const int nmay = __builtin_amdgcn_readlane(may, k), need = __builtin_amdgcn_readlane(take - at, k);
-    double mine = 0;
+    double mine = 0;  // lane c: candidate c's score and block
     int mj = 0, c = 0;
 #pragma unroll
     for (int w = 0; w < NWORD; ++w) {
       unsigned bits = (unsigned)__builtin_amdgcn_readlane((int)mayw[w], k);
       while (bits) {  // (the same in every lane)
-        const int j = w * 32 + __ffs(bits) - 1;
+        mj = lane == c ? w * 32 + __ffs(bits) - 1 : mj;
         bits &= bits - 1;
-        double x = 0;
-        const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          if (lane + 64 * y < a.dk) x += qd[y] * m[lane + 64 * y];
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) x += shfl_xor_d(x, o);
-        if (lane == c) mine = x, mj = j;
         ++c;
       }
     }
+    for (int c0 = 0; c0 < nmay; c0 += 4) {  // four candidates at a time, sixteen lanes each
+      const int j = __shfl(mj, min(c0 + (lane >> 4), nmay - 1));
+      const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
+      double x = 0;
+      for (int d = lane & 15; d < a.dk; d += 16) x += qsum[d] * m[d];
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) x += shfl_xor_d(x, o);
+      const double y = __shfl(x, (lane - c0 & 3) * 16);
+      if (lane >= c0 && lane < c0 + 4) mine = y;
+    }
+    __builtin_amdgcn_wave_barrier();
     int before = 0;  // candidates in front of this lane's
     for (int x = 0; x < nmay; ++x) {
       const double v = __shfl(mine, x);
