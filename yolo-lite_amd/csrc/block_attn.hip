@@ -616,7 +616,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
 //
 // A block's results pass unnormalised (sum of p v; the maximum and sum of p beside them in fp32).  For fp16 tensors they are fp32.  For
 // bf16 tensors they are fp16, toward zero (2^-10 at most, a quarter of a bf16 step; fp32 took 278 instead of 150 us on the 128x128
-// map): the unit's values are scaled by a power of two, exact in bf16, that puts their largest at 2^8, so that the sums fill fp16's
+// map): a power of two per unit, carried by the weights (exact in bf16), puts the unit's largest value at 2^8, so that the sums fill fp16's
 // range from the top and what lies up to 2^23 below the largest value still has all its bits; the join scales back.
 //
 // Lists: 64 queries form a group; lists[group] holds its (query, slot) pairs sorted by block, starts[group][j] where block j's begin.
@@ -795,56 +795,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   const bool lok = lane < kn && (!a.mask || a.mask[b * a.mask_stride + k0 + lane]);
   const unsigned long long ok = __ballot(lok);  // the keys that may be read
   const bool alone = DIRECT && p.slots == 1;  // a row has this one result: it is the output
-  // ---- values, transposed, keys in a row; a masked value counts as 0 whatever it holds
-  __shared__ unsigned vmax;
-  if (HALF && !alone) {
-    if (tid == 0) vmax = 0;
-    __syncthreads();
-  }
-  const T* vb = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh;
-  constexpr int NV = (KEYS / 8 * (DVP / 8) + NT - 1) / NT;  // 8 x 8 pieces of a thread
-  t8 v[NV][8];
-  unsigned big = 0;  // bits of the largest finite |v|
-#pragma unroll
-  for (int x = 0; x < NV; ++x) {
-    const int it = tid + x * NT, c8 = it % (DVP / 8), kg = it / (DVP / 8);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      v[x][u] = t8{};
-      if (it < KEYS / 8 * (DVP / 8) && c8 * 8 < a.dv && (ok >> (kg * 8 + u) & 1))
-        v[x][u] = *reinterpret_cast<const t8*>(vb + token(a, k0 + kg * 8 + u) * a.v.st + c8 * a.v.sc);
-    }
-    if (HALF && !alone)
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned m = __float_as_uint((float)v[x][u][e]) & 0x7FFFFFFFu;
-          big = max(big, m < 0x7F800000u ? m : 0u);
-        }
-  }
-  float vscale = 1.f;
-  if (HALF && !alone) {
-    if (big) atomicMax(&vmax, big);
-    __syncthreads();
-    const int e = (int)(vmax >> 23) - 127;                // floor(log2 of the largest); -127: zeros, or not normal
-    const int up = vmax ? min(8 - e, 126) : 0;            // 2^up puts it at 2^8: sums of 64 weighted values stay under 2^15
-    vscale = up > -127 ? __uint_as_float((unsigned)(up + 127) << 23) : 0.f;
-    if (tid == 0) p.vexp[((long long)bh * a.nb + j) * p.subs + sub] = (signed char)-up;
-  }
-#pragma unroll
-  for (int x = 0; x < NV; ++x) {
-    const int it = tid + x * NT, c8 = it % (DVP / 8), kg = it / (DVP / 8);
-    if (it < KEYS / 8 * (DVP / 8))
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        t8 y;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) y[u] = HALF ? (T)((float)v[x][u][e] * vscale) : v[x][u][e];
-        *reinterpret_cast<t8*>(sVt + (c8 * 8 + e) * VP + kg * 8) = y;
-      }
-  }
-  // ---- keys: fragments of the first product (row = key, 8 dims of group g)
+  // ---- keys: fragments of the first product (row = key, 8 dims of group g), asked for first
   t8 kf[KT][DK32];
   const T* kb = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh;
 #pragma unroll
@@ -854,10 +805,63 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       kf[t][c] = t8{};
       if (t * 16 + n < kn && (c * 4 + g) * 8 < a.dk) kf[t][c] = *reinterpret_cast<const t8*>(kb + token(a, k0 + t * 16 + n) * a.k.st + (c * 4 + g) * a.k.sc);
     }
+  // ---- values, transposed, keys in a row; a masked value counts as 0 whatever it holds.  A thread moves two keys x 8 channels.
+  __shared__ unsigned vmax;
+  const T* vb = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh;
+  constexpr int ITEMS = KEYS / 2 * (DVP / 8), NV = (ITEMS + NT - 1) / NT;
+  u32x4 v[NV][2];
+#pragma unroll
+  for (int x = 0; x < NV; ++x) {
+    const int it = tid + x * NT, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      v[x][u] = u32x4{0, 0, 0, 0};
+      if (it < ITEMS && c8 * 8 < a.dv && (ok >> (key + u) & 1))
+        v[x][u] = *reinterpret_cast<const u32x4*>(vb + token(a, k0 + key + u) * a.v.st + c8 * a.v.sc);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < NV; ++x) {
+    const int it = tid + x * NT, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
+    if (it < ITEMS)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)  // (lower halves of a pair of words, upper halves)
+        *reinterpret_cast<unsigned*>(sVt + (c8 * 8 + e) * VP + key) =
+            __builtin_amdgcn_perm(v[x][1][e >> 1], v[x][0][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+  }
+  // The power of two 2^up that puts the largest finite |v| at 2^8: sums of 64 weighted values stay under 2^15.  The weights carry it
+  // (as far as they can without leaving bf16's range; the rest, where values are beyond 2^60, the stores).
+  float upw = 0.f, ups = 1.f;
+  if constexpr (HALF) {
+    if (tid == 0) vmax = 0;
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    us2 big = {0, 0};
+#pragma unroll
+    for (int x = 0; x < NV; ++x)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          us2 m = __builtin_bit_cast(us2, v[x][u][e] & 0x7FFF7FFFu);
+          m = us2{m[0] < 0x7F80 ? m[0] : (unsigned short)0, m[1] < 0x7F80 ? m[1] : (unsigned short)0};
+          big = __builtin_elementwise_max(big, m);
+        }
+    const unsigned top = max((unsigned)big[0], (unsigned)big[1]);
+    __syncthreads();
+    if (top) atomicMax(&vmax, top);
+    __syncthreads();
+    const int e = (int)(vmax >> 7) - 127;          // floor(log2 of the largest); -127: zeros, or not normal
+    const int up = vmax ? min(8 - e, 120) : 0;
+    const int uw = max(up, -60);
+    upw = (float)uw;
+    ups = __uint_as_float((unsigned)(up - uw + 127) << 23);  // (up - uw >= -59)
+    if (tid == 0) p.vexp[((long long)bh * a.nb + j) * p.subs + sub] = (signed char)-up;
+  } else {
+    __syncthreads();
+  }
   unsigned okt = 0;  // this lane's keys t * 16 + 4 g + r, four bits per tile
 #pragma unroll
   for (int t = 0; t < KT; ++t) okt |= (unsigned)(ok >> (t * 16 + 4 * g) & 15) << (4 * t);
-  __syncthreads();
   // values: which channel is row i of tile d -- one that lets the four lanes of a query store 64 neighbouring bytes at a time
   auto channel = [](int d, int i) { return HALF ? (d >> 1) * 32 + (i >> 2) * 8 + (d & 1) * 4 + (i & 3) : d * 16 + i; };
   t8 vf[DV16][KS];
@@ -873,6 +877,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   const float scale = fabsf(a.scale) * 1.44269504088896340736f;
   const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
   const bool all = ok == ~0ull >> (64 - KEYS);  // no key is masked: uniform
+  const float downw = __builtin_amdgcn_exp2f(-upw);  // (a whole power: exact)
   t8 one;
 #pragma unroll
   for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
@@ -946,12 +951,16 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     u32x4 pw[KS];
     if (all) {
       // max(x, y) = med3(x, y, inf): one instruction where fmaxf first quiets a possible signalling NaN (a NaN score makes NaN below)
+      float mt[KT];
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
+      for (int t = 0; t < KT; ++t) {  // (pairs, then pairs of pairs: a short chain)
+        const float x = __builtin_amdgcn_fmed3f(s[t][0], s[t][1], __builtin_huge_valf());
+        mt[t] = __builtin_amdgcn_fmed3f(x, __builtin_amdgcn_fmed3f(s[t][2], s[t][3], __builtin_huge_valf()), __builtin_huge_valf());
+      }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m = __builtin_amdgcn_fmed3f(m, s[t][r], __builtin_huge_valf());
-      m = quad_max(m) * scale;
-      const float base = m == ninf ? 0.f : m;  // (every score -inf: all weights 0)
+      for (int t = 1; t < KT; ++t) mt[0] = __builtin_amdgcn_fmed3f(mt[0], mt[t], __builtin_huge_valf());
+      m = quad_max(mt[0]) * scale;
+      const float base = (m == ninf ? 0.f : m) - upw;  // (every score -inf: all weights 0)
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -965,7 +974,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
         for (int r = 0; r < 4; ++r) m = okt >> (4 * t + r) & 1 ? fmaxf(m, s[t][r]) : m;
       m = quad_max(m);
       m = m == ninf ? m : m * scale;  // (no key: -inf, also where the scale is 0)
-      const float base = m == ninf ? 0.f : m;
+      const float base = (m == ninf ? 0.f : m) - upw;
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -981,7 +990,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < KS; ++x) lsum = Vec<T>::mfma(one, pf[x], lsum);
-    const float l = lsum[0];
+    const float l = HALF ? lsum[0] * downw : lsum[0];
     f32x4 o[DV16];
 #pragma unroll
     for (int d = 0; d < DV16; ++d) {
@@ -1004,6 +1013,9 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     }
     part_t* const dst = pb + (long long)(__umul24(local, (unsigned)p.slots) + (unsigned)w.slot) * DVP;
     if constexpr (HALF) {
+      if (ups != 1.f)
+#pragma unroll
+        for (int d = 0; d < DV16; ++d) o[d] *= ups;
       auto pk = [](float lo, float hi) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(lo, hi)); };
 #pragma unroll
       for (int d = 0; d < DV16; d += 2)
