@@ -225,44 +225,52 @@ __device__ __forceinline__ unsigned wave_or(unsigned c) {
   return (unsigned)__builtin_amdgcn_readlane((int)c, 63);
 }
 
-// One wave: lane holds the keys of blocks 64 i + lane (0 behind the last) -> the n-th largest by its bits, upper word first (the lower
-// words are looked at where the upper ones leave it open: ties), then the blocks at or over it in ascending order.
-template <int NI>
-__device__ __forceinline__ void pick_row(const unsigned long long (&key)[NI], int topk, int lane, int* out) {
-  int can = 0;
+// The n-th largest of the keys that the lanes hold (0: none), by its bits, upper word first: the lower words are looked at where the
+// upper ones leave it open (ties).  sum, any: over all lanes that hold keys.
+template <int NI, typename SUM, typename ANY>
+__device__ __forceinline__ unsigned long long nth_key(const unsigned long long (&key)[NI], int n, SUM sum, ANY any_of) {
   unsigned any = 0, none = 0;  // bits set in some key, clear in some key
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    can += key[i] != 0;
     any |= (unsigned)(key[i] >> 32);
     none |= ~(unsigned)(key[i] >> 32);
   }
+  any = any_of(any);
+  const unsigned differ = any & any_of(none);  // bits that all keys share need no decision
+  unsigned vh = any & ~differ, vl = 0;
+  bool exact = false;
+  for (unsigned left = differ; left && !exact;) {
+    const unsigned bit = 1u << (31 - __clz(left));
+    left &= ~bit;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) c += (unsigned)(key[i] >> 32) >= (vh | bit);
+    c = sum(c);
+    if (c >= n) vh |= bit;
+    exact = c == n;
+  }
+  for (int bit = 31; bit >= 0 && !exact; --bit) {
+    const unsigned long long t = (unsigned long long)vh << 32 | vl | 1u << bit;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) c += key[i] >= t;
+    c = sum(c);
+    if (c >= n) vl |= 1u << bit;
+    exact = c == n;
+  }
+  return (unsigned long long)vh << 32 | vl;
+}
+
+// One wave: lane holds the keys of blocks 64 i + lane (0 behind the last) -> the topk largest in ascending order; of equal ones the
+// first.
+template <int NI>
+__device__ __forceinline__ void pick_row(const unsigned long long (&key)[NI], int topk, int lane, int* out) {
+  int can = 0;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) can += key[i] != 0;
   const int n = min(topk, wave_sum(can));
   if (n > 0) {
-    any = wave_or(any);
-    const unsigned differ = any & wave_or(none);  // bits that all keys share need no decision
-    unsigned vh = any & ~differ, vl = 0;
-    bool exact = false;
-    for (unsigned left = differ; left && !exact;) {
-      const unsigned bit = 1u << (31 - __clz(left));
-      left &= ~bit;
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) c += (unsigned)(key[i] >> 32) >= (vh | bit);
-      c = wave_sum(c);
-      if (c >= n) vh |= bit;
-      exact = c == n;
-    }
-    for (int bit = 31; bit >= 0 && !exact; --bit) {
-      const unsigned long long t = (unsigned long long)vh << 32 | vl | 1u << bit;
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) c += key[i] >= t;
-      c = wave_sum(c);
-      if (c >= n) vl |= 1u << bit;
-      exact = c == n;
-    }
-    const unsigned long long v = (unsigned long long)vh << 32 | vl;
+    const unsigned long long v = nth_key(key, n, wave_sum, wave_or);
     int over = 0;  // keys > v
 #pragma unroll
     for (int i = 0; i < NI; ++i) over += key[i] > v;
@@ -281,9 +289,10 @@ __device__ __forceinline__ void pick_row(const unsigned long long (&key)[NI], in
   for (int t = n + lane; t < topk; t += 64) out[t] = -1;
 }
 
-// One wave: the exact scores of one (image, kv head, query) from the 64-bit means, then pick_row.  qs: dk doubles of LDS.
+// One wave: the exact scores of one (image, kv head, query) from the 64-bit means, as keys of blocks j0 + 64 x + lane.  qs: dk doubles
+// of LDS.
 template <typename T, int NI>
-__device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int lane, double* qs) {
+__device__ __forceinline__ void exact_keys(const BlockArgs& a, int bh, int i, int j0, int lane, double* qs, unsigned long long (&key)[NI]) {
   const int h = bh % a.kv, b = bh / a.kv;
   for (int d = lane; d < a.dk; d += 64) {
     double s = 0;
@@ -292,10 +301,9 @@ __device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int
     qs[d] = s;
   }
   __builtin_amdgcn_wave_barrier();
-  unsigned long long key[NI];
 #pragma unroll
   for (int x = 0; x < NI; ++x) {
-    const int j = x * 64 + lane;
+    const int j = j0 + x * 64 + lane;
     key[x] = 0;
     if (j < a.nb) {
       double s = 0;
@@ -305,71 +313,39 @@ __device__ __forceinline__ void exact_row(const BlockArgs& a, int bh, int i, int
       key[x] = order_key(s, a.count[b * a.nb + j] > 0);
     }
   }
-  pick_row<NI>(key, a.topk, lane, a.picked + ((long long)bh * a.nq + i) * a.topk);
+  __builtin_amdgcn_wave_barrier();
 }
 
-// SCORED: the scores are there (few queries); else from the means.  One wave per (image, kv head, query); up to 64 NI blocks.
-template <typename T, int NI, bool SCORED>
+// Few queries: the scores are there.  One wave per (image, kv head, query); up to 64 NI blocks.
+template <int NI>
 __global__ __launch_bounds__(64) void block_select_kernel(BlockArgs a) {
-  __shared__ double qs[SCORED ? 1 : 128];
   const int lane = threadIdx.x;
   const long long row = blockIdx.x;  // (b * kv + h) * nq + i
-  const int i = (int)(row % a.nq), bh = (int)(row / a.nq);
-  if constexpr (SCORED) {
-    unsigned long long key[NI];
-    double s[NI];
-    int n[NI];
+  const int b = (int)(row / a.nq) / a.kv;
+  unsigned long long key[NI];
+  double s[NI];
+  int n[NI];
 #pragma unroll
-    for (int x = 0; x < NI; ++x) {  // (all in flight together)
-      const int j = min(x * 64 + lane, a.nb - 1);
-      s[x] = a.nb ? a.score[row * a.nb + j] : 0.0;
-      n[x] = a.nb && x * 64 + lane < a.nb ? a.count[bh / a.kv * a.nb + j] : 0;
-    }
-#pragma unroll
-    for (int x = 0; x < NI; ++x) key[x] = order_key(s[x], n[x] > 0);
-    pick_row<NI>(key, a.topk, lane, a.picked + row * a.topk);
-  } else {
-    exact_row<T, NI>(a, bh, i, lane, qs);
+  for (int x = 0; x < NI; ++x) {  // (all in flight together)
+    const int j = min(x * 64 + lane, a.nb - 1);
+    s[x] = a.nb ? a.score[row * a.nb + j] : 0.0;
+    n[x] = a.nb && x * 64 + lane < a.nb ? a.count[b * a.nb + j] : 0;
   }
+#pragma unroll
+  for (int x = 0; x < NI; ++x) key[x] = order_key(s[x], n[x] > 0);
+  pick_row<NI>(key, a.topk, lane, a.picked + row * a.topk);
 }
 
-// Many queries, up to 16 NT blocks: a wave scores 16 queries at once on the matrix pipe, in less than 64 bits, and decides only what
-// that can decide.  q (summed over the group) and the means are split into two bf16 each; hi hi + hi lo + lo hi leaves out less than
-//   err = (3 * 2^-18 + 4 dk 2^-24) |q| |c|     (two splits, the product lo lo, an fp32 sum of 3 dk terms; |.| the 2-norms)
-// of a score (and, where a part is not a normal number any more, dk 2^-126 times the other norm; near the ends of fp32's range nothing
-// is decided here).  Lane (query n, group g) holds the scores of blocks 16 t + 4 g + r; the cut that leaves topk of them over it is found by
-// bisection, 16 queries in step.  Where the last block over the cut and the first under it are more than 2 err apart -- all but a
-// few in a thousand -- the order is the exact one's; the other queries (ties, NaN and infinities among them) are scored in 64 bits.
+// Scores of 16 queries with the means of blocks 16 t0 .. 16 (t0 + NT) on the matrix pipe: lane (query n, group g) gets those of
+// blocks 16 (t0 + t) + 4 g + r, and its share of the query's squared norm.  qp: the query's first head; bh: its means.
 template <typename T, int NT>
-__global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(BlockArgs a, int qtiles) {
-  __shared__ double qs[4][128];
-  constexpr int NWORD = (NT + 1) / 2;  // 32 blocks to a word
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
-  const unsigned unit = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x) * 4u + (unsigned)wave;  // (below 2^31: the rows are)
-  if (unit >= (unsigned)(a.batch * a.kv) * (unsigned)qtiles) return;  // (no barrier below: waves are on their own)
-  const int bh = (int)(unit / (unsigned)qtiles), qt = (int)(unit - (unsigned)bh * (unsigned)qtiles), h = bh % a.kv, b = bh / a.kv;
-  const int i = qt * 16 + n;
-  const bool live = i < a.nq;
-  const float ninf = -__builtin_huge_valf();
+__device__ __forceinline__ void score_tiles(const BlockArgs& a, int bh, const T* qp, int t0, int lane, f32x4 (&s)[NT], float& qq) {
   typedef T t8 __attribute__((ext_vector_type(8)));
-
-  // how many keys each block has to read, |c| -- asked for ahead of everything else
-  int cnt[(NWORD + 1) / 2];
-  float norm[(NWORD + 1) / 2];
-#pragma unroll
-  for (int w = 0; w < (NWORD + 1) / 2; ++w) {
-    const int j = min(w * 64 + lane, a.nb - 1);
-    cnt[w] = a.count[b * a.nb + j];
-    norm[w] = a.norm[(long long)bh * a.nb + j];
-    if (w * 64 + lane >= a.nb) cnt[w] = 0, norm[w] = 0.f;
-  }
-  // ---- scores
-  f32x4 s[NT];
+  const int g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < NT; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float qq = 0.f;
+  qq = 0.f;
   const __bf16* sp = a.split + split_at(a, bh, 0, 0) + lane * 8;
-  const T* qp = head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group);
   for (int c0 = 0; c0 < a.dkp; c0 += 32) {
     const int c = c0 + g * 8;
     float q[8] = {};
@@ -395,23 +371,97 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
     }
     constexpr int TB = NT < 8 ? NT : 8;  // tiles whose loads are in flight together
 #pragma unroll
-    for (int t0 = 0; t0 < NT; t0 += TB) {
-      if (t0 * 16 >= a.nb) break;
+    for (int u0 = 0; u0 < NT; u0 += TB) {
+      if ((t0 + u0) * 16 >= a.nb) break;
       bf16x8 mh[TB], ml[TB];
 #pragma unroll
       for (int t = 0; t < TB; ++t) {
-        const unsigned m = ((unsigned)min(t0 + t, (a.nbp >> 4) - 1) * (unsigned)(a.dkp >> 5) + (unsigned)(c0 >> 5)) * 1024u;
+        const unsigned m = ((unsigned)min(t0 + u0 + t, (a.nbp >> 4) - 1) * (unsigned)(a.dkp >> 5) + (unsigned)(c0 >> 5)) * 1024u;
         mh[t] = *reinterpret_cast<const bf16x8*>(sp + m);
         ml[t] = *reinterpret_cast<const bf16x8*>(sp + m + 512);
       }
 #pragma unroll
       for (int t = 0; t < TB; ++t) {
-        s[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], qh, s[t0 + t], 0, 0, 0);
-        s[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml[t], qh, s[t0 + t], 0, 0, 0);
-        s[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], ql, s[t0 + t], 0, 0, 0);
+        s[u0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], qh, s[u0 + t], 0, 0, 0);
+        s[u0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml[t], qh, s[u0 + t], 0, 0, 0);
+        s[u0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], ql, s[u0 + t], 0, 0, 0);
       }
     }
   }
+}
+// what such a score may be off by; qn, cn: the norms of the query and of the largest mean
+__device__ __forceinline__ float score_error(int dk, float qn, float cn) {
+  return (3.f / 262144.f + 4.f * dk / 16777216.f) * qn * cn + (qn + cn) * 2e-36f + 1e-30f;
+}
+
+// One wave: of nmay <= 16 candidates (lane c < nmay: block mj) the `need` with the largest 64-bit scores, as a mask of lanes; of equal
+// scores the lower block first.  qsum: dk doubles of LDS.
+template <typename T>
+__device__ __forceinline__ unsigned long long choose_exact(const BlockArgs& a, int bh, int i, int lane, int nmay, int need, int mj, double* qsum) {
+  const int h = bh % a.kv, b = bh / a.kv;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int d = lane + 64 * x;
+    if (d < a.dk) {
+      double q = 0;
+      for (int e = 0; e < a.group; ++e) q += (double)(float)head_ptr<const T>(a, a.q, b, i, h * a.group + e)[(d >> 3) * a.q.sc + (d & 7)];
+      qsum[d] = q;
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  double mine = 0;
+  for (int c0 = 0; c0 < nmay; c0 += 4) {  // four candidates at a time, sixteen lanes each
+    const int j = __shfl(mj, min(c0 + (lane >> 4), nmay - 1));
+    const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
+    double x = 0;
+    for (int d = lane & 15; d < a.dk; d += 16) x += qsum[d] * m[d];
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) x += shfl_xor_d(x, o);
+    const double y = __shfl(x, (lane - c0 & 3) * 16);
+    if (lane >= c0 && lane < c0 + 4) mine = y;
+  }
+  __builtin_amdgcn_wave_barrier();
+  int before = 0;  // candidates in front of this lane's
+  for (int x = 0; x < nmay; ++x) {
+    const double v = __shfl(mine, x);
+    before += v > mine || (v == mine && x < lane);
+  }
+  return __ballot(lane < nmay && before < need);
+}
+
+// Many queries, up to 16 NT blocks: a wave scores 16 queries at once on the matrix pipe, in less than 64 bits, and decides only what
+// that can decide.  q (summed over the group) and the means are split into two bf16 each; hi hi + hi lo + lo hi leaves out less than
+//   score_error = (3 * 2^-18 + 4 dk 2^-24) |q| |c|     (two splits, the product lo lo, an fp32 sum of 3 dk terms; |.| the 2-norms)
+// of a score (and, where a part is not a normal number any more, dk 2^-126 times the other norm; near the ends of fp32's range nothing
+// is decided here).  Lane (query n, group g) holds the scores of blocks 16 t + 4 g + r; the cut that leaves topk of them over it is found by
+// bisection, 16 queries in step.  Where the last block over the cut and the first under it are more than 2 err apart -- all but a
+// few in a thousand -- the order is the exact one's; the other queries (ties, NaN and infinities among them) are scored in 64 bits.
+template <typename T, int NT>
+__global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(BlockArgs a, int qtiles) {
+  __shared__ double qs[4][128];
+  constexpr int NWORD = (NT + 1) / 2;  // 32 blocks to a word
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  const unsigned unit = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x) * 4u + (unsigned)wave;  // (below 2^31: the rows are)
+  if (unit >= (unsigned)(a.batch * a.kv) * (unsigned)qtiles) return;  // (no barrier below: waves are on their own)
+  const int bh = (int)(unit / (unsigned)qtiles), qt = (int)(unit - (unsigned)bh * (unsigned)qtiles), h = bh % a.kv, b = bh / a.kv;
+  const int i = qt * 16 + n;
+  const bool live = i < a.nq;
+  const float ninf = -__builtin_huge_valf();
+
+  // how many keys each block has to read, |c| -- asked for ahead of everything else
+  int cnt[(NWORD + 1) / 2];
+  float norm[(NWORD + 1) / 2];
+#pragma unroll
+  for (int w = 0; w < (NWORD + 1) / 2; ++w) {
+    const int j = min(w * 64 + lane, a.nb - 1);
+    cnt[w] = a.count[b * a.nb + j];
+    norm[w] = a.norm[(long long)bh * a.nb + j];
+    if (w * 64 + lane >= a.nb) cnt[w] = 0, norm[w] = 0.f;
+  }
+  // ---- scores
+  f32x4 s[NT];
+  float qq;
+  score_tiles<T, NT>(a, bh, head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group), 0, lane, s, qq);
   // ---- which blocks can be selected, how many there are, the largest |c|
   unsigned okw[NWORD];
   int can = 0;
@@ -429,7 +479,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   big = quad_max(big);
   const int take = min(a.topk, can);
   const float qn = sqrtf(quad_sum(qq));
-  const float err = (3.f / 262144.f + 4.f * a.dk / 16777216.f) * qn * big + (qn + big) * 2e-36f + 1e-30f;
+  const float err = score_error(a.dk, qn, big);
 
   // ---- the cut.  Blocks that cannot be selected (and places behind the last) go under every cut
 #pragma unroll
@@ -546,24 +596,13 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
     todo &= todo - 1;
     const int qi = qt * 16 + k;
     if (!__builtin_amdgcn_readlane((int)few, k)) {
-      exact_row<T, (NT + 3) / 4>(a, bh, qi, lane, qs[wave]);
-      __builtin_amdgcn_wave_barrier();
+      unsigned long long key[(NT + 3) / 4];
+      exact_keys<T>(a, bh, qi, 0, lane, qs[wave], key);
+      pick_row(key, a.topk, lane, a.picked + ((long long)bh * a.nq + qi) * a.topk);
       continue;
     }
-    double* const qsum = qs[wave];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int d = lane + 64 * x;
-      if (d < a.dk) {
-        double q = 0;
-        for (int e = 0; e < a.group; ++e) q += (double)(float)head_ptr<const T>(a, a.q, b, qi, h * a.group + e)[(d >> 3) * a.q.sc + (d & 7)];
-        qsum[d] = q;
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
     const int nmay = __builtin_amdgcn_readlane(may, k), need = __builtin_amdgcn_readlane(take - at, k);
-    double mine = 0;  // lane c: candidate c's score and block
-    int mj = 0, c = 0;
+    int mj = 0, c = 0;  // lane c: candidate c
 #pragma unroll
     for (int w = 0; w < NWORD; ++w) {
       unsigned bits = (unsigned)__builtin_amdgcn_readlane((int)mayw[w], k);
@@ -573,23 +612,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
         ++c;
       }
     }
-    for (int c0 = 0; c0 < nmay; c0 += 4) {  // four candidates at a time, sixteen lanes each
-      const int j = __shfl(mj, min(c0 + (lane >> 4), nmay - 1));
-      const double* m = a.mean + ((long long)bh * a.nb + j) * a.dk;
-      double x = 0;
-      for (int d = lane & 15; d < a.dk; d += 16) x += qsum[d] * m[d];
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) x += shfl_xor_d(x, o);
-      const double y = __shfl(x, (lane - c0 & 3) * 16);
-      if (lane >= c0 && lane < c0 + 4) mine = y;
-    }
-    __builtin_amdgcn_wave_barrier();
-    int before = 0;  // candidates in front of this lane's
-    for (int x = 0; x < nmay; ++x) {
-      const double v = __shfl(mine, x);
-      before += v > mine || (v == mine && x < lane);
-    }
-    const unsigned long long chosen = __ballot(lane < nmay && before < need);
+    const unsigned long long chosen = choose_exact<T>(a, bh, qi, lane, nmay, need, mj, qs[wave]);
     int* const to = a.picked + ((long long)bh * a.nq + qi) * a.topk;
     int base = 0;
 #pragma unroll
@@ -606,11 +629,214 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   }
 }
 
+// The same by NW waves (4 or 8) for 16 queries: wave w has blocks 16 NT w .., each step of the bisection adds up their counts through
+// LDS.  Then a wave finishes 16 / NW queries, from words of 64 blocks.  What it is for: more blocks than a wave's registers hold scores
+// of (16384 queries, 513 blocks, 4 heads of 64: a wave per query with every score in 64 bits 707 us, this 84; 8192 queries, 1024 blocks,
+// 8 heads of 128: 1159 and 78 us), and few queries.  It is bound by its comparisons: 12 steps over the scores in registers.
+template <typename T, int NW, int NT>
+__global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, int qtiles) {
+  constexpr int WORDS = NT / 4;  // of a wave
+  __shared__ double qs[NW][128];
+  __shared__ unsigned long long inw[16][64], mayw[16][64];
+  __shared__ int red[2][NW][16];
+  __shared__ int cand[NW][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  const unsigned unit = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x);
+  const int bh = (int)(unit / (unsigned)qtiles), qt = (int)(unit - (unsigned)bh * (unsigned)qtiles), h = bh % a.kv, b = bh / a.kv;
+  const int i = qt * 16 + n, t0 = wave * NT;
+  const bool live = i < a.nq;
+  const float ninf = -__builtin_huge_valf(), inf = __builtin_huge_valf();
+
+  // a value per wave and query -> over the waves.  (Two buffers: one barrier is enough)
+  int turn = 0;
+  auto gather = [&](int x, int* lo, int* hi) __attribute__((always_inline)) {
+    turn ^= 1;
+    if (g == 0) red[turn][wave][n] = x;
+    __syncthreads();
+    *lo = red[turn][g][n], *hi = NW == 8 ? red[turn][NW - 4 + g][n] : 0;
+  };
+  auto sum_all = [&](int x) __attribute__((always_inline)) {
+    int p, q;
+    gather(x, &p, &q);
+    return quad_sum(p + q);
+  };
+  auto max_all = [&](float x) __attribute__((always_inline)) {
+    int p, q;
+    gather((int)__float_as_uint(x), &p, &q);
+    return quad_max(NW == 8 ? fmaxf(__uint_as_float((unsigned)p), __uint_as_float((unsigned)q)) : __uint_as_float((unsigned)p));
+  };
+
+  // ---- which of this wave's blocks can be selected, how many there are in all, the largest |c|; scores
+  unsigned long long okw[WORDS];
+  int can = 0;
+  float big = 0.f;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int j = t0 * 16 + w * 64 + lane;
+    const float norm = j < a.nb ? a.norm[(long long)bh * a.nb + j] : 0.f;
+    okw[w] = __ballot(j < a.nb && a.count[b * a.nb + min(j, a.nb - 1)] > 0);
+    can += __popcll(okw[w]);
+    big = fmaxf(big, norm < inf ? norm : inf);  // (NaN: no bound)
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
+  big = max_all(quad_max(big));
+  can = sum_all(can);
+  f32x4 s[NT];
+  float qq;
+  score_tiles<T, NT>(a, bh, head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group), t0, lane, s, qq);
+  const int take = min(a.topk, can);
+  const float qn = sqrtf(quad_sum(qq));
+  const float err = score_error(a.dk, qn, big);
+
+  // ---- the cut, as above
+  float hi = ninf;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const unsigned m = (unsigned)(okw[t >> 2] >> ((t & 3) * 16 + 4 * g));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[t][r] = m >> r & 1 ? s[t][r] : ninf;
+      hi = fmaxf(hi, s[t][r]);
+    }
+  }
+  hi = max_all(quad_max(hi));
+  float lo = -1.01f * qn * big - 1e-30f;
+  float cut = ninf;
+  bool found = take == can;
+  for (int it = 0; it < 32 && __ballot(!found && live); ++it) {  // (the same in every wave)
+    const float mid = 0.5f * (lo + hi);
+    int c = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c += s[t][r] > mid;
+    c = sum_all(quad_sum(c));
+    if (c == take) cut = found ? cut : mid, found = true;
+    lo = c > take && !found ? mid : lo;
+    hi = c < take && !found ? mid : hi;
+  }
+  float in = inf, out = ninf;  // the two sides of the cut
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool over = s[t][r] > cut;
+      in = over ? fminf(in, s[t][r]) : in;
+      out = over ? out : fmaxf(out, s[t][r]);
+    }
+  in = -max_all(-quad_min(in));
+  out = max_all(quad_max(out));
+  const bool fine = qn * big < 1e37f, sure = take == can || (found && fine && in - out > 2.f * err);
+  const float up = (found ? out : hi) + 2.f * err, dn = (found ? in : lo) - 2.f * err;
+  const float floor_ = sure ? cut : up;
+
+  // ---- words of 64 blocks: picked, and in the band around a cut that is not sure
+  int at = 0, may = 0;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    unsigned long long over = 0, band = 0;
+#pragma unroll
+    for (int t = 4 * w; t < 4 * w + 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        over |= (unsigned long long)(s[t][r] > floor_) << ((t & 3) * 16 + r);
+        band |= (unsigned long long)(!sure && s[t][r] <= up && s[t][r] >= dn) << ((t & 3) * 16 + r);
+      }
+    over <<= 4 * g, band <<= 4 * g;
+    over = (unsigned long long)quad_or((unsigned)(over >> 32)) << 32 | quad_or((unsigned)over);
+    band = (unsigned long long)quad_or((unsigned)(band >> 32)) << 32 | quad_or((unsigned)band);
+    over = take == can ? okw[w] : over;
+    band &= okw[w];
+    at += __popcll(over), may += __popcll(band);
+    if (g == 0) inw[n][wave * WORDS + w] = over, mayw[n][wave * WORDS + w] = band;
+  }
+  at = sum_all(at);
+  may = sum_all(may);  // (and the words of all waves are there)
+  const bool few = fine && may <= 16 && at <= take && at + may >= take;
+
+  // ---- queries about which that says too little: 64-bit scores of all blocks, by all waves
+  const unsigned long long all = __ballot(!sure && !few && live) & 0xFFFF;  // (the same in every wave)
+  for (unsigned long long todo = all; todo; todo &= todo - 1) {
+    const int k = __ffsll(todo) - 1;
+    unsigned long long key[WORDS];
+    exact_keys<T>(a, bh, qt * 16 + k, t0 * 16, lane, qs[wave], key);
+    // (sums of waves lie at query 0 of `red`; a lane of the first eight has a wave's)
+    auto sum = [&](int x) __attribute__((always_inline)) {
+      x = wave_sum(x);
+      turn ^= 1;
+      if (lane == 0) red[turn][wave][0] = x;
+      __syncthreads();
+      return wave_sum(lane < NW ? red[turn][lane][0] : 0);
+    };
+    auto any = [&](unsigned x) __attribute__((always_inline)) {
+      x = wave_or(x);
+      turn ^= 1;
+      if (lane == 0) red[turn][wave][0] = (int)x;
+      __syncthreads();
+      return wave_or(lane < NW ? (unsigned)red[turn][lane][0] : 0u);
+    };
+    const int want = __builtin_amdgcn_readlane(take, k);  // (fewer than can be selected: the others are sure)
+    const unsigned long long v = nth_key(key, want, sum, any);
+    int over = 0, same = 0;
+#pragma unroll
+    for (int x = 0; x < WORDS; ++x) over += key[x] > v, same += key[x] == v;
+    int ties = want - sum(over);
+    sum(same);
+    const int before = wave_sum(lane < wave ? red[turn][lane][0] : 0);  // ties in the waves ahead
+    ties = max(0, ties - before);
+#pragma unroll
+    for (int x = 0; x < WORDS; ++x) {
+      const unsigned long long eq = __ballot(key[x] == v);
+      const bool got = key[x] > v || (key[x] == v && __popcll(eq & ((1ull << lane) - 1)) < ties);
+      ties -= min(ties, (int)__popcll(eq));
+      const unsigned long long bits = __ballot(got);
+      if (lane == 0) inw[k][wave * WORDS + x] = bits;
+    }
+  }
+  if (all) __syncthreads();
+
+  // ---- this wave's two queries: lane l has blocks 64 l ..
+  for (int k = 16 / NW * wave; k < 16 / NW * (wave + 1); ++k) {
+    const int qi = qt * 16 + k;
+    if (qi >= a.nq) break;
+    const bool some = __builtin_amdgcn_readlane((int)(!sure && few), k);  // some of the blocks of the band
+    auto places = [&](unsigned long long bits, int* total) {  // bits in the lanes before this one
+      const int c = __popcll(bits);
+      int x = c;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+      }
+      *total = __shfl(x, 63);
+      return x - c;
+    };
+    unsigned long long bits = lane < NW * WORDS ? inw[k][lane] : 0;
+    if (some) {
+      int nmay;
+      unsigned long long band = lane < NW * WORDS ? mayw[k][lane] : 0;
+      for (int c = places(band, &nmay); band; band &= band - 1) cand[wave][c++] = lane * 64 + __ffsll(band) - 1;
+      __builtin_amdgcn_wave_barrier();
+      const int mj = cand[wave][max(0, min(lane, nmay - 1))];
+      const int need = __builtin_amdgcn_readlane(take - at, k);
+      for (unsigned long long left = choose_exact<T>(a, bh, qi, lane, nmay, need, mj, qs[wave]); left; left &= left - 1) {
+        const int j = __builtin_amdgcn_readlane(mj, __ffsll(left) - 1);
+        if (j >> 6 == lane) bits |= 1ull << (j & 63);
+      }
+    }
+    int* const to = a.picked + ((long long)bh * a.nq + qi) * a.topk;
+    int total;
+    for (int c = places(bits, &total); bits; bits &= bits - 1) to[c++] = lane * 64 + __ffsll(bits) - 1;
+    for (int t = total + lane; t < a.topk; t += 64) to[t] = -1;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ attention
 // Queries that pick their blocks one by one share no tile of keys.  Turned round they do: a workgroup takes ONE block (its keys in
 // the registers of every wave, its values through LDS) and gathers the queries that picked it, 16 (query, head) rows to an MFMA
 // tile -- S^T = K Q^T, softmax over the block, O^T = V^T P^T, where the S^T accumulators of two 16-key tiles are, after exp2, the B
-// fragment of the second product -- and writes the block's normalised result of each row with its maximum and sum; a second launch
+// fragment of the second product -- and writes the block's result of each row with its maximum and sum; a second launch
 // joins a row's blocks.  Keys are read once per block and range of queries instead of once per query; the price is that every (row,
 // block) result passes through memory, which is what bounds the stage (2 (dv + 4) bytes written and read per row and block).
 //
@@ -1141,8 +1367,7 @@ static int by_type16(int dtype, F f) {
 using namespace yl;
 
 // ---- how the selection runs, and where things lie in the workspace
-constexpr int SCORE_MAX_NQ = 4;       // so few queries are scored by the wave that has the mean
-constexpr int SCORE_MAX_BLOCKS = 512; // scores of 16 queries in a wave's registers
+constexpr int SCORE_MAX_NQ = 4;  // so few queries are scored by the wave that has the mean
 struct SelectPlan {
   long long mean, score, split, norm, count, all;  // byte offsets
 };
@@ -1188,40 +1413,45 @@ static int mean_launch(const BlockArgs& a, hipStream_t s) {
   return 0;
 }
 
-template <typename T, int NT>
-static int score_launch(const BlockArgs& a, hipStream_t s) {
-  const int qtiles = (a.nq + 15) / 16;
-  const long long wg = ((long long)a.batch * a.kv * qtiles + 3) / 4;
-  hipLaunchKernelGGL((block_score_kernel<T, NT>), dim3((unsigned)wg), dim3(256), 0, s, a, qtiles);
+template <typename T, int NW, int NT>
+static int score_launch(const BlockArgs& a, int qtiles, unsigned units, hipStream_t s) {
+  if constexpr (NW > 1)
+    hipLaunchKernelGGL((block_score_wide_kernel<T, NW, NT>), dim3(units), dim3(64 * NW), 0, s, a, qtiles);
+  else
+    hipLaunchKernelGGL((block_score_kernel<T, NT>), dim3((units + 3) / 4), dim3(256), 0, s, a, qtiles);
   YL_HIP(hipGetLastError());
   return 0;
+}
+// One wave per 16 queries up to 128 blocks (6400 of them: 38 us where four waves take 100, the whole call).  Above, as few waves as have
+// the registers where 16-query tiles alone fill the card (256 blocks, 8192 tiles: one wave 102, four 140 us; 512 blocks, 4096 tiles: four
+// 145, eight 167 us), more waves where they do not (256 blocks, 512 tiles: 33 and 27 us; 512 blocks, 128 tiles: 31 and 28 us).
+template <typename T>
+static int score_by_size(const BlockArgs& a, hipStream_t s) {
+  const int qtiles = (a.nq + 15) / 16;
+  const unsigned units = (unsigned)((long long)a.batch * a.kv * qtiles);  // (below 2^31)
+  if (a.nb <= 64) return score_launch<T, 1, 4>(a, qtiles, units, s);
+  if (a.nb <= 128) return score_launch<T, 1, 8>(a, qtiles, units, s);
+  if (a.nb <= 256) return units < 2048 ? score_launch<T, 4, 4>(a, qtiles, units, s) : score_launch<T, 1, 16>(a, qtiles, units, s);
+  if (a.nb <= 512) return units <= 512 ? score_launch<T, 8, 4>(a, qtiles, units, s) : score_launch<T, 4, 8>(a, qtiles, units, s);
+  if (a.nb <= 1024) return score_launch<T, 8, 8>(a, qtiles, units, s);
+  return a.nb <= 2048 ? score_launch<T, 8, 16>(a, qtiles, units, s) : score_launch<T, 8, 32>(a, qtiles, units, s);
 }
 
 // the selection of `a` (sizes and tensors filled in) into a.picked, with plan `p` and its workspace
 static int select_run(BlockArgs& a, const SelectPlan& p, int dtype, char* w, hipStream_t s) {
-  const int batch = a.batch, nq = a.nq, kv_heads = a.kv;
   a.mean = reinterpret_cast<double*>(w + p.mean), a.score = reinterpret_cast<double*>(w + p.score);
   a.split = reinterpret_cast<__bf16*>(w + p.split), a.norm = reinterpret_cast<float*>(w + p.norm);
   a.count = reinterpret_cast<int*>(w + p.count);
   return by_type16(dtype, [&](auto* t) {
     typedef BA_T(t) T;
-    const bool few = nq <= SCORE_MAX_NQ;
+    const bool few = a.nq <= SCORE_MAX_NQ;
     if (a.nb > 0)
       if (int rc = few ? mean_launch<T, true>(a, s) : mean_launch<T, false>(a, s)) return rc;
-    if (!few && a.nb > 0 && a.nb <= SCORE_MAX_BLOCKS) {
-      if (a.nb <= 64) return score_launch<T, 4>(a, s);
-      if (a.nb <= 128) return score_launch<T, 8>(a, s);
-      return a.nb <= 256 ? score_launch<T, 16>(a, s) : score_launch<T, 32>(a, s);
-    }
-#define BA_SELECT(NI)                                                                                                  \
-  do {                                                                                                                 \
-    if (few) hipLaunchKernelGGL((block_select_kernel<T, NI, true>), dim3(batch * kv_heads * nq), dim3(64), 0, s, a);   \
-    else hipLaunchKernelGGL((block_select_kernel<T, NI, false>), dim3(batch * kv_heads * nq), dim3(64), 0, s, a);      \
-  } while (0)
-    if (a.nb <= 256) BA_SELECT(4);
-    else if (a.nb <= 1024) BA_SELECT(16);
-    else BA_SELECT(64);
-#undef BA_SELECT
+    if (!few && a.nb > 0) return score_by_size<T>(a, s);
+    const dim3 grid((unsigned)(a.batch * a.kv * a.nq));
+    if (a.nb <= 256) hipLaunchKernelGGL(block_select_kernel<4>, grid, dim3(64), 0, s, a);
+    else if (a.nb <= 1024) hipLaunchKernelGGL(block_select_kernel<16>, grid, dim3(64), 0, s, a);
+    else hipLaunchKernelGGL(block_select_kernel<64>, grid, dim3(64), 0, s, a);
     YL_HIP(hipGetLastError());
     return 0;
   });
@@ -1252,7 +1482,6 @@ struct AttendPlan {
 
 constexpr long long CHUNK_BYTES = 256LL << 20;  // block results in memory at once (measured: 128 MB and more the same time, 64 MB 15 % more, 16 MB twice)
 static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
-
   AttendPlan p{};
   p.subs = a.block == 128 ? 2 : 1;
   p.slots = a.topk * p.subs;
