@@ -684,8 +684,11 @@ static Plan plan_linear(int x_dtype, long long rows, long long n, long long k) {
     p.k4 = (kb + 15) / 16, p.xgroups = (rows + 63) / 64, p.wgroups = (n + 63) / 64;
     p.xs = p.k4 * p.xgroups * 1024, p.ws = p.k4 * p.wgroups * 1024;
   } else {
-    p.wt = rows <= 32 ? 1 : 2;
-    p.xt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    // 32 weight rows x 64 rows of x to a workgroup, 16 x 32 where that makes few workgroups (whole call: 300 x 96 x 16384 (15 of the
+    // large) 44 / 23 us, 64 x 4096 x 4096 (128) 13.4 / 12.9; 33 x 8192 x 8192 (256) 19 / 33)
+    const bool small = rows <= 32 || (n + 31) / 32 * ((rows + 63) / 64) <= 128;
+    p.wt = small ? 1 : 2;
+    p.xt = rows <= 16 ? 1 : (small ? 2 : 4);
     p.ntiles = (n + 16 * p.wt - 1) / (16 * p.wt), p.mtiles = (rows + 16 * p.xt - 1) / (16 * p.xt);
     if (p.xt == 1) p.codes = 0;  // (x is quantised where it is read)
     p.xs = x_dtype == YL_MX4 || p.xt == 1 ? 0 : (rows * kb + 255) / 256 * 256;
