@@ -149,6 +149,15 @@ def test_linear_sizes(gpu_device, rows, n, k, dtype):
     _check_product(y, mx4_ref.rounded(_np(x)), mx4_ref.rounded(_np(w)), b, False, r)
 
 
+@pytest.mark.parametrize("rows, n, k", [(1, 16400, 1056), (9, 16385, 1100), (2, 300, 60000), (16, 4100, 4128), (70, 4100, 160), (300, 96, 4000)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_linear_of_few_rows_with_large_weights(gpu_device, rows, n, k, packed):
+    ya = _ya()
+    x, w, b, r = _linear_case(gpu_device, rows, n, k, "bf16", True, False, True)
+    y = ya.mx4_linear(ya.mx4_quantize(x) if packed else x, ya.mx4_quantize(w), bias=b, res=r)
+    _check_product(y, mx4_ref.rounded(_np(x)), mx4_ref.rounded(_np(w)), b, False, r)
+
+
 @pytest.mark.parametrize("rows, n, k", [(1, 72, 160), (40, 200, 288), (400, 304, 416), (2048, 512, 256)])
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("bias, act, res", [(0, 0, 0), (1, 1, 0), (0, 1, 1), (1, 0, 1), (1, 1, 1)])

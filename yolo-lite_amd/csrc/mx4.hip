@@ -246,7 +246,8 @@ __device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 v, long long 
 // tiles would leave most of the chip idle.  A workgroup owns 16 WT weight rows x 16 XT rows of x; its NW waves take the k-steps in
 // turn, operands straight from memory into registers, and the partial sums meet in LDS in a fixed order.
 // X: what x is: codes (uint8_t), or the values themselves -- a lane's part of the operand is one row's block of 32, so each lane
-// quantises its own, without a launch, a workspace or an exchange (16 rows; every workgroup does it again, under the weight's loads).
+// quantises its own, without a launch, a workspace or an exchange (16 rows and weights of up to 2^24 elements: see plan_linear).
+// Measured, one row: 4096 x 4096 values 8 us (cold caches 11), codes 5-6; 128000 x 4096 codes 63 us, 4400 GB/s.
 template <typename T, typename X, int WT, int XT, int NW>
 __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
   __shared__ __attribute__((aligned(16))) f32x4 part[NW][WT * XT][64];
@@ -659,7 +660,7 @@ extern "C" int yl_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, in
 
 // ---- how a product runs: a wave per 16 x 16 tile for few rows, else tiles through LDS on the pipe's own order of the scales
 struct Plan {
-  bool tiled, big;
+  bool tiled, big, inplace;
   int wt, xt;                    // split over k: 16-row tiles of a workgroup
   long long ntiles, mtiles;
   long long codes, xs, ws, all;  // bytes: codes of x, scales of x, tiled scales of the weight, the workspace
@@ -687,11 +688,16 @@ static Plan plan_linear(int x_dtype, long long rows, long long n, long long k) {
     // 32 weight rows x 64 rows of x to a workgroup, 16 x 32 where that makes few workgroups (whole call: 300 x 96 x 16384 (15 of the
     // large) 44 / 23 us, 64 x 4096 x 4096 (128) 13.4 / 12.9; 33 x 8192 x 8192 (256) 19 / 33)
     const bool small = rows <= 32 || (n + 31) / 32 * ((rows + 63) / 64) <= 128;
-    p.wt = small ? 1 : 2;
     p.xt = rows <= 16 ? 1 : (small ? 2 : 4);
+    // Up to 16 rows of values are quantised where they are read, by every workgroup again: what that costs grows with the weight, a launch
+    // of its own does not.  In place / two launches: 1 x 4096 x 4096 11.4 / 6.1 + 4.7 us with a gap between (kernels alone, cold caches),
+    // 1 x 11008 x 4096 18.6 / 11.7, 1 x 32000 x 4096 59 / 21 (whole call).
+    p.inplace = x_dtype != YL_MX4 && p.xt == 1 && n * k <= 1 << 24;
+    // two weight tiles share a workgroup's codes where there are many (16 x 32000 x 4096 30 / 23 us, 1 x 8192 x 4096 no difference)
+    p.wt = small ? (p.xt == 1 && !p.inplace && n >= 16384 ? 2 : 1) : 2;
     p.ntiles = (n + 16 * p.wt - 1) / (16 * p.wt), p.mtiles = (rows + 16 * p.xt - 1) / (16 * p.xt);
-    if (p.xt == 1) p.codes = 0;  // (x is quantised where it is read)
-    p.xs = x_dtype == YL_MX4 || p.xt == 1 ? 0 : (rows * kb + 255) / 256 * 256;
+    if (p.inplace) p.codes = 0;
+    p.xs = x_dtype == YL_MX4 || p.inplace ? 0 : (rows * kb + 255) / 256 * 256;
   }
   p.all = p.codes + p.xs + p.ws;
   return p;
@@ -753,7 +759,7 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
   a.x = packed ? x : codes, a.x_stride = 16LL * a.kb;
   if (!p.tiled) {
     a.xs = packed ? x_scales : xs;
-    if (!packed && p.xt == 1) {
+    if (p.inplace) {
       a.x = x, a.x_stride = x_stride, a.xvec = xvec;
       return by_type(y_dtype, [&](auto* t) {
         return by_type(x_dtype, [&](auto* u) {
@@ -765,7 +771,7 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
       if (int rc = quantize_launch(x, x_dtype, rows, k, x_stride, codes, xs, s)) return rc;
     return by_type(y_dtype, [&](auto* t) {
       typedef std::remove_pointer_t<decltype(t)> T;
-      if (p.xt == 1) return split_launch<T, uint8_t, 1, 1, 8>(a, s);
+      if (p.xt == 1) return p.wt == 1 ? split_launch<T, uint8_t, 1, 1, 8>(a, s) : split_launch<T, uint8_t, 2, 1, 8>(a, s);
       return p.xt == 2 ? split_launch<T, uint8_t, 1, 2, 8>(a, s) : split_launch<T, uint8_t, 2, 4, 8>(a, s);
     });
   }
