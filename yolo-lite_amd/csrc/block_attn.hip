@@ -938,8 +938,10 @@ __global__ __launch_bounds__(64) void block_lists_kernel(AttendArgs p) {
 }
 
 // DIRECT: one wave per (image, kv head, query, slot, unit) straight from `picked` -- few queries, where lists would hold one entry.
+// Four workgroups on a CU where the fragments leave room (128 registers; at 131, three of them, the 128x128 map's launch took 119 instead
+// of 108 us; five spill).
 template <typename T, int KEYS, int DK32, int DV16, bool DIRECT>
-__global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(AttendArgs p) {
+__global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 4 ? 4 : 2) void block_attend_kernel(AttendArgs p) {
   typedef typename Vec<T>::t8 t8;
   typedef typename Vec<T>::t4 t4;
   constexpr int NT = DIRECT ? 64 : 256;
@@ -953,7 +955,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int g = lane >> 4, n = lane & 15;
   const float ninf = -__builtin_huge_valf();
-  // ---- which block, which queries
+  // ---- which block
   int unit = xcd_remap((int)blockIdx.x, (int)gridDim.x);  // neighbours share an image, a head, a range of queries: one L2
   int sub = 0, j, bh, grp0 = 0, nrows, qdirect = 0, tdirect = 0;
   if (KEYS == 64) {
@@ -985,6 +987,40 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
     unit /= a.nb;
     grp0 = p.g0 + unit % p.nrange * p.range;
     bh = unit / p.nrange;
+  }
+  const int h = bh % a.kv, b = bh / a.kv;
+  const int k0 = j * a.block + sub * KEYS;
+  const int kn = min(min(KEYS, a.block - sub * KEYS), a.nk - k0);  // keys of this unit; <= 0: none
+  const bool lok = lane < kn && (!a.mask || a.mask[b * a.mask_stride + k0 + lane]);
+  const unsigned long long ok = __ballot(lok);  // the keys that may be read
+  const bool alone = DIRECT && p.slots == 1;  // a row has this one result: it is the output
+  // ---- keys: fragments of the first product (row = key, 8 dims of group g).  Keys and values are asked for ahead of the lists.
+  t8 kf[KT][DK32];
+  const T* kb = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int c = 0; c < DK32; ++c) {
+      kf[t][c] = t8{};
+      if (t * 16 + n < kn && (c * 4 + g) * 8 < a.dk) kf[t][c] = *reinterpret_cast<const t8*>(kb + token(a, k0 + t * 16 + n) * a.k.st + (c * 4 + g) * a.k.sc);
+    }
+  // ---- values; a masked one counts as 0 whatever it holds.  A thread moves two keys x 8 channels.
+  __shared__ unsigned vmax;
+  const T* vb = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh;
+  constexpr int ITEMS = KEYS / 2 * (DVP / 8), NV = (ITEMS + NT - 1) / NT;
+  u32x4 v[NV][2];
+#pragma unroll
+  for (int x = 0; x < NV; ++x) {
+    const int it = tid + x * NT, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      v[x][u] = u32x4{0, 0, 0, 0};
+      if (it < ITEMS && c8 * 8 < a.dv && (ok >> (key + u) & 1))
+        v[x][u] = *reinterpret_cast<const u32x4*>(vb + token(a, k0 + key + u) * a.v.st + c8 * a.v.sc);
+    }
+  }
+  // ---- which queries
+  if constexpr (!DIRECT) {
     const int ng = min(p.range, p.g0 + p.gn - grp0);
     if (wave == 0) {  // a lane per group: where its share of the list begins, here and there
       int lo = 0, cnt = 0;
@@ -1015,37 +1051,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, 2) void block_attend_kernel(Atte
       rows[e] = (unsigned)x << 12 | p.lists[at + from[x] + e - first[x]];
     }
   }
-  const int h = bh % a.kv, b = bh / a.kv;
-  const int k0 = j * a.block + sub * KEYS;
-  const int kn = min(min(KEYS, a.block - sub * KEYS), a.nk - k0);  // keys of this unit; <= 0: none
-  const bool lok = lane < kn && (!a.mask || a.mask[b * a.mask_stride + k0 + lane]);
-  const unsigned long long ok = __ballot(lok);  // the keys that may be read
-  const bool alone = DIRECT && p.slots == 1;  // a row has this one result: it is the output
-  // ---- keys: fragments of the first product (row = key, 8 dims of group g), asked for first
-  t8 kf[KT][DK32];
-  const T* kb = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh;
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int c = 0; c < DK32; ++c) {
-      kf[t][c] = t8{};
-      if (t * 16 + n < kn && (c * 4 + g) * 8 < a.dk) kf[t][c] = *reinterpret_cast<const t8*>(kb + token(a, k0 + t * 16 + n) * a.k.st + (c * 4 + g) * a.k.sc);
-    }
-  // ---- values, transposed, keys in a row; a masked value counts as 0 whatever it holds.  A thread moves two keys x 8 channels.
-  __shared__ unsigned vmax;
-  const T* vb = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh;
-  constexpr int ITEMS = KEYS / 2 * (DVP / 8), NV = (ITEMS + NT - 1) / NT;
-  u32x4 v[NV][2];
-#pragma unroll
-  for (int x = 0; x < NV; ++x) {
-    const int it = tid + x * NT, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      v[x][u] = u32x4{0, 0, 0, 0};
-      if (it < ITEMS && c8 * 8 < a.dv && (ok >> (key + u) & 1))
-        v[x][u] = *reinterpret_cast<const u32x4*>(vb + token(a, k0 + key + u) * a.v.st + c8 * a.v.sc);
-    }
-  }
+  // ... transposed, keys in a row
 #pragma unroll
   for (int x = 0; x < NV; ++x) {
     const int it = tid + x * NT, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
