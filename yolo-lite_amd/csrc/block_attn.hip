@@ -897,19 +897,29 @@ __global__ __launch_bounds__(64) void block_lists_kernel(AttendArgs p) {
   __syncthreads();
   const long long q = (long long)bh * p.a.nq + i;
   const int* pick = p.a.picked + q * topk;
+  const unsigned long long me = 1ull << lane;
   unsigned long long first = 0;  // this query's slots that count
-  if (i < p.a.nq)
-    for (int t = 0; t < topk; ++t) {
-      const int j = pick[t];
-      if (j >= 0 && j < nb && !(word[j] >> lane & 1)) {  // (only this lane sets this bit)
-        atomicOr(&word[j], 1ull << lane);
-        first |= 1ull << t;
-      } else {
-        for (int u = 0; u < p.subs; ++u)
+  constexpr int U = 8;           // picks in flight together (one by one a memory latency each: the launch took 11 instead of 9 us on the 128x128 map)
+  auto picks = [&](int t0, int (&js)[U]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) js[u] = i < p.a.nq && t0 + u < topk ? pick[t0 + u] : -1;
+  };
+  for (int t0 = 0; t0 < topk; t0 += U) {
+    int js[U];
+    picks(t0, js);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = js[u];
+      if (j >= 0 && j < nb && !(word[j] & me)) {  // (only this lane sets this bit)
+        atomicOr(&word[j], me);
+        first |= 1ull << (t0 + u);
+      } else if (i < p.a.nq && t0 + u < topk) {
+        for (int sub = 0; sub < p.subs; ++sub)
           for (int g = 0; g < p.a.group; ++g)
-            p.ml[((long long)bh * p.slots + t * p.subs + u) * p.mlrow + (long long)i * p.a.group + g] = float2{-__builtin_huge_valf(), 0.f};
+            p.ml[((long long)bh * p.slots + (t0 + u) * p.subs + sub) * p.mlrow + (long long)i * p.a.group + g] = float2{-__builtin_huge_valf(), 0.f};
       }
     }
+  }
   __syncthreads();
   int base = 0;
   for (int j0 = 0; j0 < nb; j0 += 64) {  // where each block's queries begin
@@ -928,12 +938,13 @@ __global__ __launch_bounds__(64) void block_lists_kernel(AttendArgs p) {
   __syncthreads();
   const long long at = (long long)bh * p.groups + grp;
   unsigned short* list = p.lists + at * (64 * topk);
-  if (i < p.a.nq)
-    for (int t = 0; t < topk; ++t) {
-      if (!(first >> t & 1)) continue;
-      const int j = pick[t];
-      list[start[j] + __popcll(word[j] & ((1ull << lane) - 1))] = (unsigned short)(lane << 6 | t);
-    }
+  for (int t0 = 0; t0 < topk; t0 += U) {
+    int js[U];
+    picks(t0, js);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first >> (t0 + u) & 1) list[start[js[u]] + __popcll(word[js[u]] & (me - 1))] = (unsigned short)(lane << 6 | (t0 + u));
+  }
   for (int j = lane; j <= nb; j += 64) p.starts[at * (nb + 1) + j] = start[j];
 }
 
