@@ -205,41 +205,45 @@ struct LinearArgs {
 
 __device__ __forceinline__ v8i widen(v4i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1); }
 
-// y[m][n .. n + 4): bias, SiLU, residual, one rounding (everything is loaded before anything is used)
+// y[m][n .. n + 4): bias, SiLU, residual, one rounding.  What is added is asked for ahead of the product.
 template <typename T>
-__device__ __forceinline__ void finish4(const LinearArgs& a, f32x4 v, long long m, int n) {
+struct Finish4 {
   typedef T t4 __attribute__((ext_vector_type(4)));
-  const int left = a.n - n;
-  const T* rp = static_cast<const T*>(a.res) + m * a.res_stride + n;
-  T* yp = static_cast<T*>(a.y) + m * a.y_stride + n;
-  const bool vec = a.vec && left >= 4;
   float bias[4], res[4];
+  __device__ __forceinline__ void load(const LinearArgs& a, long long m, int n) {
+    const int left = a.n - n;
+    const T* rp = static_cast<const T*>(a.res) + m * a.res_stride + n;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) bias[r] = a.bias && r < left ? a.bias[n + r] : 0.f;
-  if (a.res) {
-    if (vec) {
-      const t4 q = *reinterpret_cast<const t4*>(rp);
+    for (int r = 0; r < 4; ++r) bias[r] = a.bias && r < left ? a.bias[n + r] : 0.f;
+    if (a.res) {
+      if (a.vec && left >= 4) {
+        const t4 q = *reinterpret_cast<const t4*>(rp);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) res[r] = (float)q[r];
-    } else {
+        for (int r = 0; r < 4; ++r) res[r] = (float)q[r];
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) res[r] = r < left ? (float)rp[r] : 0.f;
+        for (int r = 0; r < 4; ++r) res[r] = r < left ? (float)rp[r] : 0.f;
+      }
     }
   }
+  __device__ __forceinline__ void store(const LinearArgs& a, f32x4 v, long long m, int n) const {
+    const int left = a.n - n;
+    T* yp = static_cast<T*>(a.y) + m * a.y_stride + n;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    v[r] += bias[r];
-    if (a.act) v[r] = silu_f(v[r]);
-    if (a.res) v[r] += res[r];
-  }
-  if (vec) {
-    *reinterpret_cast<t4*>(yp) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-  } else {
+    for (int r = 0; r < 4; ++r) {
+      v[r] += bias[r];
+      if (a.act) v[r] = silu_f(v[r]);
+      if (a.res) v[r] += res[r];
+    }
+    if (a.vec && left >= 4) {
+      *reinterpret_cast<t4*>(yp) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (r < left) yp[r] = (T)v[r];
+      for (int r = 0; r < 4; ++r)
+        if (r < left) yp[r] = (T)v[r];
+    }
   }
-}
+};
 
 // ------------------------------------------------------------------------------------------------ product, split over k
 // Few rows: the product is the time it takes to read the weight (one row of x: 0.53 bytes per multiply-add), and a grid of large
@@ -275,6 +279,13 @@ __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
   for (int i = 0; i < WT; ++i)
 #pragma unroll
     for (int j = 0; j < XT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the tile that this wave finishes
+  static_assert(WT * XT <= NW, "a wave finishes one tile at most");
+  const int fi = wave / XT, fj = wave % XT, fn = n0 + fi * 16 + 4 * g;
+  const long long fm = m0 + fj * 16 + r;
+  const bool finishes = wave < WT * XT && fm < a.rows;
+  Finish4<T> fin;
+  if (finishes) fin.load(a, fm, fn);
   const int nk = (a.kb + 3) >> 2;
   constexpr int U = WT * XT <= 2 ? 4 : 2;  // k-steps whose loads are in flight together
   for (int it0 = wave; it0 < nk; it0 += U * NW) {
@@ -282,6 +293,7 @@ __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
     int sw[U][WT], sx[U][XT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (u && it0 + u * NW >= nk) break;  // (the same in every lane)
       const int b = (it0 + u * NW) * 4 + g;
       const bool in = b < a.kb;  // columns behind the last: zeros
       const int bb = in ? b : 0;
@@ -302,29 +314,25 @@ __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      if (u && it0 + u * NW >= nk) break;
 #pragma unroll
       for (int i = 0; i < WT; ++i)
 #pragma unroll
         for (int j = 0; j < XT; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(w[u][i]), widen(x[u][j]), acc[i][j], 4, 4, 0, sw[u][i], 0, sx[u][j]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < WT; ++i)
 #pragma unroll
     for (int j = 0; j < XT; ++j) part[wave][i * XT + j][lane] = acc[i][j];
   __syncthreads();
+  if (!finishes) return;
+  f32x4 s = part[0][wave][lane];
 #pragma unroll
-  for (int t0 = 0; t0 < WT * XT; t0 += NW) {
-    const int t = t0 + wave;
-    if (t >= WT * XT) break;
-    const int i = t / XT, j = t % XT;
-    const long long m = m0 + j * 16 + r;
-    f32x4 s = part[0][t][lane];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) s += part[w][t][lane];
-    if (m < a.rows) finish4<T>(a, s, m, n0 + i * 16 + 4 * g);
-  }
+  for (int w = 1; w < NW; ++w) s += part[w][wave][lane];
+  fin.store(a, s, fm, fn);
 }
 
 // ------------------------------------------------------------------------------------------------ tiled product
