@@ -102,9 +102,9 @@ __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
   typedef T t8 __attribute__((ext_vector_type(8)));
   constexpr int KL = 64 / CP;
   const int lane = threadIdx.x & 63;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= (long long)a.batch * a.kv * a.nb) return;
-  const int j = (int)(unit % a.nb), bh = (int)(unit / a.nb), h = bh % a.kv, b = bh / a.kv;
+  const unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6);  // (below 2^31, as the blocks are: no 64-bit division)
+  if (unit >= (unsigned)(a.batch * a.kv * a.nb)) return;
+  const int bh = (int)(unit / (unsigned)a.nb), j = (int)(unit - (unsigned)bh * (unsigned)a.nb), h = bh % a.kv, b = bh / a.kv;
   const int c = lane % CP, kl = lane / CP;
   const int k0 = j * a.block, kn = min(a.block, a.nk - k0);
   const T* kp = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh + c * a.k.sc;
@@ -225,18 +225,47 @@ __device__ __forceinline__ unsigned wave_or(unsigned c) {
   return (unsigned)__builtin_amdgcn_readlane((int)c, 63);
 }
 
+// The same over a workgroup's NW waves (all of them call), through two small buffers of LDS in turn: one barrier each.
+template <int NW>
+struct Waves {
+  int (*red)[NW];  // [2][NW]
+  int lane, wave, turn;
+  __device__ __forceinline__ void put(int x) {
+    turn ^= 1;
+    if (lane == 0) red[turn][wave] = x;
+    __syncthreads();
+  }
+  __device__ __forceinline__ int sum(int x) {
+    x = wave_sum(x);
+    if constexpr (NW == 1) return x;
+    put(x);
+    return wave_sum(lane < NW ? red[turn][lane] : 0);
+  }
+  __device__ __forceinline__ unsigned any(unsigned x) {
+    x = wave_or(x);
+    if constexpr (NW == 1) return x;
+    put((int)x);
+    return wave_or(lane < NW ? (unsigned)red[turn][lane] : 0u);
+  }
+  __device__ __forceinline__ int before(int x) {  // sum over the waves ahead of this one
+    if constexpr (NW == 1) return 0;
+    put(wave_sum(x));
+    return wave_sum(lane < wave ? red[turn][lane] : 0);
+  }
+};
+
 // The n-th largest of the keys that the lanes hold (0: none), by its bits, upper word first: the lower words are looked at where the
-// upper ones leave it open (ties).  sum, any: over all lanes that hold keys.
-template <int NI, typename SUM, typename ANY>
-__device__ __forceinline__ unsigned long long nth_key(const unsigned long long (&key)[NI], int n, SUM sum, ANY any_of) {
+// upper ones leave it open (ties).
+template <int NW, int NI>
+__device__ __forceinline__ unsigned long long nth_key(const unsigned long long (&key)[NI], int n, Waves<NW>& ws) {
   unsigned any = 0, none = 0;  // bits set in some key, clear in some key
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     any |= (unsigned)(key[i] >> 32);
     none |= ~(unsigned)(key[i] >> 32);
   }
-  any = any_of(any);
-  const unsigned differ = any & any_of(none);  // bits that all keys share need no decision
+  any = ws.any(any);
+  const unsigned differ = any & ws.any(none);  // bits that all keys share need no decision
   unsigned vh = any & ~differ, vl = 0;
   bool exact = false;
   for (unsigned left = differ; left && !exact;) {
@@ -245,7 +274,7 @@ __device__ __forceinline__ unsigned long long nth_key(const unsigned long long (
     int c = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) c += (unsigned)(key[i] >> 32) >= (vh | bit);
-    c = sum(c);
+    c = ws.sum(c);
     if (c >= n) vh |= bit;
     exact = c == n;
   }
@@ -254,27 +283,33 @@ __device__ __forceinline__ unsigned long long nth_key(const unsigned long long (
     int c = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) c += key[i] >= t;
-    c = sum(c);
+    c = ws.sum(c);
     if (c >= n) vl |= 1u << bit;
     exact = c == n;
   }
   return (unsigned long long)vh << 32 | vl;
 }
 
-// One wave: lane holds the keys of blocks 64 i + lane (0 behind the last) -> the topk largest in ascending order; of equal ones the
-// first.
-template <int NI>
-__device__ __forceinline__ void pick_row(const unsigned long long (&key)[NI], int topk, int lane, int* out) {
+// NW waves: lane holds the keys of blocks 64 (NI wave + i) + lane (0 behind the last) -> the topk largest in ascending order; of equal
+// ones the first.
+template <int NW, int NI>
+__device__ __forceinline__ void pick_row(const unsigned long long (&key)[NI], int topk, Waves<NW>& ws, int* out) {
+  const int lane = ws.lane;
   int can = 0;
 #pragma unroll
   for (int i = 0; i < NI; ++i) can += key[i] != 0;
-  const int n = min(topk, wave_sum(can));
+  const int n = min(topk, ws.sum(can));
   if (n > 0) {
-    const unsigned long long v = nth_key(key, n, wave_sum, wave_or);
-    int over = 0;  // keys > v
+    const unsigned long long v = nth_key(key, n, ws);
+    int over = 0, same = 0;  // keys > v, keys equal to v
 #pragma unroll
-    for (int i = 0; i < NI; ++i) over += key[i] > v;
-    int at = 0, ties = n - wave_sum(over);  // of the keys equal to v the first `ties` belong to the set
+    for (int i = 0; i < NI; ++i) over += key[i] > v, same += key[i] == v;
+    int ties = n - ws.sum(over), at = 0;  // of the equal keys the first `ties` belong to the set
+    if constexpr (NW > 1) {
+      ties = max(0, ties - ws.before(same));
+      const int mine = wave_sum(over) + min(ties, wave_sum(same));
+      at = ws.before(lane == 0 ? mine : 0);
+    }
     const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -282,11 +317,11 @@ __device__ __forceinline__ void pick_row(const unsigned long long (&key)[NI], in
       const bool take = key[i] > v || (key[i] == v && __popcll(eq & below) < ties);
       ties -= min(ties, (int)__popcll(eq));
       const unsigned long long got = __ballot(take);
-      if (take) out[at + __popcll(got & below)] = i * 64 + lane;
+      if (take) out[at + __popcll(got & below)] = (ws.wave * NI + i) * 64 + lane;
       at += __popcll(got);
     }
   }
-  for (int t = n + lane; t < topk; t += 64) out[t] = -1;
+  for (int t = n + ws.wave * 64 + lane; t < topk; t += 64 * NW) out[t] = -1;
 }
 
 // One wave: the exact scores of one (image, kv head, query) from the 64-bit means, as keys of blocks j0 + 64 x + lane.  qs: dk doubles
@@ -316,24 +351,27 @@ __device__ __forceinline__ void exact_keys(const BlockArgs& a, int bh, int i, in
   __builtin_amdgcn_wave_barrier();
 }
 
-// Few queries: the scores are there.  One wave per (image, kv head, query); up to 64 NI blocks.
-template <int NI>
-__global__ __launch_bounds__(64) void block_select_kernel(BlockArgs a) {
-  const int lane = threadIdx.x;
+// Few queries: the scores are there.  NW waves per (image, kv head, query), up to 256 NW blocks.  Nothing here but latency: 256 blocks 5,
+// 1024 blocks 8.4 us (by one wave, 16 to a lane, 11.6).
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void block_select_kernel(BlockArgs a) {
+  constexpr int NI = 4;
+  __shared__ int red[2][NW];
+  Waves<NW> ws{red, (int)threadIdx.x & 63, (int)threadIdx.x >> 6, 0};
   const long long row = blockIdx.x;  // (b * kv + h) * nq + i
-  const int b = (int)(row / a.nq) / a.kv;
+  const int b = (int)(blockIdx.x / (unsigned)a.nq / (unsigned)a.kv);
   unsigned long long key[NI];
   double s[NI];
   int n[NI];
 #pragma unroll
   for (int x = 0; x < NI; ++x) {  // (all in flight together)
-    const int j = min(x * 64 + lane, a.nb - 1);
+    const int at = (ws.wave * NI + x) * 64 + ws.lane, j = min(at, a.nb - 1);
     s[x] = a.nb ? a.score[row * a.nb + j] : 0.0;
-    n[x] = a.nb && x * 64 + lane < a.nb ? a.count[b * a.nb + j] : 0;
+    n[x] = at < a.nb ? a.count[b * a.nb + j] : 0;
   }
 #pragma unroll
   for (int x = 0; x < NI; ++x) key[x] = order_key(s[x], n[x] > 0);
-  pick_row<NI>(key, a.topk, lane, a.picked + row * a.topk);
+  pick_row(key, a.topk, ws, a.picked + row * a.topk);
 }
 
 // Scores of 16 queries with the means of blocks 16 t0 .. 16 (t0 + NT) on the matrix pipe: lane (query n, group g) gets those of
@@ -598,7 +636,8 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
     if (!__builtin_amdgcn_readlane((int)few, k)) {
       unsigned long long key[(NT + 3) / 4];
       exact_keys<T>(a, bh, qi, 0, lane, qs[wave], key);
-      pick_row(key, a.topk, lane, a.picked + ((long long)bh * a.nq + qi) * a.topk);
+      Waves<1> ws{nullptr, lane, 0, 0};
+      pick_row(key, a.topk, ws, a.picked + ((long long)bh * a.nq + qi) * a.topk);
       continue;
     }
     const int nmay = __builtin_amdgcn_readlane(may, k), need = __builtin_amdgcn_readlane(take - at, k);
@@ -638,7 +677,7 @@ __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, 
   constexpr int WORDS = NT / 4;  // of a wave
   __shared__ double qs[NW][128];
   __shared__ unsigned long long inw[16][64], mayw[16][64];
-  __shared__ int red[2][NW][16];
+  __shared__ int red[2][NW][16], red1[2][NW];
   __shared__ int cand[NW][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   const unsigned unit = (unsigned)xcd_remap((int)blockIdx.x, (int)gridDim.x);
@@ -757,34 +796,18 @@ __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, 
 
   // ---- queries about which that says too little: 64-bit scores of all blocks, by all waves
   const unsigned long long all = __ballot(!sure && !few && live) & 0xFFFF;  // (the same in every wave)
+  Waves<NW> ws{red1, lane, wave, 0};
   for (unsigned long long todo = all; todo; todo &= todo - 1) {
     const int k = __ffsll(todo) - 1;
     unsigned long long key[WORDS];
     exact_keys<T>(a, bh, qt * 16 + k, t0 * 16, lane, qs[wave], key);
-    // (sums of waves lie at query 0 of `red`; a lane of the first eight has a wave's)
-    auto sum = [&](int x) __attribute__((always_inline)) {
-      x = wave_sum(x);
-      turn ^= 1;
-      if (lane == 0) red[turn][wave][0] = x;
-      __syncthreads();
-      return wave_sum(lane < NW ? red[turn][lane][0] : 0);
-    };
-    auto any = [&](unsigned x) __attribute__((always_inline)) {
-      x = wave_or(x);
-      turn ^= 1;
-      if (lane == 0) red[turn][wave][0] = (int)x;
-      __syncthreads();
-      return wave_or(lane < NW ? (unsigned)red[turn][lane][0] : 0u);
-    };
     const int want = __builtin_amdgcn_readlane(take, k);  // (fewer than can be selected: the others are sure)
-    const unsigned long long v = nth_key(key, want, sum, any);
+    const unsigned long long v = nth_key(key, want, ws);
     int over = 0, same = 0;
 #pragma unroll
     for (int x = 0; x < WORDS; ++x) over += key[x] > v, same += key[x] == v;
-    int ties = want - sum(over);
-    sum(same);
-    const int before = wave_sum(lane < wave ? red[turn][lane][0] : 0);  // ties in the waves ahead
-    ties = max(0, ties - before);
+    int ties = want - ws.sum(over);
+    ties = max(0, ties - ws.before(same));
 #pragma unroll
     for (int x = 0; x < WORDS; ++x) {
       const unsigned long long eq = __ballot(key[x] == v);
@@ -1278,13 +1301,12 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   typedef typename Vec<T>::t8 t8;
   const BlockArgs& a = p.a;
   constexpr int C = DVP / 8;
-  const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int c = (int)(item % C) * 8;
-  const long long prow = item / C;  // rows of this launch's queries
-  const int cq = min(p.gn * 64, a.nq - p.g0 * 64);
-  if (prow >= (long long)a.batch * a.kv * cq * a.group || c >= a.dv) return;
-  const int gh = (int)(prow % a.group);
-  const int i = p.g0 * 64 + (int)(prow / a.group % cq), bh = (int)(prow / a.group / cq);
+  const int c = (int)(threadIdx.x % C) * 8;
+  const unsigned prow = blockIdx.x * (256 / C) + threadIdx.x / C;  // rows of this launch's queries, fewer than 2^31
+  const unsigned cq = (unsigned)min(p.gn * 64, a.nq - p.g0 * 64);
+  if (prow >= (unsigned)a.batch * (unsigned)a.heads * cq || c >= a.dv) return;
+  const unsigned e = prow / (unsigned)a.group, q = e / cq;
+  const int gh = (int)(prow - e * (unsigned)a.group), i = p.g0 * 64 + (int)(e - q * cq), bh = (int)q;
   const float2* ml = p.ml + (long long)bh * p.slots * p.mlrow + (long long)i * a.group + gh;
   typedef P p8 __attribute__((ext_vector_type(8)));
   constexpr bool HALF = sizeof(P) == 2;
@@ -1466,9 +1488,9 @@ static int select_run(BlockArgs& a, const SelectPlan& p, int dtype, char* w, hip
       if (int rc = few ? mean_launch<T, true>(a, s) : mean_launch<T, false>(a, s)) return rc;
     if (!few && a.nb > 0) return score_by_size<T>(a, s);
     const dim3 grid((unsigned)(a.batch * a.kv * a.nq));
-    if (a.nb <= 256) hipLaunchKernelGGL(block_select_kernel<4>, grid, dim3(64), 0, s, a);
-    else if (a.nb <= 1024) hipLaunchKernelGGL(block_select_kernel<16>, grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL(block_select_kernel<64>, grid, dim3(64), 0, s, a);
+    if (a.nb <= 256) hipLaunchKernelGGL(block_select_kernel<1>, grid, dim3(64), 0, s, a);
+    else if (a.nb <= 1024) hipLaunchKernelGGL(block_select_kernel<4>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(block_select_kernel<16>, grid, dim3(1024), 0, s, a);
     YL_HIP(hipGetLastError());
     return 0;
   });
