@@ -379,7 +379,7 @@ int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype, int64_t r
  *   mask: [batch][nk] bytes (row stride mask_stride), non-zero = the key may be read; NULL: all.  What a masked key or value holds
  *   does not matter.  A query without a readable key gets zeros (and -1 for every block).
  * An element (b, t, h, c) of a tensor lies at data[b * batch + t * token + h * head + c]: strides in elements, multiples of 8, not
- * negative (0 broadcasts); data 16-byte aligned. */
+ * negative (0 broadcasts; not in `out`); data 16-byte aligned. */
 typedef struct yl_heads {
   void* data;
   int64_t batch, token, head;

@@ -84,6 +84,22 @@ def test_attention_refusals(change, code):
     assert _run("attention", change) == code
 
 
+def test_products_of_sizes_that_wrap_in_64_bits_are_refused():
+    from yololite_amd import _lib
+
+    L = _lib.lib()
+    for name in ("select", "attention"):
+        assert _run(name, dict(batch=1 << 22, heads=1 << 21, kv_heads=1 << 21, nq=1 << 21)) == -3
+        assert _run(name, dict(batch=1 << 30, heads=1 << 30, kv_heads=1 << 30, nq=1, nk=64 * 4096)) == -3
+    assert L.yl_block_attention_workspace_bytes(0, 1 << 22, 1 << 21, 100, 1 << 21, 1 << 21, 32, 64, 64, 2) == -1
+    assert L.yl_attention_scratch_bytes(1 << 30, 1 << 30, 16, 64, 2) == -1
+
+
+@pytest.mark.parametrize("out", [dict(token=0), dict(head=0), dict(batch=0)])
+def test_broadcast_results_are_refused(out):
+    assert _run("attention", dict(out=out, batch=2)) == -1
+
+
 def test_workspace_refusals():
     from yololite_amd import _lib
 

@@ -244,6 +244,18 @@ def test_long_maps(gpu_device):
     _check_attend(q, k, far, picked, 32)
 
 
+def test_queries_far_apart(gpu_device):
+    """Queries and keys whose token strides do not fit 24 bits, with one and with several heads."""
+    room = torch.zeros((40 << 24) + 4096, dtype=torch.bfloat16, device=gpu_device)
+    for heads in (1, 2):
+        q, k, v = _inputs(gpu_device, 1, 40, 130, heads, 1, 32, 32, seed=heads)
+        far = room.as_strided((1, 40, heads, 32), (8, 1 << 24, 40, 1))
+        far.copy_(q)
+        picked = _check_select(far, k, 32, 2)
+        _check_attend(far, k, v, picked, 32)
+        _check_attend(far[:, :3], k, v, picked[:, :, :3], 32)
+
+
 def test_refusals(gpu_device):
     ya = _ya()
     q, k, v = _inputs(gpu_device, 1, 10, 100, 4, 2, 32, 64)

@@ -1359,6 +1359,9 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
 // ------------------------------------------------------------------------------------------------ host
 static long long round256(long long n) { return (n + 255) / 256 * 256; }
 
+// a * b * c below 2^31 (factors below 2^31: a product in 64 bits could wrap around)
+static bool fits31(long long a, long long b, long long c) { return (double)a * (double)b * (double)c < 2147483648.0; }
+
 static int check_heads(const std::string& who, const char* name, const yl_heads* t) {
   if (!t || !t->data) return fail(-1, who + ": null " + name);
   if ((reinterpret_cast<uintptr_t>(t->data) & 15) || ((t->batch | t->token | t->head) & 7))
@@ -1379,7 +1382,7 @@ static int fill_args(const std::string& who, const yl_heads* q, const yl_heads* 
   if (topk < 1 || topk > BA_MAX_TOPK) return fail(-3, who + ": 1 to 64 blocks for a query");
   const long long nb = ((long long)nk + block - 1) / block;
   if (nb > BA_MAX_BLOCKS) return fail(-3, who + ": more than 4096 key blocks");
-  if ((long long)batch * heads * nq > 0x7FFFFFFFLL || (long long)batch * kv_heads * nb > 0x7FFFFFFFLL)
+  if (!fits31(batch, heads, nq) || !fits31(batch, kv_heads, nb))
     return fail(-3, who + ": more rows or blocks than one launch covers");
   if (batch * (long long)nq == 0) return 0;
   if (int rc = check_heads(who, "q", q)) return rc;
@@ -1636,6 +1639,8 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
   if (nk > 0)
     if (int rc = check_heads("block_attention", "v", v)) return rc;
   if (int rc = check_heads("block_attention", "out", out)) return rc;
+  if ((batch > 1 && out->batch == 0) || (nq > 1 && out->token == 0) || (heads > 1 && out->head == 0))
+    return fail(-1, "block_attention: out has a stride of 0");
   if (!picked) return fail(-1, "block_attention: null pointer");
   const AttendPlan pl = plan_attend(a, dv, dtype);
   if (!work || work_bytes < pl.all || (reinterpret_cast<uintptr_t>(work) & 15))
@@ -1678,7 +1683,7 @@ int block_attention_map_launch(const AttnArgs& t, int block, int topk, char* wor
 
 extern "C" int64_t yl_attention_scratch_bytes(int batch, int heads, int tokens, int block, int topk) {
   if (batch < 1 || heads < 1 || tokens < 1 || (block != 32 && block != 64 && block != 128) || topk < 1 || topk > BA_MAX_TOPK ||
-      ((long long)tokens + block - 1) / block > BA_MAX_BLOCKS || (long long)batch * heads * tokens > 0x7FFFFFFFLL) {
+      ((long long)tokens + block - 1) / block > BA_MAX_BLOCKS || !yl::fits31(batch, heads, tokens)) {
     fail(-3, "attention: blocks of 32, 64 or 128 tokens, at most 4096 of them, 1 to 64 for a token");
     return -1;
   }
