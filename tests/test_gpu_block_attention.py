@@ -244,6 +244,19 @@ def test_long_maps(gpu_device):
     _check_attend(q, k, far, picked, 32)
 
 
+@pytest.mark.parametrize("nq, topk, block", [(1, 1, 64), (1, 3, 64), (3, 64, 128), (90, 1, 32), (90, 5, 64), (200, 64, 128)])
+@pytest.mark.parametrize("exponent", [127, 90, -60, -100])
+def test_ends_of_the_range_of_values(gpu_device, nq, topk, block, exponent):
+    """Every value next to the largest (or tiny): no sum on the way leaves the range."""
+    q, k, v = _inputs(gpu_device, 1, nq, 64 * 128 if topk == 64 else 300, 2, 1, 32, 32)
+    v = (v.sign() * (2 - 2.0 ** -7) * 2.0 ** (exponent / 2) * 2.0 ** (exponent - exponent / 2)).bfloat16()
+    v[..., 3] = v[..., 3].abs()
+    v[..., 4:] = torch.where(torch.rand(v[..., 4:].shape, generator=torch.Generator().manual_seed(1)).to(gpu_device) < 0.9, v[..., 4:], 0)
+    picked = _check_select(q, k, block, topk)
+    out = _check_attend(q, k, v, picked, block)
+    assert torch.equal(out[..., 3], v[0, 0, 0, 3].expand_as(out[..., 3]))
+
+
 def test_queries_far_apart(gpu_device):
     """Queries and keys whose token strides do not fit 24 bits, with one and with several heads."""
     room = torch.zeros((40 << 24) + 4096, dtype=torch.bfloat16, device=gpu_device)

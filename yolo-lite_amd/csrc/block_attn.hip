@@ -876,6 +876,8 @@ struct Vec;
 template <>
 struct Vec<__bf16> {
   typedef _Float16 part;  // a block's results between the launches
+  // sums of weighted values are held times 2^-down: 64 keys x 64 blocks of the largest values stay in fp32's range
+  static constexpr int down = 16;
   typedef bf16x8 t8;
   typedef bf16x4 t4;
   static __device__ __forceinline__ f32x4 mfma(t8 a, t8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -884,6 +886,7 @@ struct Vec<__bf16> {
 template <>
 struct Vec<_Float16> {
   typedef float part;
+  static constexpr int down = 0;
   typedef f16x8 t8;
   typedef _Float16 t4 __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ f32x4 mfma(t8 a, t8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -981,6 +984,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
   constexpr int NT = DIRECT ? 64 : 256;
   typedef std::conditional_t<DIRECT, float, typename Vec<T>::part> part_t;  // (few rows: nothing to save)
   constexpr bool HALF = sizeof(part_t) == 2;
+  constexpr int DOWN = Vec<T>::down;
   constexpr int KT = KEYS / 16, KS = KEYS / 32, DVP = DV16 * 16, VP = KEYS + 8;
   __shared__ __attribute__((aligned(16))) T sVt[DVP * VP];
   extern __shared__ unsigned rows[];  // [64 * range]: group in the range << 12 | query << 6 | slot
@@ -1095,9 +1099,9 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
         *reinterpret_cast<unsigned*>(sVt + (c8 * 8 + e) * VP + key) =
             __builtin_amdgcn_perm(v[x][1][e >> 1], v[x][0][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
   }
-  // The power of two 2^up that puts the largest finite |v| at 2^8: sums of 64 weighted values stay under 2^15.  The weights carry it
-  // (as far as they can without leaving bf16's range; the rest, where values are beyond 2^60, the stores).
-  float upw = 0.f, ups = 1.f;
+  // The power of two 2^up that puts the largest finite |v| at 2^8 (values under 2^-92: less): sums of 64 weighted values stay under 2^15.
+  // The weights carry it (as far as they can without leaving bf16's range; the rest, where values are beyond 2^60, the stores).
+  float upw = HALF ? 0.f : -DOWN, ups = 1.f;
   if constexpr (HALF) {
     if (tid == 0) vmax = 0;
     typedef unsigned short us2 __attribute__((ext_vector_type(2)));
@@ -1117,7 +1121,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
     if (top) atomicMax(&vmax, top);
     __syncthreads();
     const int e = (int)(vmax >> 7) - 127;          // floor(log2 of the largest); -127: zeros, or not normal
-    const int up = vmax ? min(8 - e, 120) : 0;
+    const int up = vmax ? min(8 - e, 100) : 0;
     const int uw = max(up, -60);
     upw = (float)uw;
     ups = __uint_as_float((unsigned)(up - uw + 127) << 23);  // (up - uw >= -59)
@@ -1143,7 +1147,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
   const float scale = fabsf(a.scale) * 1.44269504088896340736f;
   const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
   const bool all = ok == ~0ull >> (64 - KEYS);  // no key is masked: uniform
-  const float downw = __builtin_amdgcn_exp2f(-upw);  // (a whole power: exact)
+  const float downw = __builtin_amdgcn_exp2f(-upw);  // (a whole power: exact; 1 for fp16 tensors)
   t8 one;
 #pragma unroll
   for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
@@ -1256,7 +1260,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
     f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < KS; ++x) lsum = Vec<T>::mfma(one, pf[x], lsum);
-    const float l = HALF ? lsum[0] * downw : lsum[0];
+    const float l = DOWN ? lsum[0] * downw : lsum[0];
     f32x4 o[DV16];
 #pragma unroll
     for (int d = 0; d < DV16; ++d) {
@@ -1272,7 +1276,9 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
 #pragma unroll
       for (int d = 0; d < DV16; ++d) {
         const int c = channel(d, 4 * g);
-        const u32x2 y = {Vec<T>::pack(o[d][0] * inv, o[d][1] * inv), Vec<T>::pack(o[d][2] * inv, o[d][3] * inv)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] = o[d][e] * inv * (float)(1 << DOWN);
+        const u32x2 y = {Vec<T>::pack(o[d][0], o[d][1]), Vec<T>::pack(o[d][2], o[d][3])};
         if (c < a.dv) *reinterpret_cast<u32x2*>(dst + (c >> 3) * a.o.sc + (c & 7)) = y;
       }
       continue;
@@ -1344,7 +1350,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
     for (int u = 0; u < U; ++u) {
       if (l[u] == 0.f) continue;
       sum += w[u] * l[u];
-      const float x = HALF ? __builtin_amdgcn_ldexpf(w[u], ve[u]) : w[u];
+      const float x = HALF ? __builtin_amdgcn_ldexpf(w[u], ve[u] - Vec<T>::down) : w[u];
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] += x * (float)y[u][e];
     }
@@ -1352,7 +1358,7 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   t8 y;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv);
+  for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv * (float)(1 << Vec<T>::down));
   *reinterpret_cast<t8*>(head_ptr<T>(a, a.o, bh / a.kv, i, bh % a.kv * a.group + gh) + (c >> 3) * a.o.sc) = y;
 }
 
