@@ -274,7 +274,7 @@ def lib() -> C.CDLL:
     L.yl_mx4_linear_workspace_bytes.argtypes = [i32, i64, i64, i64]
     L.yl_mx4_linear.restype = i32
     L.yl_mx4_linear.argtypes = [vp, vp, i32, i64, i64, vp, vp, i64, i64, vp, i32, vp, i64, vp, i32, i64, vp, i64, vp]
-    hp = C.POINTER(Heads)
+    hp = vp  # a yl_heads: byref(Heads), or its 32 bytes
     L.yl_block_select_workspace_bytes.restype = i64
     L.yl_block_select_workspace_bytes.argtypes = [i32] * 7
     L.yl_block_select.restype = i32

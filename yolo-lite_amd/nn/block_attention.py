@@ -12,7 +12,7 @@ current stream of the tensors' device; inference only, no autograd.
 """
 from __future__ import annotations
 
-from ctypes import byref
+import struct
 from typing import Optional
 
 import torch
@@ -23,27 +23,39 @@ from ._face import call, on_gpu
 _TYPES = {torch.bfloat16: _lib.YL_BF16, torch.float16: _lib.YL_F16}
 
 
+_pack = struct.Struct("Pqqq").pack  # a yl_heads
+
+
 def _heads(t: torch.Tensor):
-    """A tensor (batch, tokens, heads, width) the kernels can read in place, copied only where it is not one; and its strides."""
-    if t.data_ptr() % 16 or (t.stride(3) != 1 and t.shape[3] > 1) or any(s % 8 for s in t.stride()[:3]):
+    """A tensor (batch, tokens, heads, width) the kernels can read in place, copied only where it is not one; and its yl_heads."""
+    at, (b, n, h, c) = t.data_ptr(), t.stride()
+    if at & 15 or (b | n | h) & 7 or (c != 1 and t.shape[3] > 1):
         t = t.clone(memory_format=torch.contiguous_format)
-    return t, _lib.Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+        at, (b, n, h, c) = t.data_ptr(), t.stride()
+    return t, _pack(at, b, n, h)
 
 
 def _check(what: str, q: torch.Tensor, k: torch.Tensor, mask: Optional[torch.Tensor]):
+    """-> the sizes batch, nq, heads, dk, nk, kv heads; and the mask as rows of bytes, its address and row stride."""
     if q.dtype not in _TYPES or k.dtype != q.dtype:
         raise TypeError(f"{what}: q and k are both bf16 or both fp16, got {q.dtype} and {k.dtype}")
-    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"{what}: q (batch, nq, heads, dk) and k (batch, nk, kv heads, dk) are needed, got {tuple(q.shape)} and {tuple(k.shape)}")
-    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f"{what}: {q.shape[2]} query heads for {k.shape[2]} kv heads")
-    if mask is None:
-        return None
-    if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (k.shape[0], k.shape[1]):
-        raise ValueError(f"{what}: a mask is (batch, nk) in bool or uint8, got {tuple(mask.shape)} in {mask.dtype}")
-    if mask.shape[1] > 1 and mask.stride(1) != 1 or mask.shape[0] > 1 and mask.stride(0) < mask.shape[1]:
-        mask = mask.contiguous()
-    return mask
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[3] != ks[3]:
+        raise ValueError(f"{what}: q (batch, nq, heads, dk) and k (batch, nk, kv heads, dk) are needed, got {tuple(qs)} and {tuple(ks)}")
+    batch, nq, heads, dk = qs
+    nk, kv = ks[1], ks[2]
+    if kv == 0 or heads == 0 or heads % kv:
+        raise ValueError(f"{what}: {heads} query heads for {kv} kv heads")
+    at = row = None
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (batch, nk):
+            raise ValueError(f"{what}: a mask is (batch, nk) in bool or uint8, got {tuple(mask.shape)} in {mask.dtype}")
+        row, one = mask.stride()
+        if nk > 1 and one != 1 or batch > 1 and row < nk:
+            mask = mask.contiguous()
+            row = nk
+        at = mask.data_ptr()
+    return qs, nk, kv, mask, at, row or 0
 
 
 def _workspace(what: str, nbytes: int, like: torch.Tensor):
@@ -57,18 +69,15 @@ def block_select(q: torch.Tensor, k: torch.Tensor, block: int = 64, topk: int = 
     (batch, kv heads, nq, topk): ascending block indices, -1 behind the last.  Score: (q summed over the kv head's query heads) .
     (mean of the block's readable keys), in 64 bits; ties go to the lower index; a block without a readable key is never picked."""
     dev = on_gpu("block_select", q, k, mask)
-    mask = _check("block_select", q, k, mask)
-    batch, nq, heads, dk = q.shape
-    nk, kv = k.shape[1], k.shape[2]
+    (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_select", q, k, mask)
     L = _lib.lib()
     nbytes = L.yl_block_select_workspace_bytes(batch, nq, nk, heads, kv, dk, block)
     work = _workspace("block_select", nbytes, q)
     q, qh = _heads(q)
     k, kh = _heads(k)
     picked = q.new_empty((batch, kv, nq, topk), dtype=torch.int32)
-    call(dev, L.yl_block_select, "block_select", byref(qh), byref(kh), _TYPES[q.dtype], batch, nq, nk, heads, kv, dk, block, topk,
-         mask.data_ptr() if mask is not None else None, mask.stride(0) if mask is not None else 0, picked.data_ptr(),
-         work.data_ptr() if work is not None else None, nbytes)
+    call(dev, L.yl_block_select, "block_select", qh, kh, _TYPES[q.dtype], batch, nq, nk, heads, kv, dk, block, topk, mask_at, mask_row,
+         picked.data_ptr(), work.data_ptr() if work is not None else None, nbytes)
     return picked
 
 
@@ -79,14 +88,13 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, picked: t
     picked: int32 (batch, kv heads, nq, topk), as ``block_select`` gives it; entries that name no block are skipped and a block
     named twice counts once.  A query without a readable key gets zeros."""
     dev = on_gpu("block_attention", q, k, v, picked, mask)
-    mask = _check("block_attention", q, k, mask)
-    batch, nq, heads, dk = q.shape
-    nk, kv = k.shape[1], k.shape[2]
-    if v.dtype != q.dtype or v.dim() != 4 or v.shape[:3] != k.shape[:3]:
-        raise ValueError(f"block_attention: v (batch, nk, kv heads, dv) in q's type is needed, got {tuple(v.shape)} in {v.dtype}")
-    if picked.dtype != torch.int32 or picked.dim() != 4 or picked.shape[:3] != (batch, kv, nq):
-        raise ValueError(f"block_attention: picked (batch, kv heads, nq, topk) in int32 is needed, got {tuple(picked.shape)} in {picked.dtype}")
-    dv, topk = v.shape[3], picked.shape[3]
+    (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_attention", q, k, mask)
+    vs, ps = v.shape, picked.shape
+    if v.dtype != q.dtype or len(vs) != 4 or vs[:3] != (batch, nk, kv):
+        raise ValueError(f"block_attention: v (batch, nk, kv heads, dv) in q's type is needed, got {tuple(vs)} in {v.dtype}")
+    if picked.dtype != torch.int32 or len(ps) != 4 or ps[:3] != (batch, kv, nq):
+        raise ValueError(f"block_attention: picked (batch, kv heads, nq, topk) in int32 is needed, got {tuple(ps)} in {picked.dtype}")
+    dv, topk = vs[3], ps[3]
     L = _lib.lib()
     nbytes = L.yl_block_attention_workspace_bytes(_TYPES[q.dtype], batch, nq, nk, heads, kv, dk, dv, block, topk)
     work = _workspace("block_attention", nbytes, q)
@@ -95,8 +103,8 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, picked: t
     v, vh = _heads(v)
     picked = picked.contiguous()
     out = q.new_empty((batch, nq, heads, dv))
-    oh = _lib.Heads(out.data_ptr(), out.stride(0), out.stride(1), out.stride(2))
-    call(dev, L.yl_block_attention, "block_attention", byref(qh), byref(kh), byref(vh), _TYPES[q.dtype], batch, nq, nk, heads, kv, dk, dv,
-         block, topk, picked.data_ptr(), mask.data_ptr() if mask is not None else None, mask.stride(0) if mask is not None else 0,
-         dk ** -0.5 if scale is None else float(scale), byref(oh), work.data_ptr() if work is not None else None, nbytes)
+    oh = _pack(out.data_ptr(), nq * heads * dv, heads * dv, dv)
+    call(dev, L.yl_block_attention, "block_attention", qh, kh, vh, _TYPES[q.dtype], batch, nq, nk, heads, kv, dk, dv, block, topk,
+         picked.data_ptr(), mask_at, mask_row, dk ** -0.5 if scale is None else float(scale), oh,
+         work.data_ptr() if work is not None else None, nbytes)
     return out

@@ -32,7 +32,8 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     """(..., k) as (rows, k) with unit column stride; copied only where no such view exists."""
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    if x.stride(1) != 1 and x.shape[1] > 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+    (rows, cols), (step, one) = x.shape, x.stride()
+    if one != 1 and cols > 1 or rows > 1 and step < cols:
         x = x.contiguous()
     return x
 
@@ -43,9 +44,10 @@ def _dense(what: str, t: Mx4Tensor):
     kb = (cols + BLOCK - 1) // BLOCK
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise TypeError(f"{what}: codes and scales are uint8 tensors")
-    if cols < 1 or codes.shape[-1] != kb * 16 or scales.shape[-1] != kb or codes.shape[:-1] != scales.shape[:-1]:
-        raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold {cols} columns")
-    if not codes.is_contiguous() or codes.data_ptr() % 16:
+    cs, ss = codes.shape, scales.shape
+    if cols < 1 or len(ss) == 0 or ss[-1] != kb or cs != (*ss[:-1], kb * 16):
+        raise ValueError(f"{what}: codes {tuple(cs)} and scales {tuple(ss)} do not hold {cols} columns")
+    if not codes.is_contiguous() or codes.data_ptr() & 15:
         codes = codes.clone(memory_format=torch.contiguous_format)
     return codes, scales if scales.is_contiguous() else scales.contiguous()
 
