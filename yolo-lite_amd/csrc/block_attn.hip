@@ -974,6 +974,14 @@ __global__ __launch_bounds__(64) void block_lists_kernel(AttendArgs p) {
   for (int j = lane; j <= nb; j += 64) p.starts[at * (nb + 1) + j] = start[j];
 }
 
+// Where the values of channel c lie in LDS: keys in a row, the row's parts exchanged by xor with the channel -- lanes that write the
+// same two keys of eight channels 8 apart would all meet in two banks.
+template <int KEYS, int DVP>
+__device__ __forceinline__ int value_at(int c, int key) {
+  constexpr int STEP = DVP == 128 ? 8 : 16;  // keys that stay together
+  return c * (KEYS + 8) + (key ^ (((c >> 4) & (KEYS / STEP - 1)) * STEP));
+}
+
 // DIRECT: one wave per (image, kv head, query, slot, unit) straight from `picked` -- few queries, where lists would hold one entry.
 // Four workgroups on a CU where the fragments leave room (128 registers; at 131, three of them, the 128x128 map's launch took 119 instead
 // of 108 us; five spill).
@@ -1012,11 +1020,6 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
     if (!use) {
       const long long at = ((long long)bh * p.slots + tdirect * p.subs + sub) * p.mlrow + (long long)qdirect * a.group;
       for (int e = lane; e < a.group; e += 64) p.ml[at + e] = float2{ninf, 0.f};
-      if (p.slots == 1) {  // (nothing is joined: the result itself is zeros)
-        const int b0 = bh / a.kv, h0 = bh % a.kv;
-        for (int e = lane; e < a.group * a.dv; e += 64)
-          head_ptr<T>(a, a.o, b0, qdirect, h0 * a.group + e / a.dv)[e % a.dv / 8 * a.o.sc + (e & 7)] = (T)0.f;
-      }
       return;
     }
     nrows = a.group;
@@ -1031,7 +1034,6 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
   const int kn = min(min(KEYS, a.block - sub * KEYS), a.nk - k0);  // keys of this unit; <= 0: none
   const bool lok = lane < kn && (!a.mask || a.mask[b * a.mask_stride + k0 + lane]);
   const unsigned long long ok = __ballot(lok);  // the keys that may be read
-  const bool alone = DIRECT && p.slots == 1;  // a row has this one result: it is the output
   // ---- keys: fragments of the first product (row = key, 8 dims of group g).  Keys and values are asked for ahead of the lists.
   t8 kf[KT][DK32];
   const T* kb = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh;
@@ -1096,7 +1098,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
     if (it < ITEMS)
 #pragma unroll
       for (int e = 0; e < 8; ++e)  // (lower halves of a pair of words, upper halves)
-        *reinterpret_cast<unsigned*>(sVt + (c8 * 8 + e) * VP + key) =
+        *reinterpret_cast<unsigned*>(sVt + value_at<KEYS, DVP>(c8 * 8 + e, key)) =
             __builtin_amdgcn_perm(v[x][1][e >> 1], v[x][0][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
   }
   // The power of two 2^up that puts the largest finite |v| at 2^8 (values under 2^-92: less): sums of 64 weighted values stay under 2^15.
@@ -1139,8 +1141,8 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
   for (int d = 0; d < DV16; ++d)
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const T* vr = sVt + channel(d, n) * VP + s * 32 + 4 * g;
-      const t4 lo = *reinterpret_cast<const t4*>(vr), hi = *reinterpret_cast<const t4*>(vr + 16);
+      const t4 lo = *reinterpret_cast<const t4*>(sVt + value_at<KEYS, DVP>(channel(d, n), s * 32 + 4 * g));
+      const t4 hi = *reinterpret_cast<const t4*>(sVt + value_at<KEYS, DVP>(channel(d, n), s * 32 + 16 + 4 * g));
       vf[d][s] = t8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     }
   // scores are scaled by |scale| inside the exponential's fma; a negative scale flips the queries' signs
@@ -1270,19 +1272,6 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
     }
     if (!w.live) continue;
     const unsigned local = __umul24((unsigned)w.q, (unsigned)a.group) + (unsigned)w.head;  // row behind q0's first: below 4096 * 1000
-    if (alone) {
-      T* const dst = head_ptr<T>(a, a.o, b, q0 + w.q, h * a.group + w.head);
-      const float inv = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);
-#pragma unroll
-      for (int d = 0; d < DV16; ++d) {
-        const int c = channel(d, 4 * g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][e] = o[d][e] * inv * (float)(1 << DOWN);
-        const u32x2 y = {Vec<T>::pack(o[d][0], o[d][1]), Vec<T>::pack(o[d][2], o[d][3])};
-        if (c < a.dv) *reinterpret_cast<u32x2*>(dst + (c >> 3) * a.o.sc + (c & 7)) = y;
-      }
-      continue;
-    }
     part_t* const dst = pb + (long long)(__umul24(local, (unsigned)p.slots) + (unsigned)w.slot) * DVP;
     if constexpr (HALF) {
       if (ups != 1.f)
@@ -1360,6 +1349,168 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv * (float)(1 << Vec<T>::down));
   *reinterpret_cast<t8*>(head_ptr<T>(a, a.o, bh / a.kv, i, bh % a.kv * a.group + gh) + (c >> 3) * a.o.sc) = y;
+}
+
+// Few queries and blocks: one workgroup per (image, kv head, query, 16 query heads), a wave per slot and unit in turn with the running
+// maximum and sum of its softmax, joined through LDS -- one launch, no workspace.  Bound by the latency of a round (block read, transposed,
+// multiplied: 3-5 us) and by launches; 64 queries of width 128, 268 MB of blocks: 53 us, 5000 GB/s.
+template <typename T, int KEYS, int DK32, int DV16>
+__global__ __launch_bounds__(512, DK32 <= 2 && DV16 == 4 ? 4 : 2) void block_attend_few_kernel(AttendArgs p) {
+  typedef typename Vec<T>::t8 t8;
+  typedef typename Vec<T>::t4 t4;
+  constexpr int KT = KEYS / 16, KS = KEYS / 32, DVP = DV16 * 16, VP = KEYS + 8;
+  constexpr int REGION = DVP * VP * 2;  // bytes of LDS of a wave: its values, then its result: 16 rows of DVP floats, maximum and sum
+  static_assert(REGION >= 64 * DVP + 128, "a wave's result takes the place of its values");
+  extern __shared__ __attribute__((aligned(16))) unsigned char few_sm[];
+  const BlockArgs& a = p.a;
+  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), nw = (int)blockDim.x >> 6;
+  const float ninf = -__builtin_huge_valf();
+  const int gt = (a.group + 15) >> 4;
+  unsigned unit = blockIdx.x;
+  const int tile = (int)(unit % (unsigned)gt);
+  unit /= (unsigned)gt;
+  const int i = (int)(unit % (unsigned)a.nq), bh = (int)(unit / (unsigned)a.nq), h = bh % a.kv, b = bh / a.kv;
+  const int h0 = h * a.group + tile * 16, rows = min(16, a.group - tile * 16);
+  T* const sVt = reinterpret_cast<T*>(few_sm + wave * REGION);
+  const int* pick = a.picked + ((long long)bh * a.nq + i) * a.topk;
+  const float scale = fabsf(a.scale) * 1.44269504088896340736f;
+  const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
+  t8 qf[DK32];
+#pragma unroll
+  for (int c = 0; c < DK32; ++c) {
+    u32x4 x = {0, 0, 0, 0};
+    if ((c * 4 + g) * 8 < a.dk) x = *reinterpret_cast<const u32x4*>(head_ptr<const T>(a, a.q, b, i, h0 + min(n, rows - 1)) + (c * 4 + g) * a.q.sc);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) x[d] ^= flip;
+    qf[c] = __builtin_bit_cast(t8, x);
+  }
+  const T* kb = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh;
+  const T* vb = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh;
+  t8 one;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) one[e] = (T)1.f;
+  float m = ninf;
+  f32x4 l = {0.f, 0.f, 0.f, 0.f}, o[DV16];
+#pragma unroll
+  for (int d = 0; d < DV16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int slot = wave; slot < p.slots; slot += nw) {
+    const int t = p.subs == 2 ? slot >> 1 : slot, sub = p.subs == 2 ? slot & 1 : 0;
+    const int j = pick[t];
+    bool use = j >= 0 && j < a.nb;
+    for (int u = 0; u < t; ++u) use = use && pick[u] != j;
+    const int k0 = j * a.block + sub * KEYS, kn = min(min(KEYS, a.block - sub * KEYS), a.nk - k0);
+    if (!use || kn <= 0) continue;  // (the same in every lane; no barrier of the workgroup in here)
+    const bool lok = lane < kn && (!a.mask || a.mask[b * a.mask_stride + k0 + lane]);
+    const unsigned long long ok = __ballot(lok);
+    t8 kf[KT][DK32];
+#pragma unroll
+    for (int x = 0; x < KT; ++x)
+#pragma unroll
+      for (int c = 0; c < DK32; ++c) {
+        kf[x][c] = t8{};
+        if (x * 16 + n < kn && (c * 4 + g) * 8 < a.dk) kf[x][c] = *reinterpret_cast<const t8*>(kb + token(a, k0 + x * 16 + n) * a.k.st + (c * 4 + g) * a.k.sc);
+      }
+    // values: two keys x 8 channels at a time, transposed into LDS
+    constexpr int NV = KEYS / 2 * (DVP / 8) / 64;
+#pragma unroll
+    for (int x0 = 0; x0 < NV; x0 += 4) {
+      u32x4 v[4][2];
+#pragma unroll
+      for (int x = 0; x < 4 && x0 + x < NV; ++x) {
+        const int it = lane + (x0 + x) * 64, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          v[x][u] = u32x4{0, 0, 0, 0};
+          if (c8 * 8 < a.dv && (ok >> (key + u) & 1)) v[x][u] = *reinterpret_cast<const u32x4*>(vb + token(a, k0 + key + u) * a.v.st + c8 * a.v.sc);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4 && x0 + x < NV; ++x) {
+        const int it = lane + (x0 + x) * 64, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<unsigned*>(sVt + value_at<KEYS, DVP>(c8 * 8 + e, key)) =
+              __builtin_amdgcn_perm(v[x][1][e >> 1], v[x][0][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+      }
+    }
+    f32x4 s[KT];
+#pragma unroll
+    for (int x = 0; x < KT; ++x) {
+      s[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < DK32; ++c) s[x] = Vec<T>::mfma(kf[x][c], qf[c], s[x]);
+    }
+    unsigned okt = 0;  // this lane's keys x * 16 + 4 g + r, four bits per tile
+#pragma unroll
+    for (int x = 0; x < KT; ++x) okt |= (unsigned)(ok >> (x * 16 + 4 * g) & 15) << (4 * x);
+    float top = ninf;
+#pragma unroll
+    for (int x = 0; x < KT; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = okt >> (4 * x + r) & 1 ? fmaxf(top, s[x][r]) : top;
+    top = quad_max(top);
+    top = top == ninf ? top : top * scale;  // (no key: -inf, also where the scale is 0)
+    const float now = fmaxf(m, top), base = now == ninf ? 0.f : now;
+    const float fade = __builtin_amdgcn_exp2f(m - base);
+    m = now;
+    u32x4 pw[KS];
+#pragma unroll
+    for (int x = 0; x < KT; ++x)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {  // (times 2^-down, which the division by their sum takes out again)
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], scale, -base - Vec<T>::down));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r + 1], scale, -base - Vec<T>::down));
+        pw[x >> 1][(x & 1) * 2 + r / 2] = Vec<T>::pack(okt >> (4 * x + r) & 1 ? e0 : 0.f, okt >> (4 * x + r + 1) & 1 ? e1 : 0.f);
+      }
+    // (a wave's LDS accesses are carried out in order: its own writes are there)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    l *= fade;
+#pragma unroll
+    for (int x = 0; x < KS; ++x) l = Vec<T>::mfma(one, __builtin_bit_cast(t8, pw[x]), l);
+#pragma unroll
+    for (int d = 0; d < DV16; ++d) {
+      o[d] *= fade;
+#pragma unroll
+      for (int x = 0; x < KS; ++x) {
+        const t4 lo = *reinterpret_cast<const t4*>(sVt + value_at<KEYS, DVP>(d * 16 + n, x * 32 + 4 * g));
+        const t4 hi = *reinterpret_cast<const t4*>(sVt + value_at<KEYS, DVP>(d * 16 + n, x * 32 + 16 + 4 * g));
+        o[d] = Vec<T>::mfma(t8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, __builtin_bit_cast(t8, pw[x]), o[d]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (the next values come behind these reads)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  // ---- join: row n's channels 16 d + 4 g + r of every wave
+  float* const res = reinterpret_cast<float*>(sVt);
+#pragma unroll
+  for (int d = 0; d < DV16; ++d) *reinterpret_cast<f32x4*>(res + n * DVP + d * 16 + 4 * g) = o[d];
+  if (g == 0) *reinterpret_cast<float2*>(res + 16 * DVP + 2 * n) = float2{m, l[0]};
+  __syncthreads();
+  for (int item = threadIdx.x; item < rows * (DVP / 8); item += (int)blockDim.x) {
+    const int row = item / (DVP / 8), c = item % (DVP / 8) * 8;
+    if (c >= a.dv) continue;
+    float big = ninf;
+    for (int w = 0; w < nw; ++w) big = fmaxf(big, reinterpret_cast<const float*>(few_sm + w * REGION)[16 * DVP + 2 * row]);
+    const float base = big == ninf ? 0.f : big;
+    float sum = 0.f, acc[8] = {};
+    for (int w = 0; w < nw; ++w) {
+      const float* r = reinterpret_cast<const float*>(few_sm + w * REGION);
+      const float x = __builtin_amdgcn_exp2f(r[16 * DVP + 2 * row] - base), lw = r[16 * DVP + 2 * row + 1];
+      if (lw == 0.f) continue;
+      sum += x * lw;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += x * r[row * DVP + c + e];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    t8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv);
+    *reinterpret_cast<t8*>(head_ptr<T>(a, a.o, b, i, h0 + row) + (c >> 3) * a.o.sc) = y;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -1522,7 +1673,7 @@ extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, 
 
 // ---- how the attention runs: sizes, and where things lie in the workspace
 struct AttendPlan {
-  bool direct;
+  bool direct, few;
   int subs, slots, groups, range, dvp;
   int chunk;               // groups of queries whose block results are in memory together
   long long starts, lists, vexp, part, ml, all;  // byte offsets
@@ -1537,6 +1688,12 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
   p.groups = (a.nq + 63) / 64;
   // the lists pay where a block is picked often; below that, a wave per (query, block)
   p.direct = a.nq <= 4 || (long long)a.nq * a.topk <= 2LL * a.nb;
+  // One launch for one or two rounds of eight waves.  One query, 8 kv heads, blocks of 64, that launch / two launches (captured, us):
+  // width 64, 8 blocks 8.1 / 8.5, 16 blocks 10.9 / 10.1, 32 blocks 17.6 / 13.7; width 128, 8 blocks 12.2 / 10.3, 16 blocks 17.9 / 12.2;
+  // a call of its own is 3 us less for the host.  With many queries it wins further (32 images, width 128, 16 blocks 26 / 32; 16 images with
+  // 4 query heads to one 20 / 22), but for 2048 workgroups of one round (55 / 47).
+  p.few = p.direct && (p.slots * p.dvp <= 1024 || (p.slots <= 16 && (long long)a.batch * a.kv * a.nq >= 128));
+  if (p.few) return p;  // (one launch, no workspace)
   // a workgroup's range of queries: about 512 (query, head) rows, 32 tiles, for an average block
   const long long per64 = 64LL * a.topk * a.group;
   p.range = (int)std::min<long long>(64, std::max<long long>(1, 512LL * std::max(1, a.nb) / per64));
@@ -1559,15 +1716,23 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
   p.vexp = take((long long)a.batch * a.kv * std::max(1, a.nb) * p.subs);
   p.ml = take(8 * rows * p.slots);
   const long long cq = p.direct ? a.nq : 64LL * p.chunk;
-  p.part = take(p.slots == 1 && p.direct ? 0 : (long long)part_bytes * a.batch * a.heads * cq * p.slots * p.dvp);
+  p.part = take((long long)part_bytes * a.batch * a.heads * cq * p.slots * p.dvp);
   p.all = at;
   return p;
 }
 
 template <typename T, int KEYS, int DK32, int DV16>
-static int attend_launch(const AttendArgs& p, bool direct, hipStream_t s) {
+static int attend_launch(const AttendArgs& p, bool direct, bool few, hipStream_t s) {
   const BlockArgs& a = p.a;
   const long long bh = (long long)a.batch * a.kv;
+  if (few) {
+    const int nw = std::min(8, p.slots), lds = nw * DV16 * 16 * (KEYS + 8) * 2;
+    auto kern = block_attend_few_kernel<T, KEYS, DK32, DV16>;
+    if (int rc = allow_big_lds(reinterpret_cast<const void*>(kern), 8 * DV16 * 16 * (KEYS + 8) * 2)) return rc;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(bh * a.nq * ((a.group + 15) / 16))), dim3(64 * nw), lds, s, p);  // (no more than the rows)
+    YL_HIP(hipGetLastError());
+    return 0;
+  }
   const long long wg = direct ? bh * a.nq * a.topk * p.subs : bh * p.nrange * a.nb * p.subs;
   if (wg > 0x7FFFFFFFLL) return fail(-3, "block_attention: more blocks and queries than one launch covers");
   if (direct)
@@ -1578,11 +1743,11 @@ static int attend_launch(const AttendArgs& p, bool direct, hipStream_t s) {
   return 0;
 }
 template <typename T, int KEYS>
-static int attend_by_width(const AttendArgs& p, bool direct, hipStream_t s) {
+static int attend_by_width(const AttendArgs& p, bool direct, bool few, hipStream_t s) {
   const int dk = p.a.dk;
   if (p.a.dv <= 64)
-    return dk <= 32 ? attend_launch<T, KEYS, 1, 4>(p, direct, s) : dk <= 64 ? attend_launch<T, KEYS, 2, 4>(p, direct, s) : attend_launch<T, KEYS, 4, 4>(p, direct, s);
-  return dk <= 32 ? attend_launch<T, KEYS, 1, 8>(p, direct, s) : dk <= 64 ? attend_launch<T, KEYS, 2, 8>(p, direct, s) : attend_launch<T, KEYS, 4, 8>(p, direct, s);
+    return dk <= 32 ? attend_launch<T, KEYS, 1, 4>(p, direct, few, s) : dk <= 64 ? attend_launch<T, KEYS, 2, 4>(p, direct, few, s) : attend_launch<T, KEYS, 4, 4>(p, direct, few, s);
+  return dk <= 32 ? attend_launch<T, KEYS, 1, 8>(p, direct, few, s) : dk <= 64 ? attend_launch<T, KEYS, 2, 8>(p, direct, few, s) : attend_launch<T, KEYS, 4, 8>(p, direct, few, s);
 }
 
 extern "C" int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block,
@@ -1613,12 +1778,12 @@ static int attend_run(AttendArgs& p, const AttendPlan& pl, int dtype, char* w, h
   }
   return by_type16(dtype, [&](auto* t) {
     typedef BA_T(t) T;
+    if (pl.few) return block == 32 ? attend_by_width<T, 32>(p, true, true, s) : attend_by_width<T, 64>(p, true, true, s);
     for (int g0 = 0; g0 < pl.groups; g0 += pl.chunk) {
       p.g0 = g0, p.gn = std::min(pl.chunk, pl.groups - g0);
       p.nrange = (p.gn + pl.range - 1) / pl.range;
       if (a.nb > 0 || pl.direct)
-        if (int rc = block == 32 ? attend_by_width<T, 32>(p, pl.direct, s) : attend_by_width<T, 64>(p, pl.direct, s)) return rc;
-      if (pl.slots == 1 && pl.direct) return 0;
+        if (int rc = block == 32 ? attend_by_width<T, 32>(p, pl.direct, false, s) : attend_by_width<T, 64>(p, pl.direct, false, s)) return rc;
       const long long items = (long long)batch * std::min(64 * p.gn, nq - 64 * g0) * heads * (pl.dvp / 8);
       const dim3 grid((unsigned)((items + 255) / 256));
       typedef typename Vec<T>::part P;
@@ -1649,7 +1814,7 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
     return fail(-1, "block_attention: out has a stride of 0");
   if (!picked) return fail(-1, "block_attention: null pointer");
   const AttendPlan pl = plan_attend(a, dv, dtype);
-  if (!work || work_bytes < pl.all || (reinterpret_cast<uintptr_t>(work) & 15))
+  if (pl.all > 0 && (!work || work_bytes < pl.all || (reinterpret_cast<uintptr_t>(work) & 15)))
     return fail(-1, "block_attention: workspace missing, too small or not 16-byte aligned");
   if (nk > 0) a.v = Heads{v->data, v->batch, v->token, v->head, 8};
   a.o = Heads{out->data, out->batch, out->token, out->head, 8};
