@@ -1692,7 +1692,13 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
   // width 64, 8 blocks 8.1 / 8.5, 16 blocks 10.9 / 10.1, 32 blocks 17.6 / 13.7; width 128, 8 blocks 12.2 / 10.3, 16 blocks 17.9 / 12.2;
   // a call of its own is 3 us less for the host.  With many queries it wins further (32 images, width 128, 16 blocks 26 / 32; 16 images with
   // 4 query heads to one 20 / 22), but for 2048 workgroups of one round (55 / 47).
-  p.few = p.direct && (p.slots * p.dvp <= 1024 || (p.slots <= 16 && (long long)a.batch * a.kv * a.nq >= 128));
+  const long long wgs = (long long)a.batch * a.kv * a.nq * ((a.group + 15) / 16);
+  const int work = std::min(a.topk, std::max(1, a.nb)) * p.subs;  // slots that can name a block of their own
+  // ... and in place of the lists where queries times blocks are so few that sharing keys saves less than the launches cost (one launch /
+  // lists, call): 400 queries x 2 heads x 4 blocks 11.2 / 19.7, 64 x 8 x 16 18.6 / 22.8, 128 x 8 x 8 20.5 / 19.1; 256 queries, 32 heads over 2,
+  // 8 blocks 11.7 / 28.4; width 128: 32 x 8 x 8 15.8 / 16.1, 64 x 8 x 16 38.6 / 35.2.
+  p.few = (p.direct || wgs * work * p.dvp <= 1 << 19) && (work * p.dvp <= 1024 || (work <= 16 && wgs >= 128));
+  p.direct = p.direct || p.few;
   if (p.few) return p;  // (one launch, no workspace)
   // a workgroup's range of queries: about 512 (query, head) rows, 32 tiles, for an average block
   const long long per64 = 64LL * a.topk * a.group;
