@@ -20,6 +20,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BA_MAX_BLOCKS = 4096;  // key blocks per image: scores of a row in the registers of 8 (many queries) or 16 waves
 constexpr int BA_MAX_TOPK = 64;
+constexpr int SCORE_MAX_NQ = 4;      // so few queries are scored by the wave that has the mean
 
 // Over the four lanes that share lane & 15 (an MFMA column): v_permlane32_swap / v_permlane16_swap of a register with itself leave
 // the two halves' (row pairs') values side by side -- no LDS round trip.
@@ -98,14 +99,12 @@ __device__ __forceinline__ long long split_at(const BlockArgs& a, int bh, int j,
 // lanes of a dim chunk exchange halves, then quarters, ... of their sums, so a wave reduces with 7 exchanges instead of 24.
 // SCORE: few queries -- the wave that has a block's mean also scores it, and no mean is stored.
 // Bound by reading the keys: 8 heads x 65536 keys of 64 (67 MB) 18 us, 3700 GB/s, this card's rate for reading alone.
+// That wave's part: score[i * step] of the queries, *count keys.
 template <typename T, int CP, bool SCORE>
-__global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
+__device__ __forceinline__ void block_mean(const BlockArgs& a, int bh, int j, int lane, double* score, int step, int* count) {
   typedef T t8 __attribute__((ext_vector_type(8)));
   constexpr int KL = 64 / CP;
-  const int lane = threadIdx.x & 63;
-  const unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6);  // (below 2^31, as the blocks are: no 64-bit division)
-  if (unit >= (unsigned)(a.batch * a.kv * a.nb)) return;
-  const int bh = (int)(unit / (unsigned)a.nb), j = (int)(unit - (unsigned)bh * (unsigned)a.nb), h = bh % a.kv, b = bh / a.kv;
+  const int h = bh % a.kv, b = bh / a.kv;
   const int c = lane % CP, kl = lane / CP;
   const int k0 = j * a.block, kn = min(a.block, a.nk - k0);
   const T* kp = static_cast<const T*>(a.k.p) + b * a.k.sb + h * a.k.sh + c * a.k.sc;
@@ -166,9 +165,9 @@ __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
         }
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) s += shfl_xor_d(s, o);
-      if (lane == 0) a.score[((long long)bh * a.nq + i) * a.nb + j] = n ? s : __builtin_nan("");
+      if (lane == 0) score[(long long)i * step] = n ? s : __builtin_nan("");
     }
-    if (lane == 0 && h == 0) a.count[b * a.nb + j] = n;
+    if (lane == 0 && count) *count = n;
   } else {
     float norm = 0.f;
     if (mine)
@@ -192,9 +191,17 @@ __global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
     }
     if (lane == 0) {
       a.norm[(long long)bh * a.nb + j] = sqrtf(norm);
-      if (h == 0) a.count[b * a.nb + j] = n;
+      if (count) *count = n;
     }
   }
+}
+template <typename T, int CP, bool SCORE>
+__global__ __launch_bounds__(256) void block_mean_kernel(BlockArgs a) {
+  const unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6);  // (below 2^31, as the blocks are: no 64-bit division)
+  if (unit >= (unsigned)(a.batch * a.kv * a.nb)) return;
+  const int bh = (int)(unit / (unsigned)a.nb), j = (int)(unit - (unsigned)bh * (unsigned)a.nb);
+  block_mean<T, CP, SCORE>(a, bh, j, threadIdx.x & 63, SCORE ? a.score + (long long)bh * a.nq * a.nb + j : nullptr, a.nb,
+                           bh % a.kv == 0 ? a.count + (bh / a.kv) * a.nb + j : nullptr);
 }
 
 // ------------------------------------------------------------------------------------------------ selection
@@ -373,6 +380,22 @@ __global__ __launch_bounds__(64 * NW) void block_select_kernel(BlockArgs a) {
 #pragma unroll
   for (int x = 0; x < NI; ++x) key[x] = order_key(s[x], n[x] > 0);
   pick_row(key, a.topk, ws, a.picked + row * a.topk);
+}
+
+// Few queries and up to 16 short blocks, one to a wave: one workgroup per (image, kv head) does both, in one launch.  Call, one launch / two:
+// one query, 8 kv heads, 7 blocks of 64 x 64 10.2 / 12.7 us, 16 blocks 10.2 / 13.1; two blocks to a wave 18.8 / 13.0, and 30.9 / 13.3 of 128 x 128.
+constexpr int SMALL_BLOCKS = 16, SMALL_BLOCK = 64 * 128;
+template <typename T, int CP>
+__global__ __launch_bounds__(1024) void block_select_small_kernel(BlockArgs a) {
+  __shared__ double score[SCORE_MAX_NQ][SMALL_BLOCKS];
+  __shared__ int count[SMALL_BLOCKS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bh = (int)blockIdx.x;
+  if (wave < a.nb) block_mean<T, CP, true>(a, bh, wave, lane, &score[0][wave], SMALL_BLOCKS, &count[wave]);
+  __syncthreads();
+  if (wave >= a.nq) return;
+  Waves<1> ws{nullptr, lane, 0, 0};
+  const unsigned long long key[1] = {lane < a.nb ? order_key(score[wave][lane], count[lane] > 0) : 0};
+  pick_row(key, a.topk, ws, a.picked + ((long long)bh * a.nq + wave) * a.topk);
 }
 
 // Scores of 16 queries with the means of blocks 16 t0 .. 16 (t0 + NT) on the matrix pipe: lane (query n, group g) gets those of
@@ -1572,7 +1595,6 @@ static int by_type16(int dtype, F f) {
 using namespace yl;
 
 // ---- how the selection runs, and where things lie in the workspace
-constexpr int SCORE_MAX_NQ = 4;  // so few queries are scored by the wave that has the mean
 struct SelectPlan {
   long long mean, score, split, norm, count, all;  // byte offsets
 };
@@ -1603,11 +1625,15 @@ extern "C" int64_t yl_block_select_workspace_bytes(int batch, int nq, int nk, in
   return batch * (long long)nq == 0 ? 0 : plan_select(&a).all;
 }
 
-template <typename T, bool SCORE>
+template <typename T, bool SCORE, bool SMALL = false>
 static int mean_launch(const BlockArgs& a, hipStream_t s) {
   const long long wg = ((long long)a.batch * a.kv * a.nb + 3) / 4;
-  const int c = a.dk / 8;
-#define BA_MEAN(CP) hipLaunchKernelGGL((block_mean_kernel<T, CP, SCORE>), dim3((unsigned)wg), dim3(256), 0, s, a)
+  const int c = a.dk / 8, nw = std::max(SCORE_MAX_NQ, a.nb);
+#define BA_MEAN(CP)                                                                                                           \
+  do {                                                                                                                        \
+    if constexpr (SMALL) hipLaunchKernelGGL((block_select_small_kernel<T, CP>), dim3(a.batch * a.kv), dim3(64 * nw), 0, s, a);   \
+    else hipLaunchKernelGGL((block_mean_kernel<T, CP, SCORE>), dim3((unsigned)wg), dim3(256), 0, s, a);                           \
+  } while (0)
   if (c <= 1) BA_MEAN(1);
   else if (c <= 2) BA_MEAN(2);
   else if (c <= 4) BA_MEAN(4);
@@ -1650,6 +1676,7 @@ static int select_run(BlockArgs& a, const SelectPlan& p, int dtype, char* w, hip
   return by_type16(dtype, [&](auto* t) {
     typedef BA_T(t) T;
     const bool few = a.nq <= SCORE_MAX_NQ;
+    if (few && a.nb <= SMALL_BLOCKS && std::min(a.block, a.nk) * a.dk <= SMALL_BLOCK) return mean_launch<T, true, true>(a, s);
     if (a.nb > 0)
       if (int rc = few ? mean_launch<T, true>(a, s) : mean_launch<T, false>(a, s)) return rc;
     if (!few && a.nb > 0) return score_by_size<T>(a, s);
