@@ -365,7 +365,8 @@ int yl_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
  * fp32 accumulation, act = 1: SiLU.  x: values (x_dtype YL_BF16 / YL_F16 / YL_F32, x_scales ignored), quantised by the call into
  * `work`, or x_dtype = YL_MX4: codes with x_scales (x_stride ignored: codes and scales are dense).  bias fp32 or NULL; res has
  * y's type, NULL: none; res may be y itself.  Strides in elements; y_dtype YL_BF16 / YL_F16 / YL_F32.  `work`: 16-byte aligned
- * device scratch of yl_mx4_linear_workspace_bytes bytes (-1: the sizes are refused), not shared by calls that may overlap. */
+ * device scratch of yl_mx4_linear_workspace_bytes bytes (-1: the sizes are refused; 0: none is needed, NULL then), not shared by
+ * calls that may overlap. */
 int64_t yl_mx4_linear_workspace_bytes(int x_dtype, int64_t rows, int64_t n, int64_t k);
 int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype, int64_t rows, int64_t x_stride, const uint8_t* w_codes,
                   const uint8_t* w_scales, int64_t n, int64_t k, const float* bias, int act, const void* res, int64_t res_stride,
@@ -394,7 +395,7 @@ int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, int batch, 
                     void* stream);
 /* out[b][i][h] = softmax over the readable keys of the blocks picked[b][h's kv head][i] of (scale * q . k), times v.  Entries of
  * `picked` outside [0, blocks) are no block; a block named twice counts once; the order does not matter.  fp32 accumulation.
- * `work` as above, yl_block_attention_workspace_bytes bytes. */
+ * `work` as above, yl_block_attention_workspace_bytes bytes (0 where none is needed: NULL then). */
 int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block,
                                            int topk);
 int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl_heads* v, int dtype, int batch, int nq, int nk, int heads,

@@ -887,10 +887,10 @@ __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, 
 // tile -- S^T = K Q^T, softmax over the block, O^T = V^T P^T, where the S^T accumulators of two 16-key tiles are, after exp2, the B
 // fragment of the second product -- and writes the block's result of each row with its maximum and sum; a second launch
 // joins a row's blocks.  Keys are read once per block and range of queries instead of once per query; the price is that every (row,
-// block) result passes through memory, which is what bounds the stage (2 (dv + 4) bytes written and read per row and block).  Measured, lists / blocks / join: 16384 queries, 8 heads
-// over 2, 16 blocks of 64 9.5 / 106 / 57 us (17 GMAC: 330 TFLOP/s; 270 MB of block results, read by the join at 4700 GB/s); 8 images x 1600
-// queries x 6 heads x 8 blocks 7 / 38 / 17 us.  The middle launch issues about 210 vector instructions to a tile of 16 rows x 64 keys beside 18
-// MFMAs, 16 of them exponentials at a quarter of the rate.
+// block) result passes through memory, which is what bounds the stage (2 (dv + 4) bytes written and read per row and block).
+// Measured, lists / blocks / join: 16384 queries, 8 heads over 2, 16 blocks of 64 9.5 / 106 / 57 us (17 GMAC: 330 TFLOP/s; 270 MB of block
+// results, read by the join at 4700 GB/s); 8 images x 1600 queries x 6 heads x 8 blocks 7 / 38 / 17 us.  The middle launch issues about 210
+// vector instructions to a tile of 16 rows x 64 keys beside 18 MFMAs, 16 of them exponentials at a quarter of the rate.
 //
 // A block's results pass unnormalised (sum of p v; the maximum and sum of p beside them in fp32).  For fp16 tensors they are fp32.  For
 // bf16 tensors they are fp16, toward zero (2^-10 at most, a quarter of a bf16 step; fp32 took 278 instead of 150 us on the 128x128
@@ -1784,9 +1784,12 @@ static int attend_launch(const AttendArgs& p, bool direct, bool few, hipStream_t
 template <typename T, int KEYS>
 static int attend_by_width(const AttendArgs& p, bool direct, bool few, hipStream_t s) {
   const int dk = p.a.dk;
-  if (p.a.dv <= 64)
-    return dk <= 32 ? attend_launch<T, KEYS, 1, 4>(p, direct, few, s) : dk <= 64 ? attend_launch<T, KEYS, 2, 4>(p, direct, few, s) : attend_launch<T, KEYS, 4, 4>(p, direct, few, s);
-  return dk <= 32 ? attend_launch<T, KEYS, 1, 8>(p, direct, few, s) : dk <= 64 ? attend_launch<T, KEYS, 2, 8>(p, direct, few, s) : attend_launch<T, KEYS, 4, 8>(p, direct, few, s);
+  if (p.a.dv <= 64) {
+    if (dk <= 32) return attend_launch<T, KEYS, 1, 4>(p, direct, few, s);
+    return dk <= 64 ? attend_launch<T, KEYS, 2, 4>(p, direct, few, s) : attend_launch<T, KEYS, 4, 4>(p, direct, few, s);
+  }
+  if (dk <= 32) return attend_launch<T, KEYS, 1, 8>(p, direct, few, s);
+  return dk <= 64 ? attend_launch<T, KEYS, 2, 8>(p, direct, few, s) : attend_launch<T, KEYS, 4, 8>(p, direct, few, s);
 }
 
 extern "C" int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block,

@@ -18,8 +18,6 @@ namespace yl {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef int v4i __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 
 // ------------------------------------------------------------------------------------------------ element access
 template <typename T>
