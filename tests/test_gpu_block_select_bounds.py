@@ -1,0 +1,57 @@
+"""GPU: the selection equals the 64-bit one where the scores in fewer bits say least.  The restatement sorts 64-bit scores; nothing is
+rounded but its sums."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _select64(q, k, block, topk):
+    """(b, kv, nq, topk) from the definition, on the CPU in 64 bits."""
+    q, k = q.double().cpu(), k.double().cpu()
+    b, nq, heads, dk = q.shape
+    nk, kv = k.shape[1:3]
+    nb = -(-nk // block)
+    mean = torch.stack([k[:, j * block: (j + 1) * block].mean(1) for j in range(nb)], 2)  # (b, kv, nb, dk)
+    score = torch.matmul(q.view(b, nq, kv, heads // kv, dk).sum(3).permute(0, 2, 1, 3).contiguous(), mean.transpose(2, 3).contiguous())
+    order = torch.sort(score, dim=-1, descending=True, stable=True).indices[..., :topk]
+    return torch.nn.functional.pad(order.sort(-1).values, (0, topk - order.shape[-1]), value=-1)
+
+
+def _check(q, k, block, topk):
+    import yololite_amd as ya
+
+    got = ya.block_select(q, k, block=block, topk=topk).cpu().long()
+    wrong = (got != _select64(q, k, block, topk)).any(-1)
+    assert not bool(wrong.any()), f"{int(wrong.sum())} of {wrong.numel()} queries"
+
+
+# blocks and queries for each way the scores are made: a wave up to 64, 128, 256 blocks, four and eight waves
+WAYS = [(60, 300), (100, 300), (200, 300), (200, 32768), (400, 300), (400, 9000), (1000, 300), (2000, 100), (4000, 60)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("nb, nq", WAYS)
+def test_heads_that_cancel(gpu_device, nb, nq, dtype):
+    """Heads a, s, -a, t with |s|, |t| = 2^-14 .. 2^-24 of |a|: the sum is s + t, what fp32 makes of it on the way is not."""
+    g = torch.Generator().manual_seed(nb + nq)
+    dk, block = 64, 32
+    k = torch.randn(1, nb * block, 1, dk, generator=g).to(TYPES[dtype])
+    a = 16 * torch.randn(1, nq, 1, dk, generator=g)
+    ratio = 2.0 ** -torch.linspace(14, 24, nq).view(1, nq, 1, 1)
+    s, t = (16 * ratio * torch.randn(1, nq, 1, dk, generator=g) for _ in range(2))
+    q = torch.cat((a, s, -a, t), 2).to(TYPES[dtype])
+    _check(q.to(gpu_device), k.to(gpu_device), block, 8)
+
+
+@pytest.mark.parametrize("heads", [2, 3, 7])
+def test_other_numbers_of_heads_that_cancel(gpu_device, heads):
+    g = torch.Generator().manual_seed(heads)
+    nq, dk = 1000, 64
+    k = torch.randn(1, 100 * 32, 1, dk, generator=g).bfloat16()
+    a = torch.randn(1, nq, 1, dk, generator=g).bfloat16().float()
+    s = 2.0 ** -20 * torch.randn(1, nq, heads - 1, dk, generator=g)
+    q = torch.cat((a, s), 2)
+    q[:, :, -1] += -a[:, :, 0] * (1 + 2.0 ** -7 * (heads == 2))
+    _check(q.bfloat16().to(gpu_device), k.to(gpu_device), 32, 8)

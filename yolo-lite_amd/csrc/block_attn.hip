@@ -10,6 +10,7 @@
 // Which block wins must not depend on the order of a sum: scores are 64-bit (a mean of bf16 / fp16 values in 64 bits is exact up to
 // its division, and two blocks that are not equal differ by far more than 2^-50 of a score).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "conv_common.h"
@@ -68,6 +69,7 @@ struct BlockArgs {
   __bf16* split;  // the means as two bf16, in the order the matrix pipe takes them (split_at); nbp = nb rounded up to 16, dkp = dk to 32
   float* norm;    // [batch][kv][nb]: 2-norm of a mean
   int nbp, dkp;
+  float head_err; // what the fp32 sum of a group's query heads may be off by, relative to the 2-norm over all of them
   unsigned magic; // 2^32 / group, rounded up: f / group = mulhi(f, magic) for f * group < 2^32
   int* count;     // [batch][nb]: unmasked keys of a block
   int* picked;    // [batch][kv][nq][topk]
@@ -399,14 +401,15 @@ __global__ __launch_bounds__(1024) void block_select_small_kernel(BlockArgs a) {
 }
 
 // Scores of 16 queries with the means of blocks 16 t0 .. 16 (t0 + NT) on the matrix pipe: lane (query n, group g) gets those of
-// blocks 16 (t0 + t) + 4 g + r, and its share of the query's squared norm.  qp: the query's first head; bh: its means.
+// blocks 16 (t0 + t) + 4 g + r, and its share of the squared norms of the query (qq) and of all its heads (hh).  qp: the query's first
+// head; bh: its means.
 template <typename T, int NT>
-__device__ __forceinline__ void score_tiles(const BlockArgs& a, int bh, const T* qp, int t0, int lane, f32x4 (&s)[NT], float& qq) {
+__device__ __forceinline__ void score_tiles(const BlockArgs& a, int bh, const T* qp, int t0, int lane, f32x4 (&s)[NT], float& qq, float& hh) {
   typedef T t8 __attribute__((ext_vector_type(8)));
   const int g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < NT; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  qq = 0.f;
+  qq = 0.f, hh = 0.f;
   const __bf16* sp = a.split + split_at(a, bh, 0, 0) + lane * 8;
   for (int c0 = 0; c0 < a.dkp; c0 += 32) {
     const int c = c0 + g * 8;
@@ -421,6 +424,12 @@ __device__ __forceinline__ void score_tiles(const BlockArgs& a, int bh, const T*
           if (e0 + e < a.group)
 #pragma unroll
             for (int d = 0; d < 8; ++d) q[d] += (float)x[e][d];
+        if (a.group > 1)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e0 + e < a.group)
+#pragma unroll
+              for (int d = 0; d < 8; ++d) hh = __builtin_fmaf((float)x[e][d], (float)x[e][d], hh);
       }
     }
     bf16x8 qh, ql;
@@ -451,9 +460,9 @@ __device__ __forceinline__ void score_tiles(const BlockArgs& a, int bh, const T*
     }
   }
 }
-// what such a score may be off by; qn, cn: the norms of the query and of the largest mean
-__device__ __forceinline__ float score_error(int dk, float qn, float cn) {
-  return (3.f / 262144.f + 4.f * dk / 16777216.f) * qn * cn + (qn + cn) * 2e-36f + 1e-30f;
+// what such a score may be off by; qn, hn, cn: the norms of the query, of all its heads and of the largest mean
+__device__ __forceinline__ float score_error(const BlockArgs& a, float qn, float hn, float cn) {
+  return ((3.f / 262144.f + 4.f * a.dk / 16777216.f) * qn + a.head_err * hn) * cn + (qn + cn) * 2e-36f + 1e-30f;
 }
 
 // One wave: of nmay <= 16 candidates (lane c < nmay: block mj) the `need` with the largest 64-bit scores, as a mask of lanes; of equal
@@ -495,7 +504,8 @@ __device__ __forceinline__ unsigned long long choose_exact(const BlockArgs& a, i
 // that can decide.  q (summed over the group) and the means are split into two bf16 each; hi hi + hi lo + lo hi leaves out less than
 //   score_error = (3 * 2^-18 + 4 dk 2^-24) |q| |c|     (two splits, the product lo lo, an fp32 sum of 3 dk terms; |.| the 2-norms)
 // of a score (and, where a part is not a normal number any more, dk 2^-126 times the other norm; near the ends of fp32's range nothing
-// is decided here).  Lane (query n, group g) holds the scores of blocks 16 t + 4 g + r; the cut that leaves topk of them over it is found by
+// is decided here).  The sum of a group's n heads is off by up to (n - 1) 2^-24 sum |q_h| in each dim, hence a score by up to
+// (n - 1) sqrt(n) 2^-24 |q_1 .. q_n| |c| more: heads may cancel, so this goes by the norm over all of them.  Lane (query n, group g) holds the scores of blocks 16 t + 4 g + r; the cut that leaves topk of them over it is found by
 // bisection, 16 queries in step.  Where the last block over the cut and the first under it are more than 2 err apart -- all but a
 // few in a thousand -- the order is the exact one's; the other queries (ties, NaN and infinities among them) are scored in 64 bits.
 // Bound by vector instructions, about half of them the bisection's comparisons: 12 heads x 6400 queries x 100 blocks 28 us, 48 x 1600 x 25
@@ -524,8 +534,8 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   }
   // ---- scores
   f32x4 s[NT];
-  float qq;
-  score_tiles<T, NT>(a, bh, head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group), 0, lane, s, qq);
+  float qq, hh;
+  score_tiles<T, NT>(a, bh, head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group), 0, lane, s, qq, hh);
   // ---- which blocks can be selected, how many there are, the largest |c|
   unsigned okw[NWORD];
   int can = 0;
@@ -543,7 +553,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   big = quad_max(big);
   const int take = min(a.topk, can);
   const float qn = sqrtf(quad_sum(qq));
-  const float err = score_error(a.dk, qn, big);
+  const float err = score_error(a, qn, a.group > 1 ? sqrtf(quad_sum(hh)) : 0.f, big);
 
   // ---- the cut.  Blocks that cannot be selected (and places behind the last) go under every cut
 #pragma unroll
@@ -748,11 +758,11 @@ __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, 
   big = max_all(quad_max(big));
   can = sum_all(can);
   f32x4 s[NT];
-  float qq;
-  score_tiles<T, NT>(a, bh, head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group), t0, lane, s, qq);
+  float qq, hh;
+  score_tiles<T, NT>(a, bh, head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group), t0, lane, s, qq, hh);
   const int take = min(a.topk, can);
   const float qn = sqrtf(quad_sum(qq));
-  const float err = score_error(a.dk, qn, big);
+  const float err = score_error(a, qn, a.group > 1 ? sqrtf(quad_sum(hh)) : 0.f, big);
 
   // ---- the cut, as above
   float hi = ninf;
@@ -1579,6 +1589,7 @@ static int fill_args(const std::string& who, const yl_heads* q, const yl_heads* 
   if (nk > 0) a->k = Heads{k->data, k->batch, k->token, k->head, 8};
   a->batch = batch, a->nq = nq, a->nk = nk, a->heads = heads, a->kv = kv_heads, a->group = heads / kv_heads;
   a->magic = (unsigned)((1ULL << 32) / a->group + 1);
+  a->head_err = (float)((a->group - 1) * std::sqrt((double)a->group) * 1.01 / (1 << 24));  // (1.01: the norm is an fp32 sum too)
   a->dk = dk, a->block = block, a->nb = (int)nb, a->topk = topk, a->mask = mask, a->mask_stride = mask_stride;
   return 0;
 }
