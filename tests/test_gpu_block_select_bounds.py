@@ -55,3 +55,21 @@ def test_other_numbers_of_heads_that_cancel(gpu_device, heads):
     q = torch.cat((a, s), 2)
     q[:, :, -1] += -a[:, :, 0] * (1 + 2.0 ** -7 * (heads == 2))
     _check(q.bfloat16().to(gpu_device), k.to(gpu_device), 32, 8)
+
+
+@pytest.mark.parametrize("nb", [40, 100, 250, 500, 1000])
+@pytest.mark.parametrize("kexp, qexp", [(-60, 0), (-70, 0), (-78, 0), (-90, 0), (0, -78), (-78, 70), (60, -90), (-40, -40), (-62, -62)])
+def test_squares_below_the_range(gpu_device, nb, kexp, qexp):
+    """Blocks whose means differ in the last bits of few keys, times powers of two: the order is the same at every scale."""
+    nq, dk, block = 200, 64, 64
+    g = torch.Generator().manual_seed(nb)
+    q = torch.randn(1, nq, 1, dk, generator=g).bfloat16()
+    base = torch.randn(1, 1, 1, dk, generator=g).bfloat16()
+    k = base.repeat(1, nb * block, 1, 1)
+    at = torch.arange(nb) * block
+    for d in (5, 9, 33):
+        k[0, at, 0, d] = (base[0, 0, 0, d].float() * (1 + 2.0 ** -7 * torch.randint(-3, 4, (nb,), generator=g))).bfloat16()
+        k[0, at + 1, 0, d] = (2.0 ** -10 * torch.randn(nb, generator=g)).bfloat16()
+    q, k = (q.double() * 2.0 ** qexp).bfloat16(), (k.double() * 2.0 ** kexp).bfloat16()
+    for topk in (1, 8, 30):
+        _check(q.to(gpu_device), k.to(gpu_device), block, topk)

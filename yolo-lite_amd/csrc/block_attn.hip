@@ -67,7 +67,7 @@ struct BlockArgs {
   double* mean;   // [batch][kv][nb][dk]
   double* score;  // few queries: [batch][kv][nq][nb]
   __bf16* split;  // the means as two bf16, in the order the matrix pipe takes them (split_at); nbp = nb rounded up to 16, dkp = dk to 32
-  float* norm;    // [batch][kv][nb]: 2-norm of a mean
+  float* norm;    // [batch][kv][nb]: no less than the 2-norm of a mean
   int nbp, dkp;
   float head_err; // what the fp32 sum of a group's query heads may be off by, relative to the 2-norm over all of them
   unsigned magic; // 2^32 / group, rounded up: f / group = mulhi(f, magic) for f * group < 2^32
@@ -88,6 +88,8 @@ __device__ __forceinline__ void split2(float x, __bf16* hi, __bf16* lo) {
   *hi = (__bf16)x;
   *lo = (__bf16)(x - (float)*hi);
 }
+// At least the 2-norm, from the sum of up to 2^17 squares: those below 2^-126 may have been lost, 2^-54.5 of a norm at most.
+__device__ __forceinline__ float norm_of(float squares) { return sqrtf(squares) + 0x1p-54f; }
 __device__ __forceinline__ double shfl_xor_d(double x, int o) { return __shfl_xor(x, o); }
 
 // Where the upper half of dim d of block j's mean lies among [batch][kv][nbp / 16][dkp / 32][2][64 lanes][8]: lane (block j % 16, dims
@@ -192,7 +194,7 @@ __device__ __forceinline__ void block_mean(const BlockArgs& a, int bh, int j, in
       at[0] = at[512] = (__bf16)0.f;
     }
     if (lane == 0) {
-      a.norm[(long long)bh * a.nb + j] = sqrtf(norm);
+      a.norm[(long long)bh * a.nb + j] = norm_of(norm);
       if (count) *count = n;
     }
   }
@@ -552,8 +554,8 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
   for (int o = 1; o < 16; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
   big = quad_max(big);
   const int take = min(a.topk, can);
-  const float qn = sqrtf(quad_sum(qq));
-  const float err = score_error(a, qn, a.group > 1 ? sqrtf(quad_sum(hh)) : 0.f, big);
+  const float qn = norm_of(quad_sum(qq));
+  const float err = score_error(a, qn, a.group > 1 ? norm_of(quad_sum(hh)) : 0.f, big);
 
   // ---- the cut.  Blocks that cannot be selected (and places behind the last) go under every cut
 #pragma unroll
@@ -761,8 +763,8 @@ __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, 
   float qq, hh;
   score_tiles<T, NT>(a, bh, head_ptr<const T>(a, a.q, b, live ? i : 0, h * a.group), t0, lane, s, qq, hh);
   const int take = min(a.topk, can);
-  const float qn = sqrtf(quad_sum(qq));
-  const float err = score_error(a, qn, a.group > 1 ? sqrtf(quad_sum(hh)) : 0.f, big);
+  const float qn = norm_of(quad_sum(qq));
+  const float err = score_error(a, qn, a.group > 1 ? norm_of(quad_sum(hh)) : 0.f, big);
 
   // ---- the cut, as above
   float hi = ninf;
