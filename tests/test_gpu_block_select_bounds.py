@@ -1,5 +1,5 @@
-"""GPU: the selection equals the 64-bit one where the scores in fewer bits say least.  The restatement sorts 64-bit scores; nothing is
-rounded but its sums."""
+"""GPU: the selection equals the 64-bit one where the scores in fewer bits say least: query heads that cancel, keys and queries whose
+squares are below fp32's range, values that two bf16 hold worst.  The restatement sorts 64-bit scores; nothing is rounded but its sums."""
 import pytest
 import torch
 
@@ -72,4 +72,25 @@ def test_squares_below_the_range(gpu_device, nb, kexp, qexp):
         k[0, at + 1, 0, d] = (2.0 ** -10 * torch.randn(nb, generator=g)).bfloat16()
     q, k = (q.double() * 2.0 ** qexp).bfloat16(), (k.double() * 2.0 ** kexp).bfloat16()
     for topk in (1, 8, 30):
+        _check(q.to(gpu_device), k.to(gpu_device), block, topk)
+
+
+@pytest.mark.parametrize("heads", [1, 2])
+@pytest.mark.parametrize("dk", [8, 16, 64])
+@pytest.mark.parametrize("nb", [40, 100, 200, 400, 600, 1500])
+def test_values_that_two_bf16_hold_worst(gpu_device, nb, dk, heads):
+    """Every dim of a mean 2^-17 under or over 1 + 2^-8, half way between two bf16: the lower parts are +-2^-8.  A query of 1 + 3 2^-8
+    (half way, lower part -2^-8) differs by 2^-16 between the two sorts of blocks; the product of the lower parts adds 2^-16 to
+    the one and takes it from the other, and what two parts leave of the mean does half as much."""
+    block, nq, over = 128, 64, 20
+    k = torch.full((1, nb * block, 1, dk), 1 + 2.0 ** -8)
+    sign = torch.full((nb,), -1.0)
+    sign[torch.randperm(nb, generator=torch.Generator().manual_seed(dk + nb))[:over]] = 1.0
+    k[0, torch.arange(nb) * block, 0] += (sign * 2.0 ** -10)[:, None]
+    q = torch.full((1, nq, heads, dk), 1 + 3 * 2.0 ** -8 if heads == 1 else 2.0 ** -8)
+    if heads == 2:
+        q[:, :, 0] = 1 + 2.0 ** -7
+    q, k = q.half(), k.half()
+    assert bool((k.float().view(nb, block, dk).mean(1) == (1 + 2.0 ** -8 + sign * 2.0 ** -17)[:, None]).all())
+    for topk in (over - 4, over, over + 3):
         _check(q.to(gpu_device), k.to(gpu_device), block, topk)

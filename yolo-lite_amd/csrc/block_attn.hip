@@ -69,6 +69,7 @@ struct BlockArgs {
   __bf16* split;  // the means as two bf16, in the order the matrix pipe takes them (split_at); nbp = nb rounded up to 16, dkp = dk to 32
   float* norm;    // [batch][kv][nb]: no less than the 2-norm of a mean
   int nbp, dkp;
+  float part_err; // what two bf16 for each factor may leave out of a score, relative to the product of the 2-norms
   float head_err; // what the fp32 sum of a group's query heads may be off by, relative to the 2-norm over all of them
   unsigned magic; // 2^32 / group, rounded up: f / group = mulhi(f, magic) for f * group < 2^32
   int* count;     // [batch][nb]: unmasked keys of a block
@@ -83,7 +84,7 @@ __device__ __forceinline__ T* head_ptr(const BlockArgs& a, const Heads& x, int b
 }
 
 // ------------------------------------------------------------------------------------------------ block means
-// value x as two bf16: x = hi + lo up to 2^-18 |x|
+// value x as two bf16: |x - hi| <= 2^-8 |x|, x = hi + lo up to 2^-17 |x|
 __device__ __forceinline__ void split2(float x, __bf16* hi, __bf16* lo) {
   *hi = (__bf16)x;
   *lo = (__bf16)(x - (float)*hi);
@@ -458,13 +459,14 @@ __device__ __forceinline__ void score_tiles(const BlockArgs& a, int bh, const T*
         s[u0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], qh, s[u0 + t], 0, 0, 0);
         s[u0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml[t], qh, s[u0 + t], 0, 0, 0);
         s[u0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[t], ql, s[u0 + t], 0, 0, 0);
+        s[u0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml[t], ql, s[u0 + t], 0, 0, 0);
       }
     }
   }
 }
 // what such a score may be off by; qn, hn, cn: the norms of the query, of all its heads and of the largest mean
 __device__ __forceinline__ float score_error(const BlockArgs& a, float qn, float hn, float cn) {
-  return ((3.f / 262144.f + 4.f * a.dk / 16777216.f) * qn + a.head_err * hn) * cn + (qn + cn) * 2e-36f + 1e-30f;
+  return ((a.part_err + 4.f * a.dk / 16777216.f) * qn + a.head_err * hn) * cn + (qn + cn) * 2e-36f + 1e-30f;
 }
 
 // One wave: of nmay <= 16 candidates (lane c < nmay: block mj) the `need` with the largest 64-bit scores, as a mask of lanes; of equal
@@ -503,13 +505,17 @@ __device__ __forceinline__ unsigned long long choose_exact(const BlockArgs& a, i
 }
 
 // Many queries, up to 16 NT blocks: a wave scores 16 queries at once on the matrix pipe, in less than 64 bits, and decides only what
-// that can decide.  q (summed over the group) and the means are split into two bf16 each; hi hi + hi lo + lo hi leaves out less than
-//   score_error = (3 * 2^-18 + 4 dk 2^-24) |q| |c|     (two splits, the product lo lo, an fp32 sum of 3 dk terms; |.| the 2-norms)
-// of a score (and, where a part is not a normal number any more, dk 2^-126 times the other norm; near the ends of fp32's range nothing
-// is decided here).  The sum of a group's n heads is off by up to (n - 1) 2^-24 sum |q_h| in each dim, hence a score by up to
-// (n - 1) sqrt(n) 2^-24 |q_1 .. q_n| |c| more: heads may cancel, so this goes by the norm over all of them.  Lane (query n, group g) holds the scores of blocks 16 t + 4 g + r; the cut that leaves topk of them over it is found by
-// bisection, 16 queries in step.  Where the last block over the cut and the first under it are more than 2 err apart -- all but a
-// few in a thousand -- the order is the exact one's; the other queries (ties, NaN and infinities among them) are scored in 64 bits.
+// that can decide.  q (summed over the group) and the means are split into two bf16 each; all four products together are off by less than
+//   score_error = (part_err + 4 dk 2^-24) |q| |c|     (|.| the 2-norms; 4 dk 2^-24: an fp32 sum of 4 dk terms, the fourth below 2^-16)
+// of a score, part_err = 2^-17 for what the mean's two parts leave out, 2^-17 for what q's leave (none of one head's 8 or 11 bits) and a
+// twentieth of that for the mean's own rounding to fp32 (2^-24) and products of these (and, where a part is not a normal number any more,
+// dk 2^-126 times the other norm; near the ends of fp32's range nothing is decided here).  Without the product of the two lower parts
+// part_err is 2^-16 more, and 2 x 16384 queries x 256 blocks, four heads to one, took 40 instead of 39 us.  The sum of a group's n heads
+// is off by up to (n - 1) 2^-24 sum |q_h| in each dim, hence a score by up to (n - 1) sqrt(n) 2^-24 |q_1 .. q_n| |c| more: heads may
+// cancel, so this goes by the norm over all of them.  Lane (query n, group g) holds the scores of blocks 16 t + 4 g + r; the cut that
+// leaves topk of them over it is found by bisection, 16 queries in step.  Where the last block over the cut
+// and the first under it are more than 2 err apart -- all but a few in a thousand -- the order is the exact one's; the other queries
+// (ties, NaN and infinities among them) are scored in 64 bits.
 // Bound by vector instructions, about half of them the bisection's comparisons: 12 heads x 6400 queries x 100 blocks 28 us, 48 x 1600 x 25
 // 17 us, 2 x 16384 x 256 (four query heads to one) 38 us.
 template <typename T, int NT>
@@ -1568,6 +1574,11 @@ static int check_heads(const std::string& who, const char* name, const yl_heads*
   return 0;
 }
 
+static void fill_errors(BlockArgs* a) {  // (block_score_kernel says what these are)
+  a->part_err = (float)(((a->group > 1 ? 2 : 1) + 0.05) / (1 << 17));
+  a->head_err = (float)((a->group - 1) * std::sqrt((double)a->group) * 1.01 / (1 << 24));  // (1.01: the norm is an fp32 sum too)
+}
+
 // sizes that the calls share -> BlockArgs; nothing is launched where batch * nq is 0
 static int fill_args(const std::string& who, const yl_heads* q, const yl_heads* k, int dtype, int batch, int nq, int nk, int heads,
                      int kv_heads, int dk, int block, int topk, const uint8_t* mask, int64_t mask_stride, BlockArgs* a) {
@@ -1591,7 +1602,7 @@ static int fill_args(const std::string& who, const yl_heads* q, const yl_heads* 
   if (nk > 0) a->k = Heads{k->data, k->batch, k->token, k->head, 8};
   a->batch = batch, a->nq = nq, a->nk = nk, a->heads = heads, a->kv = kv_heads, a->group = heads / kv_heads;
   a->magic = (unsigned)((1ULL << 32) / a->group + 1);
-  a->head_err = (float)((a->group - 1) * std::sqrt((double)a->group) * 1.01 / (1 << 24));  // (1.01: the norm is an fp32 sum too)
+  fill_errors(a);
   a->dk = dk, a->block = block, a->nb = (int)nb, a->topk = topk, a->mask = mask, a->mask_stride = mask_stride;
   return 0;
 }
@@ -1882,6 +1893,7 @@ static BlockArgs map_args(int batch, int heads, int n, int block, int topk) {
   BlockArgs a{};
   a.batch = batch, a.nq = a.nk = n, a.heads = a.kv = heads, a.group = 1, a.magic = 1;
   a.dk = 32, a.dv = 64, a.block = block, a.nb = (n + block - 1) / block, a.topk = topk;
+  fill_errors(&a);
   return a;
 }
 namespace yl {
