@@ -418,21 +418,21 @@ __device__ __forceinline__ void score_tiles(const BlockArgs& a, int bh, const T*
     const int c = c0 + g * 8;
     float q[8] = {};
     if (c < a.dk) {
-      for (int e0 = 0; e0 < a.group; e0 += 4) {  // four heads' loads in flight together
-        t8 x[4];
+      if (a.group == 1) {  // (the loop below would ask for it four times: 80x80 maps 31.9 us instead of 30.6)
+        const t8 x = *reinterpret_cast<const t8*>(qp + (c >> 3) * a.q.sc);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const t8*>(qp + min(e0 + e, a.group - 1) * a.q.sh + (c >> 3) * a.q.sc);
+        for (int d = 0; d < 8; ++d) q[d] = (float)x[d];
+      } else {
+        for (int e0 = 0; e0 < a.group; e0 += 4) {  // four heads' loads in flight together
+          t8 x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e0 + e < a.group)
-#pragma unroll
-            for (int d = 0; d < 8; ++d) q[d] += (float)x[e][d];
-        if (a.group > 1)
+          for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const t8*>(qp + min(e0 + e, a.group - 1) * a.q.sh + (c >> 3) * a.q.sc);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (e0 + e < a.group)
 #pragma unroll
-              for (int d = 0; d < 8; ++d) hh = __builtin_fmaf((float)x[e][d], (float)x[e][d], hh);
+              for (int d = 0; d < 8; ++d) q[d] += (float)x[e][d], hh = __builtin_fmaf((float)x[e][d], (float)x[e][d], hh);
+        }
       }
     }
     bf16x8 qh, ql;
