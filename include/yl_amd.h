@@ -394,7 +394,9 @@ int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, int batch, 
                     int block, int topk, const uint8_t* mask, int64_t mask_stride, int32_t* picked, void* work, int64_t work_bytes,
                     void* stream);
 /* out[b][i][h] = softmax over the readable keys of the blocks picked[b][h's kv head][i] of (scale * q . k), times v.  Entries of
- * `picked` outside [0, blocks) are no block; a block named twice counts once; the order does not matter.  fp32 accumulation.
+ * `picked` outside [0, blocks) are no block; a block named twice counts once; the order does not matter.  Sums are fp32; softmax weights
+ * are rounded to the tensors' type before they multiply v, and for bf16 tensors a block's result may be rounded to fp16 once before a
+ * query's blocks are added up (2^-11 of the sum of its weights times |v|, for every channel).
  * `work` as above, yl_block_attention_workspace_bytes bytes (0 where none is needed: NULL then). */
 int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int nq, int nk, int heads, int kv_heads, int dk, int dv, int block,
                                            int topk);

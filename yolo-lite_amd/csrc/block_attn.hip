@@ -238,6 +238,21 @@ __device__ __forceinline__ unsigned wave_or(unsigned c) {
   return (unsigned)__builtin_amdgcn_readlane((int)c, 63);
 }
 
+// the larger of each pair of 16-bit numbers over the 64 lanes
+__device__ __forceinline__ unsigned wave_max2(unsigned c) {
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  auto max2 = [](unsigned x, int y) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, y)));
+  };
+  c = max2(c, __builtin_amdgcn_update_dpp(0, (int)c, 0x111, 0xF, 0xF, false));
+  c = max2(c, __builtin_amdgcn_update_dpp(0, (int)c, 0x112, 0xF, 0xF, false));
+  c = max2(c, __builtin_amdgcn_update_dpp(0, (int)c, 0x114, 0xF, 0xF, false));
+  c = max2(c, __builtin_amdgcn_update_dpp(0, (int)c, 0x118, 0xF, 0xF, false));
+  c = max2(c, __builtin_amdgcn_update_dpp(0, (int)c, 0x142, 0xA, 0xF, false));
+  c = max2(c, __builtin_amdgcn_update_dpp(0, (int)c, 0x143, 0xC, 0xF, false));
+  return (unsigned)__builtin_amdgcn_readlane((int)c, 63);
+}
+
 // The same over a workgroup's NW waves (all of them call), through two small buffers of LDS in turn: one barrier each.
 template <int NW>
 struct Waves {
@@ -911,9 +926,14 @@ __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, 
 // vector instructions to a tile of 16 rows x 64 keys beside 18 MFMAs, 16 of them exponentials at a quarter of the rate.
 //
 // A block's results pass unnormalised (sum of p v; the maximum and sum of p beside them in fp32).  For fp16 tensors they are fp32.  For
-// bf16 tensors they are fp16, toward zero (2^-10 at most, a quarter of a bf16 step; fp32 took 278 instead of 150 us on the 128x128
-// map): a power of two per unit, carried by the weights (exact in bf16), puts the unit's largest value at 2^8, so that the sums fill fp16's
-// range from the top and what lies up to 2^23 below the largest value still has all its bits; the join scales back.
+// bf16 tensors they are fp16 (off by 2^-11 at most, an eighth of a bf16 step; fp32 took 278 instead of 150 us on the 128x128 map):
+// a power of two per unit, carried by the weights (exact in bf16), puts the unit's largest value at 2^8, so that the sums fill fp16's
+// range from the top; the join scales back.  Where no readable value of the unit is under 2^-22 of the largest, the sum of p |v| is in
+// fp16's normal range for every row and channel (the largest p is 1).  The results of other units -- zeros, channels of very different
+// size, large values that may have next to no weight -- stay in fp32: the upper 16 bits where the others have their fp16, the lower 16
+// bits in a second array that is touched for such units alone, and the rows' sums of p are stored as their negatives.  Values half of
+// which are zeros: 334 instead of 184 us on the 128x128 map, 77 instead of 59 on the 40x40 maps (whole calls in a graph).  Looking at the
+// results row by row instead costs registers that the loop over the tiles does not have (spills): 205 us on the 128x128 map for any values.
 //
 // Lists: 64 queries form a group; lists[group] holds its (query, slot) pairs sorted by block, starts[group][j] where block j's begin.
 // A block of 128 keys is two units of 64 (two results per slot): one unit's fragments fill the registers.
@@ -954,7 +974,9 @@ struct AttendArgs {
   int q32;                  // offsets of q inside a range of queries fit 32 bits, its strides 24
   signed char* vexp;        // [b * kv + h][nb * subs]: bf16 tensors: a unit's results are times 2^vexp
   void* part;               // [row][slots][DVP], row = ((b * kv + h) * cq + i - 64 g0) * group + head in the group
-  float2* ml;               // [b * kv + h][slots][nq * group]: maximum (log2), sum -- rows together: a unit's neighbours share lines
+  long long low;            // bf16 tensors: so many bytes behind `part` is the same again, for the lower halves of results in fp32
+  float2* ml;               // [b * kv + h][slots][nq * group]: maximum (log2), sum (negative: the results are in fp32) -- rows together: a
+                            // unit's neighbours share lines
 };
 
 // One wave per (image, kv head, 64 queries): the group's picks sorted by block.  A block counts once per query; slots that name no
@@ -1031,9 +1053,9 @@ __device__ __forceinline__ int value_at(int c, int key) {
 
 // DIRECT: one wave per (image, kv head, query, slot, unit) straight from `picked` -- few queries, where lists would hold one entry.
 // Four workgroups on a CU where the fragments leave room (128 registers; at 131, three of them, the 128x128 map's launch took 119 instead
-// of 108 us; five spill).
+// of 108 us; five spill), three for wide values of bf16 tensors (2 x 6400 queries, 6 heads, key width 64, value width 128: 70 us; two 91).
 template <typename T, int KEYS, int DK32, int DV16, bool DIRECT>
-__global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 4 ? 4 : 2) void block_attend_kernel(AttendArgs p) {
+__global__ __launch_bounds__(DIRECT ? 64 : 256, DIRECT || DK32 > 2 ? 2 : DV16 == 4 ? 4 : sizeof(typename Vec<T>::part) == 2 ? 3 : 2) void block_attend_kernel(AttendArgs p) {
   typedef typename Vec<T>::t8 t8;
   typedef typename Vec<T>::t4 t4;
   constexpr int NT = DIRECT ? 64 : 256;
@@ -1092,7 +1114,7 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
       if (t * 16 + n < kn && (c * 4 + g) * 8 < a.dk) kf[t][c] = *reinterpret_cast<const t8*>(kb + token(a, k0 + t * 16 + n) * a.k.st + (c * 4 + g) * a.k.sc);
     }
   // ---- values; a masked one counts as 0 whatever it holds.  A thread moves two keys x 8 channels.
-  __shared__ unsigned vmax;
+  __shared__ unsigned ends[NT / 64];  // of a wave's values: the largest, 0x7FFF - the smallest
   const T* vb = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh;
   constexpr int ITEMS = KEYS / 2 * (DVP / 8), NV = (ITEMS + NT - 1) / NT;
   u32x4 v[NV][2];
@@ -1149,28 +1171,39 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
             __builtin_amdgcn_perm(v[x][1][e >> 1], v[x][0][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
   }
   // The power of two 2^up that puts the largest finite |v| at 2^8 (values under 2^-92: less): sums of 64 weighted values stay under 2^15.
+  // (Results in fp32: at 2^100, or 2^up = 2^100.)
   // The weights carry it (as far as they can without leaving bf16's range; the rest, where values are beyond 2^60, the stores).
   float upw = HALF ? 0.f : -DOWN, ups = 1.f;
+  bool spread = false;  // some readable value is under 2^-22 of the largest
   if constexpr (HALF) {
-    if (tid == 0) vmax = 0;
     typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-    us2 big = {0, 0};
+    us2 big = {0, 0}, small = {0, 0};
 #pragma unroll
     for (int x = 0; x < NV; ++x)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        const int it = tid + x * NT, c8 = it % (DVP / 8), key = it / (DVP / 8) * 2;
+        const bool there = it < ITEMS && c8 * 8 < a.dv && (ok >> (key + u) & 1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           us2 m = __builtin_bit_cast(us2, v[x][u][e] & 0x7FFF7FFFu);
+          small = __builtin_elementwise_max(small, there ? us2{0x7FFF, 0x7FFF} - m : us2{0, 0});
           m = us2{m[0] < 0x7F80 ? m[0] : (unsigned short)0, m[1] < 0x7F80 ? m[1] : (unsigned short)0};
           big = __builtin_elementwise_max(big, m);
         }
-    const unsigned top = max((unsigned)big[0], (unsigned)big[1]);
+      }
+    const unsigned both = wave_max2(__builtin_bit_cast(unsigned, __builtin_elementwise_max(us2{big[0], small[0]}, us2{big[1], small[1]})));
+    if (lane == 0) ends[wave] = both;
     __syncthreads();
-    if (top) atomicMax(&vmax, top);
-    __syncthreads();
-    const int e = (int)(vmax >> 7) - 127;          // floor(log2 of the largest); -127: zeros, or not normal
-    const int up = vmax ? min(8 - e, 100) : 0;
+    us2 all = {0, 0};
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) all = __builtin_elementwise_max(all, __builtin_bit_cast(us2, ends[w]));
+    const unsigned ends2 = (unsigned)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, all));  // (the same in every lane)
+    const unsigned vmax = ends2 & 0xFFFF, vmin = 0x7FFF - (ends2 >> 16);
+    const int e = (int)(vmax >> 7) - 127, em = (int)(vmin >> 7);  // floor(log2 of the largest) (-127: zeros, or not normal); 0: a zero, or not normal
+    int up = vmax ? min(8 - e, 100) : 0;
+    spread = vmax != 0 && (em == 0 || em - 127 + up < -14);
+    if (spread) up = min(100 - e, 100);
     const int uw = max(up, -60);
     upw = (float)uw;
     ups = __uint_as_float((unsigned)(up - uw + 127) << 23);  // (up - uw >= -59)
@@ -1324,16 +1357,33 @@ __global__ __launch_bounds__(DIRECT ? 64 : 256, !DIRECT && DK32 <= 2 && DV16 == 
       if (ups != 1.f)
 #pragma unroll
         for (int d = 0; d < DV16; ++d) o[d] *= ups;
-      auto pk = [](float lo, float hi) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(lo, hi)); };
+      auto pk = [](float lo, float hi) {  // (round to nearest even)
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{lo, hi}), h2));
+      };
+      if (!spread) {
 #pragma unroll
-      for (int d = 0; d < DV16; d += 2)
-        *reinterpret_cast<u32x4*>(dst + channel(d, 4 * g)) =
-            u32x4{pk(o[d][0], o[d][1]), pk(o[d][2], o[d][3]), pk(o[d + 1][0], o[d + 1][1]), pk(o[d + 1][2], o[d + 1][3])};
+        for (int d = 0; d < DV16; d += 2)
+          *reinterpret_cast<u32x4*>(dst + channel(d, 4 * g)) =
+              u32x4{pk(o[d][0], o[d][1]), pk(o[d][2], o[d][3]), pk(o[d + 1][0], o[d + 1][1]), pk(o[d + 1][2], o[d + 1][3])};
+      } else {
+        auto halves = [](float x, float y, unsigned which) { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), which); };
+#pragma unroll
+        for (int d = 0; d < DV16; d += 2)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const unsigned which = u ? 0x05040100u : 0x07060302u;  // upper halves to part, lower ones behind it
+            *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(dst + channel(d, 4 * g)) + (u ? p.low : 0)) =
+                u32x4{halves(o[d][0], o[d][1], which), halves(o[d][2], o[d][3], which), halves(o[d + 1][0], o[d + 1][1], which),
+                      halves(o[d + 1][2], o[d + 1][3], which)};
+          }
+      }
     } else {
 #pragma unroll
       for (int d = 0; d < DV16; ++d) *reinterpret_cast<f32x4*>(dst + channel(d, 4 * g)) = o[d];
     }
-    if (g == 0) mlb[(long long)w.slot * p.mlrow + local] = float2{m, l};
+    if (g == 0) mlb[(long long)w.slot * p.mlrow + local] = float2{m, spread ? -l : l};
   }
 }
 
@@ -1385,10 +1435,21 @@ __global__ __launch_bounds__(256) void block_join_kernel(AttendArgs p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (l[u] == 0.f) continue;
-      sum += w[u] * l[u];
+      sum += w[u] * fabsf(l[u]);
       const float x = HALF ? __builtin_amdgcn_ldexpf(w[u], ve[u] - Vec<T>::down) : w[u];
+      float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += x * (float)y[u][e];
+      for (int e = 0; e < 8; ++e) f[e] = (float)y[u][e];
+      if constexpr (HALF) {
+        if (l[u] < 0.f) {  // in fp32, as two halves
+          typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+          const us8 hi = __builtin_bit_cast(us8, y[u]), lo = *reinterpret_cast<const us8*>(reinterpret_cast<const char*>(part + (t0 + u) * DVP) + p.low);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = __uint_as_float((unsigned)hi[e] << 16 | lo[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += x * f[e];
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -1733,10 +1794,11 @@ struct AttendPlan {
   bool direct, few;
   int subs, slots, groups, range, dvp;
   int chunk;               // groups of queries whose block results are in memory together
-  long long starts, lists, vexp, part, ml, all;  // byte offsets
+  long long starts, lists, vexp, part, low, ml, all;  // byte offsets
 };
 
-constexpr long long CHUNK_BYTES = 256LL << 20;  // block results in memory at once (measured: 128 MB and more the same time, 64 MB 15 % more, 16 MB twice)
+// block results in memory at once, the second array of bf16 tensors apart (measured: 128 MB and more the same time, 64 MB 15 % more, 16 MB twice)
+constexpr long long CHUNK_BYTES = 256LL << 20;
 static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
   AttendPlan p{};
   p.subs = a.block == 128 ? 2 : 1;
@@ -1780,6 +1842,7 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
   p.ml = take(8 * rows * p.slots);
   const long long cq = p.direct ? a.nq : 64LL * p.chunk;
   p.part = take((long long)part_bytes * a.batch * a.heads * cq * p.slots * p.dvp);
+  p.low = take(part_bytes == 2 ? 2LL * a.batch * a.heads * cq * p.slots * p.dvp : 0);
   p.all = at;
   return p;
 }
@@ -1837,7 +1900,7 @@ static int attend_run(AttendArgs& p, const AttendPlan& pl, int dtype, char* w, h
   p.mlrow = (long long)nq * a.group;
   p.q32 = a.q.st < (1 << 24) && a.q.sh < (1 << 24) && 4096 * a.q.st + 1024 * a.q.sh < (1LL << 31);
   p.starts = reinterpret_cast<unsigned short*>(w + pl.starts), p.lists = reinterpret_cast<unsigned short*>(w + pl.lists);
-  p.vexp = reinterpret_cast<signed char*>(w + pl.vexp), p.part = w + pl.part, p.ml = reinterpret_cast<float2*>(w + pl.ml);
+  p.vexp = reinterpret_cast<signed char*>(w + pl.vexp), p.part = w + pl.part, p.low = pl.low - pl.part, p.ml = reinterpret_cast<float2*>(w + pl.ml);
   if (!pl.direct) {
     hipLaunchKernelGGL(block_lists_kernel, dim3((unsigned)(batch * kv_heads * pl.groups)), dim3(64), (size_t)a.nb * 10 + 16, s, p);
     YL_HIP(hipGetLastError());

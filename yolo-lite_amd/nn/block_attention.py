@@ -86,7 +86,8 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, picked: t
     """softmax over the readable keys of the picked blocks of ``scale`` q . k (default: dk ** -0.5), times v: (batch, nq, heads, dv).
 
     picked: int32 (batch, kv heads, nq, topk), as ``block_select`` gives it; entries that name no block are skipped and a block
-    named twice counts once.  A query without a readable key gets zeros."""
+    named twice counts once.  A query without a readable key gets zeros.  Sums are fp32; weights are rounded to the tensors' type before
+    they multiply v, and for bf16 a block's result may be rounded to fp16 (2^-11 of its sum of weights times |v|)."""
     dev = on_gpu("block_attention", q, k, v, picked, mask)
     (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_attention", q, k, mask)
     vs, ps = v.shape, picked.shape
