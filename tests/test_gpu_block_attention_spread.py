@@ -45,3 +45,18 @@ def test_channels_and_keys_of_zeros(gpu_device, nq, block):
     picked = _ya().block_select(q, k, block=block, topk=8)
     out = _check_attend(q, k, v, picked, block, rows=np.arange(0, nq, 9))
     assert bool((out[..., ::5] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_several_passes_over_the_block_results(gpu_device, dtype):
+    """16 query heads x 64 results of width 128: 1024 queries in bf16 (512 in fp16) to a pass of 256 MiB.  The same queries in calls of one
+    pass each, a call once more, and the definition for some of them."""
+    nq, part = 2500, 500
+    q, k, v = _inputs(gpu_device, 1, nq, 64 * 128 - 7, 16, 4, 32, 128, dtype=dtype)
+    v[:, 100:200] = 0  # (some blocks' results in fp32)
+    picked = _ya().block_select(q, k, block=128, topk=32)
+    out = _check_attend(q, k, v, picked, 128, rows=np.array([0, 511, 512, 1023, 1024, 1500, 2047, 2048, nq - 1]))
+    assert torch.equal(out, _ya().block_attention(q, k, v, picked, block=128))
+    for i in range(0, nq, part):
+        got = _ya().block_attention(q[:, i: i + part], k, v, picked[:, :, i: i + part].contiguous(), block=128)
+        assert torch.equal(got, out[:, i: i + part])
