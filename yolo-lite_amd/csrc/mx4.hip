@@ -10,6 +10,7 @@
 // Storage: codes[rows][ceil(cols / 32) * 16] bytes, two codes to a byte, the first in the low half; scales[rows][ceil(cols / 32)].
 // Columns behind the last are zeros.  An MFMA operand of 16 rows x 128 columns is then, per lane (row = lane & 15, block
 // g = lane >> 4), one aligned 16-byte load of codes and one scale byte: nothing is rearranged between memory and the pipe.
+#include <algorithm>
 #include <type_traits>
 
 #include "conv_common.h"
@@ -358,6 +359,7 @@ __device__ __forceinline__ unsigned scale_slot(int row64, int block16, bool weig
   return (unsigned)((((block16 & 3) * 16 + r) * 4 + t) * 4 + (block16 >> 2));
 }
 
+constexpr int GROUPS_Y = 32768;  // groups of 64 rows along y of the grid, the rest along z
 struct TileArgs {
   QuantArgs q;         // x; q.codes nullptr: x comes quantised, q.scales are its scales
   uint8_t* xs;         // tiled scales of x
@@ -373,8 +375,10 @@ __global__ __launch_bounds__(1024) void mx4_tile_kernel(TileArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t sm[1024];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kb = a.q.kb;
-  const bool weight = (int)blockIdx.y >= a.xgroups;
-  const int rg = weight ? (int)blockIdx.y - a.xgroups : (int)blockIdx.y, k4 = blockIdx.x;
+  const int group = (int)(blockIdx.z * gridDim.y + blockIdx.y);  // (gridDim.y is at most GROUPS_Y)
+  if (group >= a.xgroups + a.wgroups) return;
+  const bool weight = group >= a.xgroups;
+  const int rg = weight ? group - a.xgroups : group, k4 = blockIdx.x;
   sm[tid] = 0x7F;
   __syncthreads();
   if (weight || !a.q.codes) {
@@ -731,9 +735,22 @@ static int split_launch(const LinearArgs& a, hipStream_t s) {
   return 0;
 }
 
+// the sizes and the activations' type: what the call and the size of its workspace refuse alike
+static int check_linear(int x_dtype, long long rows, long long n, long long k, Plan* p) {
+  if (!value_type(x_dtype) && x_dtype != YL_MX4) return fail(-1, "mx4_linear: activations are bf16, fp16, fp32 or MX4");
+  if (int rc = check_matrix("mx4_linear", rows, k, k)) return rc;
+  if (int rc = check_matrix("mx4_linear", n, k, k)) return rc;
+  if (n < 1 || n > (1 << 22)) return fail(n < 1 ? -1 : -3, "mx4_linear: 1 to 4194304 output columns");
+  if (rows == 0) return 0;
+  *p = plan_linear(x_dtype, rows, n, k);
+  if (p->ntiles * p->mtiles > 0xFFFFFFFFLL / (p->tiled && !p->big ? 256 : 512))  // (threads of a grid: below 2^32)
+    return fail(-3, "mx4_linear: more rows than one launch covers");
+  return 0;
+}
+
 extern "C" int64_t yl_mx4_linear_workspace_bytes(int x_dtype, int64_t rows, int64_t n, int64_t k) {
-  if (check_matrix("mx4_linear", rows, k, k) || check_matrix("mx4_linear", n, k, k)) return -1;
-  return rows == 0 ? 0 : plan_linear(x_dtype, rows, n, k).all;
+  Plan p{};
+  return check_linear(x_dtype, rows, n, k, &p) ? -1 : p.all;
 }
 
 extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype, int64_t rows, int64_t x_stride,
@@ -741,21 +758,18 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
                              const void* res, int64_t res_stride, void* y, int y_dtype, int64_t y_stride, void* work,
                              int64_t work_bytes, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!value_type(x_dtype) && x_dtype != YL_MX4) return fail(-1, "mx4_linear: activations are bf16, fp16, fp32 or MX4");
+  Plan p{};
+  if (int rc = check_linear(x_dtype, rows, n, k, &p)) return rc;
   if (!value_type(y_dtype)) return fail(-1, "mx4_linear: bf16, fp16 or fp32 results");
-  if (int rc = check_matrix("mx4_linear", rows, k, x_dtype == YL_MX4 ? k : x_stride)) return rc;
-  if (int rc = check_matrix("mx4_linear", n, k, k)) return rc;
-  if (n < 1 || n > (1 << 22)) return fail(n < 1 ? -1 : -3, "mx4_linear: 1 to 4194304 output columns");
   if (rows == 0) return 0;
+  if (x_dtype != YL_MX4)
+    if (int rc = check_matrix("mx4_linear", rows, k, x_stride)) return rc;
   if (rows > 1 && (y_stride < n || (res && res_stride < n))) return fail(-1, "mx4_linear: a row stride is smaller than a row");
   if (!x || !w_codes || !w_scales || !y) return fail(-1, "mx4_linear: null pointer");
   if (x_dtype == YL_MX4 && !x_scales) return fail(-1, "mx4_linear: MX4 activations come with their scales");
   if (!aligned16(w_codes) || (x_dtype == YL_MX4 && !aligned16(x))) return fail(-1, "mx4_linear: codes must be 16-byte aligned");
-  const Plan p = plan_linear(x_dtype, rows, n, k);
   if (p.all > 0 && (!work || work_bytes < p.all || !aligned16(work)))
     return fail(-1, "mx4_linear: workspace missing, too small or not 16-byte aligned");
-  if (p.ntiles * p.mtiles > 0x7FFFFFFFLL || p.xgroups + p.wgroups > 65535)
-    return fail(-3, "mx4_linear: more rows than one launch covers");
   LinearArgs a{};
   a.rows = rows, a.n = (int)n, a.k = (int)k, a.kb = (int)((k + 31) / 32);
   a.wc = w_codes, a.ws = w_scales, a.bias = bias, a.act = act;
@@ -792,8 +806,8 @@ extern "C" int yl_mx4_linear(const void* x, const uint8_t* x_scales, int x_dtype
   ta.q.codes = packed ? nullptr : codes, ta.q.scales = const_cast<uint8_t*>(x_scales);
   ta.xs = xs, ta.ws = w_scales, ta.wst = xs + p.xs, ta.n = (int)n, ta.xgroups = a.xgroups, ta.wgroups = a.wgroups;
   if (int rc = by_type(packed ? YL_BF16 : x_dtype, [&](auto* t) {
-        hipLaunchKernelGGL(mx4_tile_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)p.k4, (unsigned)(p.xgroups + p.wgroups)), dim3(1024), 0,
-                           s, ta);
+        const unsigned groups = (unsigned)(p.xgroups + p.wgroups), gy = std::min<unsigned>(groups, GROUPS_Y);
+        hipLaunchKernelGGL(mx4_tile_kernel<std::remove_pointer_t<decltype(t)>>, dim3((unsigned)p.k4, gy, (groups + gy - 1) / gy), dim3(1024), 0, s, ta);
         YL_HIP(hipGetLastError());
         return 0;
       }))
