@@ -355,7 +355,7 @@ int yl_letterbox_u8(const uint8_t* src_bgr_hwc, int src_h, int src_w, int src_pi
  *
  * yl_mx4_quantize: x[rows][cols] (YL_BF16, YL_F16 or YL_F32; row stride in elements) -> codes, scales.  Per block the scale byte is
  * max(E - 2, 0), E the biased fp32 exponent of the largest magnitude; elements round to nearest even and saturate at 6.  A block
- * that holds an infinity or a NaN gets scale 255 and reads as NaN.
+ * that holds an infinity or a NaN gets scale 255 and reads as NaN.  Fewer than 2^30 blocks to a call, up to 4194304 columns.
  * yl_mx4_dequantize: the values the codes stand for (exact in bf16 and fp32; fp16 rounds and overflows as a conversion does). */
 int yl_mx4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, uint8_t* codes, uint8_t* scales,
                     void* stream);

@@ -24,3 +24,16 @@ def test_many_rows_and_columns(gpu_device, rows, n, k, packed):
     c = some(n) if n > rows else torch.arange(n, device=gpu_device)
     _check_product(y[r][:, c], mx4_ref.rounded(_np(x[r])), mx4_ref.rounded(_np(w[c])), b[c], True, None)
     assert bool(torch.isfinite(y).all())
+
+
+def test_more_than_2_to_the_31_groups_of_eight_columns(gpu_device):
+    """One column of values that 4 bits hold: what comes back is what went in."""
+    ya = _ya()
+    rows = (1 << 29) + 70_001
+    g = torch.Generator(device=gpu_device).manual_seed(3)
+    part = torch.randint(2, 4, (1_000_003, 1), generator=g, device=gpu_device) * 2.0 ** torch.randint(-20, 20, (1_000_003, 1), generator=g, device=gpu_device)
+    part = (part * (torch.randint(0, 2, (1_000_003, 1), generator=g, device=gpu_device) * 2 - 1)).bfloat16()
+    x = part.repeat(rows // 1_000_003 + 1, 1)[:rows]
+    t = ya.mx4_quantize(x)
+    assert t.codes.shape == (rows, 16)
+    assert torch.equal(ya.mx4_dequantize(t), x)

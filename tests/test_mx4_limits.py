@@ -24,3 +24,14 @@ def test_sizes_that_have_a_workspace(x_dtype, rows, n, k):
     from yololite_amd import _lib
 
     assert _lib.lib().yl_mx4_linear_workspace_bytes(x_dtype, rows, n, k) >= 0
+
+
+@pytest.mark.parametrize("rows, cols", [(1 << 30, 1), (1 << 30, 32), ((1 << 29) + 1, 64), (1 << 14, 1 << 22), (1 << 34, 32)])
+def test_quantize_takes_fewer_than_2_to_the_30_blocks(rows, cols):
+    """Four threads to a block: the driver would take no launch of 2^32."""
+    from yololite_amd import _lib
+
+    L = _lib.lib()
+    at = 1 << 20
+    assert L.yl_mx4_quantize(at, 0, rows, cols, cols, at, at, None) == -3 and b"mx4_quantize" in L.yl_last_error()
+    assert L.yl_mx4_dequantize(at, at, rows, cols, at, 0, cols, None) == -3 and b"mx4_dequantize" in L.yl_last_error()

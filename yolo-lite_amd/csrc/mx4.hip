@@ -102,22 +102,14 @@ __device__ __forceinline__ float scale_value(unsigned s) {
   return __uint_as_float(s == 0 ? 0x00400000u : (s == 255u ? 0x7FC00000u : s << 23));
 }
 
-// item = (row, group of eight columns) of a [rows][per_row] list; one division per thread, in 64 bits only where the list needs it
+// item = (row, group of eight columns) of a [rows][per_row] list of fewer than 2^32
 struct Item {
   long long row;
   int c8;
 };
-__device__ __forceinline__ Item item_of(unsigned long long i, unsigned per_row) {
-  Item t;
-  if (i <= 0xFFFFFFFFull) {
-    const unsigned q = (unsigned)i / per_row;
-    t.row = q;
-    t.c8 = (int)((unsigned)i - q * per_row);
-  } else {
-    t.row = (long long)(i / per_row);
-    t.c8 = (int)(i - (unsigned long long)t.row * per_row);
-  }
-  return t;
+__device__ __forceinline__ Item item_of(unsigned i, unsigned per_row) {
+  const unsigned q = i / per_row;
+  return Item{q, (int)(i - q * per_row)};
 }
 
 // One lane holds a whole block: 32 values from p (zeros from the n-th on) -> the 16 bytes of codes, the scale byte.
@@ -156,8 +148,8 @@ struct QuantArgs {
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(QuantArgs a) {
   const unsigned per_row = 4u * (unsigned)a.kb;
-  const unsigned long long i = (unsigned long long)blockIdx.x * 256u + threadIdx.x;
-  if (i >= (unsigned long long)a.rows * per_row) return;  // (whole groups of four lanes: the list's length is a multiple of 4)
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= (unsigned)a.rows * per_row) return;  // (whole groups of four lanes: the list's length is a multiple of 4)
   const Item t = item_of(i, per_row);
   float v[8];
   load8(static_cast<const T*>(a.x) + t.row * a.stride + t.c8 * 8, a.cols - t.c8 * 8, a.vec, v);
@@ -170,8 +162,8 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(QuantArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(QuantArgs a, T* y) {
   const unsigned per_row = 4u * (unsigned)a.kb;
-  const unsigned long long i = (unsigned long long)blockIdx.x * 256u + threadIdx.x;
-  if (i >= (unsigned long long)a.rows * per_row) return;
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= (unsigned)a.rows * per_row) return;
   const Item t = item_of(i, per_row);
   const unsigned c = reinterpret_cast<const unsigned*>(a.codes)[i];
   const float x = scale_value(a.scales[t.row * a.kb + (t.c8 >> 2)]);
@@ -616,10 +608,10 @@ static int by_type(int dtype, F f) {
   return f((float*)nullptr);
 }
 
+// four threads to a block of 32; the driver takes fewer than 2^32 threads
 static int grid_of(const char* who, long long rows, int kb, unsigned* grid) {
-  const long long wg = (rows * 4 * kb + 255) / 256;
-  if (wg > 0x7FFFFFFFLL) return fail(-3, std::string(who) + ": more rows than one launch covers");
-  *grid = (unsigned)wg;
+  if (rows > (0xFFFFFF00LL / 4) / kb) return fail(-3, std::string(who) + ": more than 2^30 blocks of 32 columns in one call");
+  *grid = (unsigned)((rows * 4 * kb + 255) / 256);
   return 0;
 }
 
