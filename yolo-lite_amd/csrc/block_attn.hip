@@ -1627,6 +1627,9 @@ static long long round256(long long n) { return (n + 255) / 256 * 256; }
 // a * b * c below 2^31 (factors below 2^31: a product in 64 bits could wrap around)
 static bool fits31(long long a, long long b, long long c) { return (double)a * (double)b * (double)c < 2147483648.0; }
 
+// the driver takes launches of fewer than 2^32 threads
+static bool fits_grid(long long workgroups, int threads) { return workgroups * threads < 1LL << 32; }
+
 static int check_heads(const std::string& who, const char* name, const yl_heads* t) {
   if (!t || !t->data) return fail(-1, who + ": null " + name);
   if ((reinterpret_cast<uintptr_t>(t->data) & 15) || ((t->batch | t->token | t->head) & 7))
@@ -1703,11 +1706,22 @@ static SelectPlan plan_select(BlockArgs* a) {
   return p;
 }
 
+// (block_mean_kernel; what score_by_size and select_run launch where there are many)
+static int check_select(const BlockArgs& a) {
+  const long long bh = (long long)a.batch * a.kv;
+  const bool few = a.nq <= SCORE_MAX_NQ;
+  const bool fits = fits_grid((bh * a.nb + 3) / 4, 256) &&
+                    (few ? fits_grid(bh * a.nq, a.nb <= 256 ? 64 : a.nb <= 1024 ? 256 : 1024)
+                         : fits_grid(bh * ((a.nq + 15) / 16) + 4, a.nb <= 256 ? 64 : a.nb <= 512 ? 256 : 512));
+  return fits ? 0 : fail(-3, "block_select: more queries or blocks than one launch covers");
+}
+
 extern "C" int64_t yl_block_select_workspace_bytes(int batch, int nq, int nk, int heads, int kv_heads, int dk, int block) {
   BlockArgs a{};
   yl_heads dummy{reinterpret_cast<void*>(16), 0, 0, 0};
   if (fill_args("block_select", &dummy, &dummy, YL_BF16, batch, nq, nk, heads, kv_heads, dk, block, 1, nullptr, 0, &a)) return -1;
-  return batch * (long long)nq == 0 ? 0 : plan_select(&a).all;
+  if (batch * (long long)nq == 0) return 0;
+  return check_select(a) ? -1 : plan_select(&a).all;
 }
 
 template <typename T, bool SCORE, bool SMALL = false>
@@ -1782,6 +1796,7 @@ extern "C" int yl_block_select(const yl_heads* q, const yl_heads* k, int dtype, 
   if (int rc = fill_args("block_select", q, k, dtype, batch, nq, nk, heads, kv_heads, dk, block, topk, mask, mask_stride, &a)) return rc;
   if (batch * (long long)nq == 0) return 0;
   if (!picked) return fail(-1, "block_select: null pointer");
+  if (int rc = check_select(a)) return rc;
   const SelectPlan p = plan_select(&a);
   if (p.all > 0 && (!work || work_bytes < p.all || (reinterpret_cast<uintptr_t>(work) & 15)))
     return fail(-1, "block_select: workspace missing, too small or not 16-byte aligned");
@@ -1847,6 +1862,20 @@ static AttendPlan plan_attend(const BlockArgs& a, int dv, int dtype) {
   return p;
 }
 
+static int check_attend(const BlockArgs& a, const AttendPlan& p) {
+  const long long bh = (long long)a.batch * a.kv;
+  bool fits;
+  if (p.few) {
+    fits = fits_grid(bh * a.nq * ((a.group + 15) / 16), 512);
+  } else {
+    const long long nrange = p.direct ? 0 : (p.chunk + p.range - 1) / p.range;
+    const long long queries = p.direct ? a.nq : std::min<long long>(a.nq, 64LL * p.chunk);
+    fits = fits_grid((long long)a.batch * queries * a.heads * (p.dvp / 8) + 255, 1) &&
+           (p.direct ? fits_grid(bh * a.nq * a.topk * p.subs, 64) : fits_grid(bh * nrange * a.nb * p.subs, 256) && fits_grid(bh * p.groups, 64));
+  }
+  return fits ? 0 : fail(-3, "block_attention: more queries or blocks than one launch covers");
+}
+
 template <typename T, int KEYS, int DK32, int DV16>
 static int attend_launch(const AttendArgs& p, bool direct, bool few, hipStream_t s) {
   const BlockArgs& a = p.a;
@@ -1860,7 +1889,6 @@ static int attend_launch(const AttendArgs& p, bool direct, bool few, hipStream_t
     return 0;
   }
   const long long wg = direct ? bh * a.nq * a.topk * p.subs : bh * p.nrange * a.nb * p.subs;
-  if (wg > 0x7FFFFFFFLL) return fail(-3, "block_attention: more blocks and queries than one launch covers");
   if (direct)
     hipLaunchKernelGGL((block_attend_kernel<T, KEYS, DK32, DV16, true>), dim3((unsigned)wg), dim3(64), 0, s, p);
   else
@@ -1888,7 +1916,9 @@ extern "C" int64_t yl_block_attention_workspace_bytes(int dtype, int batch, int 
     fail(-3, "block_attention: value widths are multiples of 8 up to 128");
     return -1;
   }
-  return batch * (long long)nq == 0 ? 0 : plan_attend(a, dv, dtype).all;
+  if (batch * (long long)nq == 0) return 0;
+  const AttendPlan p = plan_attend(a, dv, dtype);
+  return check_attend(a, p) ? -1 : p.all;
 }
 
 // the attention of `p.a` (sizes, tensors, picked and scale filled in), with plan `pl` and its workspace
@@ -1943,6 +1973,7 @@ extern "C" int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl
     return fail(-1, "block_attention: out has a stride of 0");
   if (!picked) return fail(-1, "block_attention: null pointer");
   const AttendPlan pl = plan_attend(a, dv, dtype);
+  if (int rc = check_attend(a, pl)) return rc;
   if (pl.all > 0 && (!work || work_bytes < pl.all || (reinterpret_cast<uintptr_t>(work) & 15)))
     return fail(-1, "block_attention: workspace missing, too small or not 16-byte aligned");
   if (nk > 0) a.v = Heads{v->data, v->batch, v->token, v->head, 8};
@@ -1988,5 +2019,7 @@ extern "C" int64_t yl_attention_scratch_bytes(int batch, int heads, int tokens, 
     fail(-3, "attention: blocks of 32, 64 or 128 tokens, at most 4096 of them, 1 to 64 for a token");
     return -1;
   }
+  const BlockArgs a = map_args(batch, heads, tokens, block, topk);
+  if (check_select(a) || check_attend(a, plan_attend(a, a.dv, YL_BF16))) return -1;
   return yl::block_attention_map_bytes(batch, heads, tokens, block, topk);
 }
