@@ -35,7 +35,7 @@ def _heads(t: torch.Tensor):
     return t, _pack(at, b, n, h)
 
 
-def _check(what: str, q: torch.Tensor, k: torch.Tensor, mask: Optional[torch.Tensor]):
+def _check(what: str, q: torch.Tensor, k: torch.Tensor, mask: Optional[torch.Tensor], block: int, topk: int):
     """-> the sizes batch, nq, heads, dk, nk, kv heads; and the mask as rows of bytes, its address and row stride."""
     if q.dtype not in _TYPES or k.dtype != q.dtype:
         raise TypeError(f"{what}: q and k are both bf16 or both fp16, got {q.dtype} and {k.dtype}")
@@ -44,6 +44,8 @@ def _check(what: str, q: torch.Tensor, k: torch.Tensor, mask: Optional[torch.Ten
         raise ValueError(f"{what}: q (batch, nq, heads, dk) and k (batch, nk, kv heads, dk) are needed, got {tuple(qs)} and {tuple(ks)}")
     batch, nq, heads, dk = qs
     nk, kv = ks[1], ks[2]
+    if (batch | nq | heads | nk | block | topk) >> 31:  # (the C calls take 32-bit sizes; a larger one would wrap)
+        raise NotImplementedError(f"{what}: sizes from 0 to {2 ** 31 - 1}, got q {tuple(qs)}, k {tuple(ks)}, block {block}, topk {topk}")
     if kv == 0 or heads == 0 or heads % kv:
         raise ValueError(f"{what}: {heads} query heads for {kv} kv heads")
     at = row = None
@@ -69,7 +71,7 @@ def block_select(q: torch.Tensor, k: torch.Tensor, block: int = 64, topk: int = 
     (batch, kv heads, nq, topk): ascending block indices, -1 behind the last.  Score: (q summed over the kv head's query heads) .
     (mean of the block's readable keys), in 64 bits; ties go to the lower index; a block without a readable key is never picked."""
     dev = on_gpu("block_select", q, k, mask)
-    (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_select", q, k, mask)
+    (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_select", q, k, mask, block, topk)
     L = _lib.lib()
     nbytes = L.yl_block_select_workspace_bytes(batch, nq, nk, heads, kv, dk, block)
     work = _workspace("block_select", nbytes, q)
@@ -89,13 +91,14 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, picked: t
     named twice counts once.  A query without a readable key gets zeros.  Sums are fp32; weights are rounded to the tensors' type before
     they multiply v, and for bf16 a block's result may be rounded to fp16 (2^-11 of its sum of weights times |v|)."""
     dev = on_gpu("block_attention", q, k, v, picked, mask)
-    (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_attention", q, k, mask)
     vs, ps = v.shape, picked.shape
+    topk = ps[3] if len(ps) == 4 else 0
+    (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_attention", q, k, mask, block, topk)
     if v.dtype != q.dtype or len(vs) != 4 or vs[:3] != (batch, nk, kv):
         raise ValueError(f"block_attention: v (batch, nk, kv heads, dv) in q's type is needed, got {tuple(vs)} in {v.dtype}")
     if picked.dtype != torch.int32 or len(ps) != 4 or ps[:3] != (batch, kv, nq):
         raise ValueError(f"block_attention: picked (batch, kv heads, nq, topk) in int32 is needed, got {tuple(ps)} in {picked.dtype}")
-    dv, topk = vs[3], ps[3]
+    dv = vs[3]
     L = _lib.lib()
     nbytes = L.yl_block_attention_workspace_bytes(_TYPES[q.dtype], batch, nq, nk, heads, kv, dk, dv, block, topk)
     work = _workspace("block_attention", nbytes, q)
