@@ -31,10 +31,11 @@ enum {
   YL_OP_DWCONV3 = 2,  /* depthwise 3x3 stride 1, +bias, optional SiLU, optional accumulate        */
   YL_OP_SPPF_POOL = 3,/* three chained MaxPool2d(5,1,2): writes pool5/9/13 after the input slice  */
   YL_OP_UPSAMPLE = 4, /* nearest upsample by `stride` (1 = plain copy) into a channel slice        */
-  YL_OP_ATTENTION = 5,/* softmax(q^T k * scale) applied to v, per head (C2PSA).  grp = 0: over all tokens.  grp = 32, 64 or 128:
-                           over the reserved2 (1..64) blocks of grp consecutive tokens (raster order) that yl_block_select's score
-                           selects for each token and head (at most 4096 blocks): yl_block_select + yl_block_attention on the map in
-                           place; out8.offset = scratch of the op's own in the workspace (yl_attention_scratch_bytes)  */
+  YL_OP_ATTENTION = 5,/* softmax(q^T k * scale) applied to v, per head (C2PSA).  reserved2 = 0: over all tokens (grp is not
+                           read).  reserved2 = 1..64: over that many blocks of grp = 32, 64 or 128 consecutive tokens (raster order)
+                           that yl_block_select's score selects for each token and head (at most 4096 blocks): yl_block_select +
+                           yl_block_attention on the map in place; out8.offset = scratch of the op's own in the workspace
+                           (yl_attention_scratch_bytes)  */
   YL_OP_STEM = 6,     /* first layer fused with the input conversion: 3x3 stride-2 conv on the 3-channel
                          NCHW network input (fp32 / fp16 / uint8, /255 for uint8) -> bf16 planes; must be
                          op 0; weight [Cout][3][3][3]                                              */
@@ -404,7 +405,7 @@ int yl_block_attention(const yl_heads* q, const yl_heads* k, const yl_heads* v, 
                        int kv_heads, int dk, int dv, int block, int topk, const int32_t* picked, const uint8_t* mask,
                        int64_t mask_stride, float scale, const yl_heads* out, void* work, int64_t work_bytes, void* stream);
 
-/* Scratch of a YL_OP_ATTENTION op with grp != 0 on maps of `tokens` tokens. */
+/* Scratch of a YL_OP_ATTENTION op over selected blocks on maps of `tokens` tokens (-1: the sizes are refused). */
 int64_t yl_attention_scratch_bytes(int batch, int heads, int tokens, int block, int topk);
 
 /* ---- multi-GPU exchange of the sharded path ---------------------------------

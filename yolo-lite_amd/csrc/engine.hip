@@ -895,7 +895,7 @@ extern "C" int yl_engine_create(const yl_op* ops, int n_ops, int batch, int in_h
         if (o.key_dim != 32 || o.head_dim != 64)
           return fail(-3, tag + ": attention supports key_dim 32 / head_dim 64 (every YOLO11 scale)");
         if (o.in.C != o.heads * 128 || o.out.C != o.heads * 64) return fail(-1, tag + ": attention channel mismatch");
-        if (o.grp != 0) {  // over the blocks a score selects (yl_amd.h)
+        if (o.reserved2 != 0) {  // over the blocks a score selects (yl_amd.h; grp alone says nothing)
           const int n = o.in.H * o.in.W;
           if ((o.grp != 32 && o.grp != 64 && o.grp != 128) || o.reserved2 < 1 || o.reserved2 > 64 || (n + o.grp - 1) / o.grp > 4096)
             return fail(-3, tag + ": blocks of 32, 64 or 128 tokens (grp), at most 4096 of them, 1 to 64 for a token (reserved2)");
@@ -1516,7 +1516,7 @@ static int run_op(const yl_engine* e, const OpRec& r, char* ws, hipStream_t s, c
       a.heads = o.heads;
       a.batch = B;
       a.scale = o.scale;
-      if (o.grp != 0) return block_attention_map_launch(a, o.grp, o.reserved2, ws + o.out8.offset, s);
+      if (o.reserved2 != 0) return block_attention_map_launch(a, o.grp, o.reserved2, ws + o.out8.offset, s);
       return attention_launch(a, s);
     }
   }
