@@ -103,7 +103,8 @@ __device__ __forceinline__ long long split_at(const BlockArgs& a, int bh, int j,
 // One wave per (image, kv head, block): lane = (key lane, 8 dims), 64 / CP key lanes (CP: dk / 8 rounded up to a power of two); the
 // lanes of a dim chunk exchange halves, then quarters, ... of their sums, so a wave reduces with 7 exchanges instead of 24.
 // SCORE: few queries -- the wave that has a block's mean also scores it, and no mean is stored.
-// Bound by reading the keys: 8 heads x 65536 keys of 64 (67 MB) 18 us, 3700 GB/s, this card's rate for reading alone.
+// 8 heads x 65536 keys of 64 (67 MB) 18 us, 3700 GB/s: the loads, and beside them 850 vector instructions of a wave (conversions to and
+// sums in 64 bits), which take up 45 % of the SIMDs' cycles.
 // That wave's part: score[i * step] of the queries, *count keys.
 template <typename T, int CP, bool SCORE>
 __device__ __forceinline__ void block_mean(const BlockArgs& a, int bh, int j, int lane, double* score, int step, int* count) {
@@ -531,8 +532,9 @@ __device__ __forceinline__ unsigned long long choose_exact(const BlockArgs& a, i
 // leaves topk of them over it is found by bisection, 16 queries in step.  Where the last block over the cut
 // and the first under it are more than 2 err apart -- all but a few in a thousand -- the order is the exact one's; the other queries
 // (ties, NaN and infinities among them) are scored in 64 bits.
-// Bound by vector instructions, about half of them the bisection's comparisons: 12 heads x 6400 queries x 100 blocks 28 us, 48 x 1600 x 25
-// 17 us, 2 x 16384 x 256 (four query heads to one) 38 us.
+// 12 heads x 6400 queries x 100 blocks 27 us, 48 x 1600 x 25 17 us, 2 x 16384 x 256 (four query heads to one) 38 us: 1800, 1100 and 4000
+// vector instructions of a wave, about half of them the bisection's comparisons, issued in 42, 37 and 31 % of the cycles -- the steps of
+// the bisection wait for one another, and there are few waves beside each other to fill in.
 template <typename T, int NT>
 __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(BlockArgs a, int qtiles) {
   __shared__ double qs[4][128];
@@ -729,8 +731,9 @@ __global__ __launch_bounds__(256, NT <= 8 ? 4 : 2) void block_score_kernel(Block
 
 // The same by NW waves (4 or 8) for 16 queries: wave w has blocks 16 NT w .., each step of the bisection adds up their counts through
 // LDS.  Then a wave finishes 16 / NW queries, from words of 64 blocks.  What it is for: more blocks than a wave's registers hold scores
-// of (16384 queries, 513 blocks, 4 heads of 64: a wave per query with every score in 64 bits 707 us, this 84; 8192 queries, 1024 blocks,
-// 8 heads of 128: 1159 and 78 us), and few queries.  It is bound by its comparisons: 12 steps over the scores in registers.
+// of (16384 queries, 513 blocks, four heads of 64 to one kv head: a wave per query with every score in 64 bits 707 us, this 81; 8192 queries,
+// 1024 blocks, eight heads of 128 to one: 1159 and 75 us), and few queries.  Most of it are comparisons: 12 steps over the scores in
+// registers.
 template <typename T, int NW, int NT>
 __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, int qtiles) {
   constexpr int WORDS = NT / 4;  // of a wave
@@ -921,9 +924,15 @@ __global__ __launch_bounds__(64 * NW) void block_score_wide_kernel(BlockArgs a, 
 // fragment of the second product -- and writes the block's result of each row with its maximum and sum; a second launch
 // joins a row's blocks.  Keys are read once per block and range of queries instead of once per query; the price is that every (row,
 // block) result passes through memory, which is what bounds the stage (2 (dv + 4) bytes written and read per row and block).
-// Measured, lists / blocks / join: 16384 queries, 8 heads over 2, 16 blocks of 64 9.5 / 106 / 57 us (17 GMAC: 330 TFLOP/s; 270 MB of block
-// results, read by the join at 4700 GB/s); 8 images x 1600 queries x 6 heads x 8 blocks 7 / 38 / 17 us.  The middle launch issues about 210
-// vector instructions to a tile of 16 rows x 64 keys beside 18 MFMAs, 16 of them exponentials at a quarter of the rate.
+// Measured, lists / blocks / join: 16384 queries, 8 heads over 2, 16 blocks of 64 9.5 / 106 / 60 us (17 GMAC: 330 TFLOP/s; 270 MB of block
+// results, read by the join at 4500 GB/s); 8 images x 1600 queries x 6 heads x 8 blocks 7 / 38 / 17 us.  The middle launch issues about 210
+// vector instructions to a tile of 16 rows x 64 keys beside 18 MFMAs, 16 of them exponentials at a quarter of the rate (57 % of the SIMDs'
+// cycles on the 128x128 map, the matrix pipe 15 %).  A tile of 16 neighbouring queries that read all the blocks any of them picked would
+// do 2-5 times the work: 16 neighbours pick 76 of 256 blocks together there, 34 of 100 on the 80x80 map, 16 and 8 each.
+//
+// The softmax weights are rounded to the tensors' type (2^-8 of bf16, 2^-11 of fp16 at most) because the matrix pipe takes both factors in
+// one type; their sum is that of the rounded ones.  With the block results below, the error against 64 bits is 2.2e-3 of the result in
+// bf16, where rounding once alone makes 1.7e-3.
 //
 // A block's results pass unnormalised (sum of p v; the maximum and sum of p beside them in fp32).  For fp16 tensors they are fp32.  For
 // bf16 tensors they are fp16 (off by 2^-11 at most, an eighth of a bf16 step; fp32 took 278 instead of 150 us on the 128x128 map):

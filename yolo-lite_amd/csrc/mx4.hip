@@ -243,7 +243,8 @@ struct Finish4 {
 // tiles would leave most of the chip idle.  A workgroup owns 16 WT weight rows x 16 XT rows of x; its NW waves take the k-steps in
 // turn, operands straight from memory into registers, and the partial sums meet in LDS in a fixed order.
 // X: what x is: codes (uint8_t), or the values themselves -- a lane's part of the operand is one row's block of 32, so each lane
-// quantises its own, without a launch, a workspace or an exchange (16 rows and weights of up to 2^24 elements: see plan_linear).
+// quantises its own, without a launch, a workspace or an exchange (16 rows and weights of up to 2^24 elements: see plan_linear).  Lanes of
+// rows that x does not have quantise the last one's block once more: 614 vector instructions of a wave for one row of 4096, most of them that.
 // Measured, one row: 4096 x 4096 values 8 us (cold caches 11), codes 5-6; 128000 x 4096 codes 63 us, 4400 GB/s.
 template <typename T, typename X, int WT, int XT, int NW>
 __global__ __launch_bounds__(64 * NW) void mx4_split_kernel(LinearArgs a) {

@@ -69,7 +69,8 @@ def _workspace(what: str, nbytes: int, like: torch.Tensor):
 def block_select(q: torch.Tensor, k: torch.Tensor, block: int = 64, topk: int = 8, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
     """For each query and kv head the ``topk`` blocks of ``block`` (32, 64 or 128) keys with the largest score, as int32
     (batch, kv heads, nq, topk): ascending block indices, -1 behind the last.  Score: (q summed over the kv head's query heads) .
-    (mean of the block's readable keys), in 64 bits; ties go to the lower index; a block without a readable key is never picked."""
+    (mean of the block's readable keys), in 64 bits; ties go to the lower index, a NaN score ranks with -inf; a block without a readable
+    key is never picked."""
     dev = on_gpu("block_select", q, k, mask)
     (batch, nq, heads, dk), nk, kv, mask, mask_at, mask_row = _check("block_select", q, k, mask, block, topk)
     L = _lib.lib()
