@@ -1,4 +1,4 @@
-"""CPU: sizes of the block-sparse attention whose launches the driver would not take are refused with the size of their workspace."""
+"""CPU: sizes of the block-sparse attention whose launches would have 2^32 threads and more are refused with the size of their workspace."""
 import pytest
 
 from tests.test_block_attention import BASE, _run

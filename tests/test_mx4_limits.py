@@ -28,7 +28,7 @@ def test_sizes_that_have_a_workspace(x_dtype, rows, n, k):
 
 @pytest.mark.parametrize("rows, cols", [(1 << 30, 1), (1 << 30, 32), ((1 << 29) + 1, 64), (1 << 14, 1 << 22), (1 << 34, 32)])
 def test_quantize_takes_fewer_than_2_to_the_30_blocks(rows, cols):
-    """Four threads to a block: the driver would take no launch of 2^32."""
+    """Four threads to a block: a launch of 2^32 would be cut off."""
     from yololite_amd import _lib
 
     L = _lib.lib()

@@ -1636,7 +1636,7 @@ static long long round256(long long n) { return (n + 255) / 256 * 256; }
 // a * b * c below 2^31 (factors below 2^31: a product in 64 bits could wrap around)
 static bool fits31(long long a, long long b, long long c) { return (double)a * (double)b * (double)c < 2147483648.0; }
 
-// the driver takes launches of fewer than 2^32 threads
+// A launch has fewer than 2^32 threads: a larger one is cut off, without an error.
 static bool fits_grid(long long workgroups, int threads) { return workgroups * threads < 1LL << 32; }
 
 static int check_heads(const std::string& who, const char* name, const yl_heads* t) {
@@ -1784,7 +1784,9 @@ static int select_run(BlockArgs& a, const SelectPlan& p, int dtype, char* w, hip
   return by_type16(dtype, [&](auto* t) {
     typedef BA_T(t) T;
     const bool few = a.nq <= SCORE_MAX_NQ;
-    if (few && a.nb <= SMALL_BLOCKS && std::min(a.block, a.nk) * a.dk <= SMALL_BLOCK) return mean_launch<T, true, true>(a, s);
+    if (few && a.nb <= SMALL_BLOCKS && std::min(a.block, a.nk) * a.dk <= SMALL_BLOCK &&
+        fits_grid((long long)a.batch * a.kv, 64 * std::max(SCORE_MAX_NQ, a.nb)))
+      return mean_launch<T, true, true>(a, s);
     if (a.nb > 0)
       if (int rc = few ? mean_launch<T, true>(a, s) : mean_launch<T, false>(a, s)) return rc;
     if (!few && a.nb > 0) return score_by_size<T>(a, s);

@@ -609,7 +609,7 @@ static int by_type(int dtype, F f) {
   return f((float*)nullptr);
 }
 
-// four threads to a block of 32; the driver takes fewer than 2^32 threads
+// four threads to a block of 32; a launch has fewer than 2^32 threads (a larger one is cut off, without an error)
 static int grid_of(const char* who, long long rows, int kb, unsigned* grid) {
   if (rows > (0xFFFFFF00LL / 4) / kb) return fail(-3, std::string(who) + ": more than 2^30 blocks of 32 columns in one call");
   *grid = (unsigned)((rows * 4 * kb + 255) / 256);
